@@ -162,6 +162,21 @@ _SIGNATURES = {
         _c_void_p, _c_void_p, _c_void_p,         # dots_out, score_out, idx_out
         _c_void_p,
     ]),
+    "halo_update_block_tables": (_i32, [_c_void_p, _i64, _c_void_p, _i32, _i32, _c_void_p, _i32, _c_void_p, _c_void_p,
+                                        _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "halo_append_rows": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _i32,
+                                _c_void_p]),
+    "halo_tree_layout": (_i32, [_c_void_p, _c_void_p, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p, _c_void_p]),
+    "halo_tree_workspace_size": (_size_t, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
+    "halo_tree_attn": (_i32, [
+        _c_void_p, _c_void_p, _i64, _i64, _i32, _i32,    # pool (halo_block_pool), q, strides, N, H
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32,  # table, stride, B, W, lengths, cu_nodes, max_nodes
+        _c_void_p, _i64, _f32,                           # mask, stride, scale
+        _c_void_p, _i64, _i64, _i32, _c_void_p,          # out, strides, out_dtype, lse
+        _c_void_p, _size_t, _c_void_p,                   # workspace, bytes, stream
+    ]),
+    "halo_commit_path": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
+                                _c_void_p, _c_void_p]),
     "halo_copy_blocks": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32, _i64,
                                 _c_void_p, _i32, _c_void_p]),
     "halo_set_tier": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _c_void_p]),

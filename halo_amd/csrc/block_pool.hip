@@ -1,0 +1,574 @@
+// Block-pool operators of batched decoding with drafted trees (gfx950): block
+// tables and slot maps from the requests' lengths, rows written to their
+// slots, ancestor masks of drafted trees, and the accepted path's rows moved
+// behind the committed ones.
+//
+// A pool is one tier buffer of the cold-KV store: K and V as (layers, blocks,
+// H_kv, block_size, D).  Row p of a request lies in row p % block_size of
+// block table[p / block_size]; slot = block * block_size + row names a row of
+// the pool.  The reference keeps such blocks (halo/memory_tier.py:45-60) but
+// gives them to no request; everything here is this library's own.
+#include "block_pool.hpp"
+
+namespace halo {
+namespace {
+
+// ---------------------------------------------------------------------------
+// Block tables and slots.  need_b = ceil(length_b / block_size); surplus
+// blocks go back first, then requests take theirs in order.  With R_b, G_b
+// and C_b the sums over b' < b of blocks given back, blocks taken and new rows,
+// every moved id and every slot has a place of its own:
+//   entry j of b goes to   free[n_free + R - R_{b+1} + own_b - 1 - j],
+//   entry j of b comes from free[n_free + R - 1 - (G_b + j - own_b)],
+//   new row r has           b = the last one with C_b <= r.
+// One workgroup, since the free list is one stack: it is bound by the chain
+// lengths -> sums -> ids -> slots, not by bytes.  The ids of a chunk of
+// requests are spread over the threads by a search in the chunk's sums, so one
+// long request does not hold up the others.
+// ---------------------------------------------------------------------------
+constexpr int kTabThreads = 1024;
+
+struct TableParams {
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* n_blocks;
+  int B, W;
+  int32_t* free_blocks;
+  int n_cap;
+  int32_t* n_free;
+  const int32_t* lengths;
+  const int32_t* first;
+  Div bs;
+  int max_rows;
+  int32_t* cu_rows;
+  int64_t* slots;
+  uint8_t* ok;
+};
+
+struct TabReq {
+  int own, need, first, len;  // blocks it has and needs, new rows [first, len)
+};
+__device__ __forceinline__ TabReq tab_req(const TableParams& P, int b) {
+  TabReq r = {0, 0, 0, 0};
+  if (b < P.B) {
+    r.len = max(P.lengths[b], 0);
+    r.first = max(P.first[b], 0);
+    r.own = min(max(P.n_blocks[b], 0), P.W);
+    r.need = div_by(r.len, P.bs);
+    if (r.need * P.bs.d < r.len) ++r.need;
+  }
+  return r;
+}
+
+// Exclusive sum over the workgroup's threads; `total` gets the whole sum.
+__device__ __forceinline__ int64_t tab_scan(int64_t v, int64_t* wave_sums, int64_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t x = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(x, off, 64);
+    if (lane >= off) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) wave_sums[wave] = x;
+  __syncthreads();
+  int64_t base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kTabThreads / 64; ++w) {
+    if (w < wave) base += wave_sums[w];
+    all += wave_sums[w];
+  }
+  total = all;
+  return base + x - v;
+}
+
+// The last i in [0, n) with at[i] <= x (at[0] <= x, ascending).
+template <typename T>
+__device__ __forceinline__ int tab_find(const T* at, int n, T x) {
+  int lo = 0, hi = n;  // at[lo] <= x < at[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Slot of new row r: -1 behind the last row and for rows of requests that were not served.
+__device__ __forceinline__ int64_t tab_slot(const TableParams& P, const int32_t* cu, int r) {
+  if (r >= cu[P.B]) return -1;
+  const int b = tab_find(cu, P.B, r);
+  if (!P.ok[b]) return -1;
+  const int p = max(P.first[b], 0) + (r - cu[b]);
+  const int c = div_by(p, P.bs);
+  return (int64_t)P.table[b * P.table_stride + c] * P.bs.d + (p - c * P.bs.d);
+}
+
+// SLOTS: also the slots, by the same workgroup.
+template <bool SLOTS>
+__global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams P) {
+  __shared__ int64_t wave_sums[kTabThreads / 64];
+  __shared__ int s_at[kTabThreads + 1], s_own[kTabThreads], s_cu[kTabThreads + 1];
+  const int tid = threadIdx.x;
+  const int nf = min(max(*P.n_free, 0), P.n_cap);
+
+  int64_t all_back = 0;
+  for (int b0 = 0; b0 < P.B; b0 += kTabThreads) {
+    const TabReq r = tab_req(P, b0 + tid);
+    int64_t t;
+    tab_scan(max(r.own - r.need, 0), wave_sums, t);
+    all_back += t;
+  }
+  // give back: the last request's last block lands lowest
+  int64_t before = 0;
+  for (int b0 = 0; all_back > 0 && b0 < P.B; b0 += kTabThreads) {
+    const TabReq r = tab_req(P, b0 + tid);
+    int64_t t;
+    const int64_t at = tab_scan(max(r.own - r.need, 0), wave_sums, t);
+    __syncthreads();
+    s_at[tid] = (int)at;
+    s_own[tid] = r.own;
+    if (tid == 0) s_at[kTabThreads] = (int)t;
+    __syncthreads();
+    for (int x = tid; x < (int)t; x += kTabThreads) {
+      const int i = tab_find(s_at, kTabThreads, x);
+      // x counts the chunk's entries in the order (request, entry from the first surplus one on)
+      int32_t* e = P.table + (int64_t)(b0 + i) * P.table_stride + s_own[i] - (s_at[i + 1] - x);
+      const int64_t to = nf + all_back - 1 - (before + x);
+      const int32_t id = *e;
+      *e = -1;
+      if (to < P.n_cap) P.free_blocks[to] = id;
+    }
+    before += t;
+  }
+  __syncthreads();
+
+  const int64_t avail = min(nf + all_back, (int64_t)P.n_cap);
+  int64_t taken_before = 0, rows_before = 0, taken = 0;
+  for (int b0 = 0; b0 < P.B; b0 += kTabThreads) {
+    const int b = b0 + tid;
+    const TabReq r = tab_req(P, b);
+    const bool fits = r.need <= P.W;
+    const int grow = fits ? max(r.need - r.own, 0) : 0;
+    int64_t t_grow, t_rows, t_take;
+    const int64_t g = taken_before + tab_scan(grow, wave_sums, t_grow);
+    const int64_t c = rows_before + tab_scan(max(r.len - r.first, 0), wave_sums, t_rows);
+    const bool ok = fits && (grow == 0 || g + grow <= avail);
+    // served requests that grow come before the others that do, so their own sums are G_b too
+    const int64_t at = tab_scan(ok ? grow : 0, wave_sums, t_take);
+    __syncthreads();
+    s_at[tid] = (int)at;
+    s_own[tid] = r.own;
+    if (tid == 0) s_at[kTabThreads] = (int)t_take;
+    if (b < P.B) {
+      const int32_t cu = (int32_t)min(c, (int64_t)0x7fffffff);
+      P.cu_rows[b] = cu;
+      s_cu[tid] = cu;
+      P.ok[b] = ok;
+      if (ok) P.n_blocks[b] = r.need;
+    }
+    __syncthreads();
+    for (int x = tid; x < (int)t_take; x += kTabThreads) {
+      const int i = tab_find(s_at, kTabThreads, x);
+      P.table[(int64_t)(b0 + i) * P.table_stride + s_own[i] + (x - s_at[i])] =
+          P.free_blocks[avail - 1 - (taken + x)];
+    }
+    taken_before += t_grow;
+    rows_before += t_rows;
+    taken += t_take;
+    __syncthreads();
+  }
+  const int32_t n_rows = (int32_t)min(rows_before, (int64_t)0x7fffffff);
+  if (tid == 0) {
+    P.cu_rows[P.B] = n_rows;
+    *P.n_free = (int32_t)(avail - taken);
+  }
+  if constexpr (SLOTS) {
+    if (tid == 0 && P.B <= kTabThreads) s_cu[P.B] = n_rows;
+    __syncthreads();
+    const int32_t* cu = P.B <= kTabThreads ? s_cu : P.cu_rows;
+    for (int r = tid; r < P.max_rows; r += kTabThreads) P.slots[r] = tab_slot(P, cu, r);
+  }
+}
+
+__global__ void __launch_bounds__(256) slots_kernel(TableParams P) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < P.max_rows) P.slots[r] = tab_slot(P, P.cu_rows, r);
+}
+
+// ---------------------------------------------------------------------------
+// Rows to their slots and along an accepted path: copies of whole rows, PB
+// bytes a thread (16 where everything is aligned for it).
+// ---------------------------------------------------------------------------
+struct PoolView {
+  char* k;
+  char* v;
+  int64_t sl, sb, sh, sr;  // strides in bytes
+  int layers, blocks, H_kv, D_bytes;
+  Div bs;
+};
+
+template <int PB>
+struct Piece;
+template <>
+struct Piece<16> {
+  typedef uint4 type;
+};
+template <>
+struct Piece<4> {
+  typedef uint32_t type;
+};
+template <>
+struct Piece<2> {
+  typedef uint16_t type;
+};
+
+struct AppendParams {
+  PoolView pool;
+  const char* k;
+  const char* v;
+  int64_t ksl, ksn, ksh, vsl, vsn, vsh;  // strides of the new rows in bytes
+  const int64_t* slots;
+  int N;
+};
+
+constexpr int kAppThreads = 256;
+constexpr int kAppUnroll = 4;  // rows a thread has in flight
+
+template <int PB>
+__global__ void __launch_bounds__(kAppThreads) append_rows_kernel(AppendParams P) {
+  typedef typename Piece<PB>::type T;
+  const int per_head = P.pool.D_bytes / PB;
+  const int per_row = P.pool.H_kv * per_head;
+  const int cols = min(per_row, kAppThreads);
+  const int at_once = kAppThreads / cols;  // rows of one step
+  const int row_in = threadIdx.x / cols;
+  if (row_in >= at_once) return;
+  const int layer = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const char* src = is_v ? P.v + layer * P.vsl : P.k + layer * P.ksl;
+  char* dst = (is_v ? P.pool.v : P.pool.k) + layer * P.pool.sl;
+  const int64_t sn = is_v ? P.vsn : P.ksn, sh = is_v ? P.vsh : P.ksh;
+  const int64_t n_slots = (int64_t)P.pool.blocks * P.pool.bs.d;
+  const int row0 = blockIdx.x * (at_once * kAppUnroll) + row_in;
+  int64_t to[kAppUnroll];
+#pragma unroll
+  for (int u = 0; u < kAppUnroll; ++u) {
+    const int r = row0 + u * at_once;
+    const int64_t slot = r < P.N ? P.slots[r] : -1;
+    to[u] = -1;
+    if (slot >= 0 && slot < n_slots) {
+      const int blk = div_by((int)slot, P.pool.bs);
+      to[u] = blk * P.pool.sb + (slot - (int64_t)blk * P.pool.bs.d) * P.pool.sr;
+    }
+  }
+  for (int c = threadIdx.x - row_in * cols; c < per_row; c += cols) {
+    const int h = c / per_head, x = (c - h * per_head) * PB;
+    T v[kAppUnroll];
+#pragma unroll
+    for (int u = 0; u < kAppUnroll; ++u)
+      if (to[u] >= 0) v[u] = *reinterpret_cast<const T*>(src + (int64_t)(row0 + u * at_once) * sn + h * sh + x);
+#pragma unroll
+    for (int u = 0; u < kAppUnroll; ++u)
+      if (to[u] >= 0) *reinterpret_cast<T*>(dst + to[u] + h * P.pool.sh + x) = v[u];
+  }
+}
+
+struct CommitParams {
+  PoolView pool;
+  const int32_t* table;
+  int64_t table_stride;
+  int W;
+  const int32_t* lengths;
+  const int32_t* path;
+  int64_t path_stride;
+  int n_path_max;
+  const int32_t* n_path;
+  int32_t* new_lengths;
+};
+
+constexpr int kMaxPath = 64;
+constexpr int kCommitThreads = 256;
+
+// Byte offset of row p of a request in a layer of the pool, or -1.
+__device__ __forceinline__ int64_t row_offset(const PoolView& pool, const int32_t* table, int W, int64_t p) {
+  if (p < 0 || p > 0x7fffffff) return -1;
+  const int c = div_by((int)p, pool.bs);
+  if (c >= W) return -1;
+  const int blk = table[c];
+  if (blk < 0 || blk >= pool.blocks) return -1;
+  return blk * pool.sb + (p - (int64_t)c * pool.bs.d) * pool.sr;
+}
+
+// Row length + j of request b receives what row length + path[j] held.  A
+// path rises, so path[j] >= j and a row is written only after every move that
+// reads it: a thread takes one column of all rows in order and needs no other.
+// Lane j of each wave finds move j; the path ends at the first entry that does
+// not rise or whose rows the table does not hold.
+template <int PB>
+__global__ void __launch_bounds__(kCommitThreads) commit_path_kernel(CommitParams P) {
+  typedef typename Piece<PB>::type T;
+  const int b = blockIdx.y;
+  const int lane = threadIdx.x & 63;
+  const int len = max(P.lengths[b], 0);
+  const int np = min(max(P.n_path[b], 0), P.n_path_max);
+  int64_t from = -1, to = -1;
+  bool good = false;
+  {
+    const int32_t* path = P.path + b * P.path_stride;
+    const int at = lane < np ? path[lane] : -1;
+    const int last = __shfl_up(at, 1, 64);
+    if (lane < np) {
+      from = row_offset(P.pool, P.table + b * P.table_stride, P.W, (int64_t)len + at);
+      to = row_offset(P.pool, P.table + b * P.table_stride, P.W, (int64_t)len + lane);
+      good = at > (lane == 0 ? -1 : last) && from >= 0 && to >= 0;
+    }
+  }
+  const uint64_t bad = ~__ballot(good);
+  const int n = bad == 0 ? 64 : __builtin_ctzll(bad);
+  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) P.new_lengths[b] = len + n;
+
+  const int per_head = P.pool.D_bytes / PB;
+  const int per_layer = P.pool.H_kv * per_head;
+  const int64_t x = (int64_t)blockIdx.x * kCommitThreads + threadIdx.x;
+  const int layer = (int)(x / per_layer);
+  const int c = (int)(x - (int64_t)layer * per_layer);
+  const int h = c / per_head;
+  const bool live = layer < P.pool.layers;
+  char* col = (blockIdx.z != 0 ? P.pool.v : P.pool.k) + layer * P.pool.sl + h * P.pool.sh + (c - h * per_head) * PB;
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < n; j0 += U) {
+    T v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t f = __shfl(from, (j0 + u) & 63, 64);
+      if (live && j0 + u < n) v[u] = *reinterpret_cast<const T*>(col + f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t f = __shfl(from, (j0 + u) & 63, 64), t = __shfl(to, (j0 + u) & 63, 64);
+      if (live && j0 + u < n && f != t) *reinterpret_cast<T*>(col + t) = v[u];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Ancestor masks.  With M_i the set of node i and its ancestors at most s - 1
+// steps up and a_i the ancestor s steps up, M_i | M_{a_i} reaches 2 s - 1
+// steps: log2(depth) rounds, one workgroup per tree, the sets in LDS.
+// ---------------------------------------------------------------------------
+constexpr int kMaxNodes = 512;
+constexpr int kTreeThreads = 256;
+
+template <int WORDS>
+__global__ void __launch_bounds__(kTreeThreads)
+    tree_layout_kernel(const int32_t* parents, const int32_t* cu, int N, int max_nodes, int words, uint64_t* mask,
+                       int64_t mask_stride, int32_t* depth) {
+  constexpr int NODES = WORDS * 64;
+  constexpr int PER = (NODES + kTreeThreads - 1) / kTreeThreads;  // nodes a thread
+  __shared__ uint64_t s_bits[NODES][WORDS];
+  __shared__ int s_up[NODES];
+  const int lo = max(cu[blockIdx.x], 0);
+  const int n = min(min(cu[blockIdx.x + 1], N) - lo, max_nodes);
+  if (n <= 0) return;
+  uint64_t bits[PER][WORDS];
+  int up[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = threadIdx.x + k * kTreeThreads;
+    up[k] = -1;
+    if (i < n) {
+      const int p = parents[lo + i];
+      up[k] = p >= 0 && p < i ? p : -1;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        bits[k][w] = (i >> 6) == w ? 1ull << (i & 63) : 0;
+        s_bits[i][w] = bits[k][w];
+      }
+      s_up[i] = up[k];
+    }
+  }
+  bool more = false;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) more |= up[k] >= 0;
+  while (__syncthreads_or(more)) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (up[k] >= 0) {
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) bits[k][w] |= s_bits[up[k]][w];
+        up[k] = s_up[up[k]];
+      }
+    __syncthreads();
+    more = false;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = threadIdx.x + k * kTreeThreads;
+      if (i < n) {
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) s_bits[i][w] = bits[k][w];
+        s_up[i] = up[k];
+      }
+      more |= up[k] >= 0;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = threadIdx.x + k * kTreeThreads;
+    if (i < n) {
+      int ones = 0;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        if (w < words) mask[(int64_t)(lo + i) * mask_stride + w] = bits[k][w];
+        ones += __popcll(bits[k][w]);
+      }
+      depth[lo + i] = ones - 1;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace halo
+
+using namespace halo;
+
+namespace {
+
+int check_pool(const halo_block_pool* pool, PoolView* out) {
+  HALO_CHECK_ARG(pool && pool->k && pool->v, "null pool");
+  HALO_CHECK_ARG(pool->dtype == HALO_F32 || pool->dtype == HALO_BF16 || pool->dtype == HALO_F16, "bad pool dtype");
+  HALO_CHECK_ARG(pool->layers > 0 && pool->blocks > 0 && pool->H_kv > 0 && pool->block_size > 0 && pool->D > 0,
+                 "pool sizes must be positive");
+  HALO_CHECK_ARG((int64_t)pool->blocks * pool->block_size < (1ll << 31), "a pool holds at most 2^31 - 1 rows");
+  const int64_t es = elem_size(pool->dtype);
+  out->k = static_cast<char*>(pool->k);
+  out->v = static_cast<char*>(pool->v);
+  out->sl = pool->stride_l * es;
+  out->sb = pool->stride_b * es;
+  out->sh = pool->stride_h * es;
+  out->sr = pool->stride_r * es;
+  out->layers = pool->layers;
+  out->blocks = pool->blocks;
+  out->H_kv = pool->H_kv;
+  out->D_bytes = (int)(pool->D * es);
+  out->bs = make_div(pool->block_size);
+  return HALO_OK;
+}
+
+// The widest piece that every row start is a multiple of.
+int piece_bytes(const PoolView& p, uint64_t more) {
+  const uint64_t all = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | (uint64_t)p.sl |
+                       (uint64_t)p.sb | (uint64_t)p.sh | (uint64_t)p.sr | (uint64_t)p.D_bytes | more;
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
+}
+
+}  // namespace
+
+extern "C" int halo_update_block_tables(int32_t* table, int64_t table_stride, int32_t* n_blocks, int B, int W,
+                                        int32_t* free_blocks, int n_cap, int32_t* n_free, const int32_t* lengths,
+                                        const int32_t* first, int block_size, int max_rows, int32_t* cu_rows,
+                                        int64_t* slots, uint8_t* ok, void* stream) {
+  HALO_CHECK_ARG(table && n_blocks && free_blocks && n_free && lengths && first && cu_rows && ok,
+                 "null pointer argument");
+  HALO_CHECK_ARG(B > 0 && W > 0 && n_cap >= 0 && block_size > 0 && max_rows >= 0 && (max_rows == 0 || slots),
+                 "bad sizes");
+  HALO_CHECK_ARG(table_stride >= W && (int64_t)B * W < (1ll << 31) && (int64_t)W * block_size < (1ll << 31),
+                 "table too large, or its rows overlap");
+  TableParams p = {table, table_stride, n_blocks, B, W, free_blocks, n_cap, n_free, lengths, first,
+                   make_div(block_size), max_rows, cu_rows, slots, ok};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // up to 4 slots a thread of the one workgroup cost less than a second launch
+  const bool here = max_rows <= 4 * kTabThreads;
+  if (here) hipLaunchKernelGGL(update_tables_kernel<true>, dim3(1), dim3(kTabThreads), 0, st, p);
+  else {
+    hipLaunchKernelGGL(update_tables_kernel<false>, dim3(1), dim3(kTabThreads), 0, st, p);
+    hipLaunchKernelGGL(slots_kernel, dim3((unsigned)((max_rows + 255) / 256)), dim3(256), 0, st, p);
+  }
+  HALO_CHECK_HIP(hipGetLastError());
+  return HALO_OK;
+}
+
+extern "C" int halo_append_rows(const halo_block_pool* pool, const void* k, int64_t k_stride_l, int64_t k_stride_n,
+                                int64_t k_stride_h, const void* v, int64_t v_stride_l, int64_t v_stride_n,
+                                int64_t v_stride_h, const int64_t* slots, int N, void* stream) {
+  AppendParams p;
+  const int rc = check_pool(pool, &p.pool);
+  if (rc != HALO_OK) return rc;
+  HALO_CHECK_ARG(N >= 0 && (N == 0 || (k && v && slots)), "null pointer argument");
+  HALO_CHECK_ARG(pool->layers <= 65535, "at most 65535 layers");
+  if (N == 0) return HALO_OK;
+  const int64_t es = elem_size(pool->dtype);
+  p.k = static_cast<const char*>(k);
+  p.v = static_cast<const char*>(v);
+  p.ksl = k_stride_l * es;
+  p.ksn = k_stride_n * es;
+  p.ksh = k_stride_h * es;
+  p.vsl = v_stride_l * es;
+  p.vsn = v_stride_n * es;
+  p.vsh = v_stride_h * es;
+  p.slots = slots;
+  p.N = N;
+  const int pb = piece_bytes(p.pool, reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                                         (uint64_t)(p.ksl | p.ksn | p.ksh | p.vsl | p.vsn | p.vsh));
+  const int per_row = p.pool.H_kv * (p.pool.D_bytes / pb);
+  const int rows = kAppThreads / (per_row < kAppThreads ? per_row : kAppThreads) * kAppUnroll;
+  const dim3 grid((unsigned)((N + rows - 1) / rows), (unsigned)pool->layers, 2), block(kAppThreads);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (pb == 16) hipLaunchKernelGGL(append_rows_kernel<16>, grid, block, 0, st, p);
+  else if (pb == 4) hipLaunchKernelGGL(append_rows_kernel<4>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(append_rows_kernel<2>, grid, block, 0, st, p);
+  HALO_CHECK_HIP(hipGetLastError());
+  return HALO_OK;
+}
+
+extern "C" int halo_commit_path(const halo_block_pool* pool, const int32_t* table, int64_t table_stride, int B, int W,
+                                const int32_t* lengths, const int32_t* path, int64_t path_stride, int n_path_max,
+                                const int32_t* n_path, int32_t* new_lengths, void* stream) {
+  CommitParams p;
+  const int rc = check_pool(pool, &p.pool);
+  if (rc != HALO_OK) return rc;
+  HALO_CHECK_ARG(table && lengths && path && n_path && new_lengths, "null pointer argument");
+  HALO_CHECK_ARG(B > 0 && B <= 65535 && W > 0 && n_path_max > 0 && n_path_max <= kMaxPath,
+                 "need 1 <= B <= 65535 and paths of at most 64 entries");
+  HALO_CHECK_ARG(new_lengths != lengths, "new_lengths must not be lengths: other workgroups still read them");
+  p.table = table;
+  p.table_stride = table_stride;
+  p.W = W;
+  p.lengths = lengths;
+  p.path = path;
+  p.path_stride = path_stride;
+  p.n_path_max = n_path_max;
+  p.n_path = n_path;
+  p.new_lengths = new_lengths;
+  const int pb = piece_bytes(p.pool, 0);
+  const int64_t cols = (int64_t)pool->layers * pool->H_kv * (p.pool.D_bytes / pb);
+  HALO_CHECK_ARG(cols < (1ll << 31), "rows of all layers too long");
+  const dim3 grid((unsigned)((cols + kCommitThreads - 1) / kCommitThreads), (unsigned)B, 2), block(kCommitThreads);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (pb == 16) hipLaunchKernelGGL(commit_path_kernel<16>, grid, block, 0, st, p);
+  else if (pb == 4) hipLaunchKernelGGL(commit_path_kernel<4>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(commit_path_kernel<2>, grid, block, 0, st, p);
+  HALO_CHECK_HIP(hipGetLastError());
+  return HALO_OK;
+}
+
+extern "C" int halo_tree_layout(const int32_t* parents, const int32_t* cu_nodes, int B, int N, int max_nodes,
+                                int64_t* mask, int64_t mask_stride, int32_t* depth, void* stream) {
+  HALO_CHECK_ARG(parents && cu_nodes && mask && depth, "null pointer argument");
+  HALO_CHECK_ARG(B > 0 && N > 0 && max_nodes > 0 && max_nodes <= kMaxNodes, "need 1 <= max_nodes <= 512");
+  const int words = (max_nodes + 63) / 64;
+  HALO_CHECK_ARG(mask_stride >= words, "mask rows overlap");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  uint64_t* m = reinterpret_cast<uint64_t*>(mask);
+  const dim3 grid((unsigned)B), block(kTreeThreads);
+#define HALO_LAYOUT(WV) \
+  hipLaunchKernelGGL(tree_layout_kernel<WV>, grid, block, 0, st, parents, cu_nodes, N, max_nodes, words, m, \
+                     mask_stride, depth)
+  if (words == 1) HALO_LAYOUT(1);
+  else if (words == 2) HALO_LAYOUT(2);
+  else if (words <= 4) HALO_LAYOUT(4);
+  else HALO_LAYOUT(8);
+#undef HALO_LAYOUT
+  HALO_CHECK_HIP(hipGetLastError());
+  return HALO_OK;
+}

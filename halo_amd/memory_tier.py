@@ -305,6 +305,16 @@ class TieredStorage:
     def block_bytes(self) -> int:
         return self.num_kv_heads * self.block_size * self.head_dim * torch.tensor([], dtype=self.dtype).element_size()
 
+    def pool(self, tier="gpu", layer: Optional[int] = None):
+        """K and V of a memory tier as a block pool, (L, max_blocks, H_kv,
+        block_size, D) or one layer's (max_blocks, H_kv, block_size, D): what
+        ``halo_amd.append_rows``, ``tree_attention`` and ``commit_path`` take."""
+        t = MemoryTier.from_name(tier)
+        if t is MemoryTier.NVME:
+            raise ValueError("the NVMe tier is a file, not a pool")
+        buf = self._buffer(t)
+        return (buf.keys, buf.values) if layer is None else (buf.keys[layer], buf.values[layer])
+
     # ----------------------------------------------------------- single blocks
     def move_block(self, *, layer: int, block: int, src, dst) -> None:
         s, d = MemoryTier.from_name(src), MemoryTier.from_name(dst)

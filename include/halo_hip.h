@@ -502,6 +502,107 @@ int halo_decode_attn_kivi(const void* q, int64_t q_stride_b, int64_t q_stride_h,
                           void* out, int out_dtype, float* lse,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- block pools: tables, drafted trees, accepted paths ------------------ */
+
+/*
+ * K and V of a tier of the cold-KV store as a pool of blocks: row r of head h
+ * of block b of layer l at k + l*stride_l + b*stride_b + h*stride_h +
+ * r*stride_r (elements; v alike, with the same strides), D elements side by
+ * side.  slot = b * block_size + r names a row of a layer; row p of a request
+ * is row p % block_size of block table[p / block_size] of its block table.
+ * Blocks and rows of one layer number below 2^31.  The layout is TieredStorage's (halo/memory_tier.py:45-60),
+ * which gives no blocks to requests; the operators below have no counterpart
+ * in the reference.
+ */
+typedef struct halo_block_pool {
+  void* k;
+  void* v;
+  int64_t stride_l, stride_b, stride_h, stride_r; /* elements */
+  int32_t layers, blocks, H_kv, block_size, D, dtype;
+} halo_block_pool; /* 72 bytes */
+
+/*
+ * Block tables, free list and slots from the requests' lengths.  Afterwards
+ * request b owns need_b = ceil(lengths[b] / block_size) blocks, in order:
+ *   1. give back: for b = B-1 .. 0 and j = n_blocks[b]-1 .. need_b, table[b][j]
+ *      is pushed on the free list and becomes -1;
+ *   2. take: for b = 0 .. B-1 and j = n_blocks[b] .. need_b-1, table[b][j] is
+ *      popped.  A request is served (ok[b] = 1) iff need_b <= W and it takes
+ *      none, or the free list covers what it and the requests before it (those
+ *      with need_b <= W) take; the others keep what they have (ok[b] = 0);
+ *   3. the new rows first[b] .. lengths[b]-1 of all requests are numbered one
+ *      after the other, cu_rows[b] .. cu_rows[b+1]-1, and slots[i] is the slot
+ *      of new row i < max_rows; -1 for rows of requests that were not served
+ *      and behind the last row.
+ * table (B, W) rows table_stride apart, n_blocks (B), free_blocks[0 .. *n_free)
+ * the stack of free blocks in a buffer of n_cap entries (ids pushed past it
+ * are dropped), all changed in place; lengths and first below 0 count as 0.
+ * cu_rows (B+1), slots (max_rows), ok (B) are written whole.  One launch, or
+ * two where there are many slots.
+ */
+int halo_update_block_tables(int32_t* table, int64_t table_stride, int32_t* n_blocks, int B, int W,
+                             int32_t* free_blocks, int n_cap, int32_t* n_free, const int32_t* lengths,
+                             const int32_t* first, int block_size, int max_rows, int32_t* cu_rows,
+                             int64_t* slots, uint8_t* ok, void* stream);
+
+/*
+ * New rows to their slots: row i of k and v (layers, N, H_kv, D; element
+ * strides) is copied to slot slots[i] of every layer of the pool.  Slots
+ * outside [0, blocks * block_size) are skipped.  Slots must differ: of rows
+ * with the same slot any may be kept, piece by piece.
+ */
+int halo_append_rows(const halo_block_pool* pool, const void* k, int64_t k_stride_l, int64_t k_stride_n,
+                     int64_t k_stride_h, const void* v, int64_t v_stride_l, int64_t v_stride_n, int64_t v_stride_h,
+                     const int64_t* slots, int N, void* stream);
+
+/*
+ * Ancestor masks of drafted trees.  Nodes cu_nodes[b] .. cu_nodes[b+1]-1 (at
+ * most N, and the first max_nodes of them, max_nodes <= 512) are request b's
+ * tree; parents[i] is a node's parent counted within its tree, anything but an
+ * earlier node makes it a root.  Bit j % 64 of word j / 64 of mask row i
+ * (ceil(max_nodes / 64) words, rows mask_stride words apart) is set iff j is
+ * node i itself or one of its ancestors; depth[i] is the number of ancestors.
+ * Rows of no tree are left as they are.
+ */
+int halo_tree_layout(const int32_t* parents, const int32_t* cu_nodes, int B, int N, int max_nodes, int64_t* mask,
+                     int64_t mask_stride, int32_t* depth, void* stream);
+
+/*
+ * Attention of drafted trees over a paged cache.  Node i of request b is row
+ * cu_nodes[b] + i of q and out (N, H, D; element strides, q rows 16-byte
+ * aligned) and of lse (N, H fp32, or NULL); it attends the request's rows
+ * [0, lengths[b]) and the tree rows lengths[b] + j whose bit j is set in its
+ * mask row (see halo_tree_layout; NULL: j <= i), each of the request's K/V
+ * rows through its block table (B, W; rows table_stride apart).  Rows in a
+ * block outside [0, blocks) or past the table are not attended; what a node
+ * does not attend has no part in its output, NaN and infinities included; a
+ * node that attends nothing gets out 0 and lse -inf.  Nodes past the first
+ * max_nodes of a request, rows of no request and their outputs are left out.
+ * scale > 0.  The pool has one layer, rows 16-byte aligned, at most 64 GiB of
+ * K; D in {64, 128}; H a multiple of H_kv.  workspace: 16-byte aligned, at
+ * least halo_tree_workspace_size(max_rows = W * block_size) bytes; calls that
+ * may overlap need their own.  Results do not depend on the batch's order in
+ * time: partials are merged in a fixed order.
+ */
+size_t halo_tree_workspace_size(int dtype, int B, int H, int H_kv, int D, int64_t max_rows, int max_nodes);
+int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int N, int H,
+                   const int32_t* table, int64_t table_stride, int B, int W, const int32_t* lengths,
+                   const int32_t* cu_nodes, int max_nodes, const int64_t* mask, int64_t mask_stride, float scale,
+                   void* out, int64_t out_stride_n, int64_t out_stride_h, int out_dtype, float* lse, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
+ * The accepted path of each request's tree becomes its next committed rows:
+ * row lengths[b] + j receives, in every layer, what row lengths[b] + path[b][j]
+ * held, for the j < n_path[b] (<= n_path_max <= 64) in front of the first entry
+ * that is not above the one before it or whose rows the table does not hold;
+ * new_lengths[b] = lengths[b] + their number (lengths below 0 count as 0).
+ * Nothing else of the pool changes.  new_lengths must not be lengths.
+ */
+int halo_commit_path(const halo_block_pool* pool, const int32_t* table, int64_t table_stride, int B, int W,
+                     const int32_t* lengths, const int32_t* path, int64_t path_stride, int n_path_max,
+                     const int32_t* n_path, int32_t* new_lengths, void* stream);
+
 /* ---- tier block moves -------------------------------------------------- */
 
 /*

@@ -24,6 +24,10 @@ Modules and what pins them (checks live in ``tests/test_oracle.py``):
                 with per-operation rounding in the storage dtype.  Pinned by
                 the reference test's error bound, exhaustive code round trips
                 and hand-computed cases at rounding boundaries.
+  paged      -- block tables, drafted trees and attention over a paged cache
+                (no counterpart in the reference), step by step in float64.
+                Pinned by hand-worked tables, closed forms and the dense
+                attention of ``attention``.
   inputs     -- seeded synthetic inputs for the five benchmark workloads.
   torch_path -- the reference's CPU torch op sequence, used only to time the
                 CPU baseline beside the GPU path.
