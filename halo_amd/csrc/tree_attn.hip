@@ -15,9 +15,8 @@
 // Work.  The query heads of a KV head and the nodes are flattened, row
 // r = (node r / rep, head r % rep); a unit is (request, KV head, block of
 // rows), so each K/V row is read once for all the heads and nodes of a block.
-// A request's key tiles are its committed rows in steps of KT from row 0 and
-// its tree rows in steps of KT from row length_b, so a tree tile meets whole
-// words of the masks.  The lengths are on the device only: every workgroup
+// A request's key tiles are its rows, committed ones and then the tree's, in
+// steps of KT from row 0.  The lengths are on the device only: every workgroup
 // sums the units' tiles, takes the share L = total / workgroups that fit the
 // GPU, and finds its item, one of ceil(tiles / L) even cuts of a unit; a
 // second launch merges the partials of the units that were cut.  The host
@@ -70,7 +69,7 @@ __device__ __forceinline__ TreeReq tree_req(const TreeParams& P, int b) {
     r.n = max(min(min(P.cu[b + 1], P.N) - r.lo, P.max_nodes), 0);
     r.ctx = min(max(P.lengths[b], 0), P.W * P.bs.d);
     r.rbs = (r.n * P.rep + R - 1) / R;
-    if (r.n > 0) r.tiles = (r.ctx + KT - 1) / KT + (r.n + KT - 1) / KT;
+    if (r.n > 0) r.tiles = (r.ctx + r.n + KT - 1) / KT;
   }
   return r;
 }
@@ -79,8 +78,30 @@ __device__ __forceinline__ TreeReq tree_req(const TreeParams& P, int b) {
 struct TreeItem {
   int b, lo, ctx, n, rbs, tiles;
   int h, rb, cut, cuts;  // the cut-th of `cuts` cuts of the unit (h, rb)
-  int64_t part;          // partial of the unit's first cut
+  int part;              // partial of the unit's first cut
 };
+
+// Inclusive sums over the 64 lanes, in registers.
+template <typename T, int CTRL, int ROWS>
+__device__ __forceinline__ T tree_dpp(T v) {
+  static_assert(sizeof(T) == 4, "one register");
+  return __builtin_bit_cast(
+      T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+template <typename T>
+__device__ __forceinline__ T wave_prefix(T v) {
+  v += tree_dpp<T, 0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += tree_dpp<T, 0x112, 0xf>(v);
+  v += tree_dpp<T, 0x114, 0xf>(v);
+  v += tree_dpp<T, 0x118, 0xf>(v);
+  v += tree_dpp<T, 0x142, 0xa>(v);  // lane 15 of each row to the row behind it
+  v += tree_dpp<T, 0x143, 0xc>(v);  // lane 31 to the upper half
+  return v;
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
 
 // Every lane returns the same; false past the last item.  ITEMS: x counts
 // items (head, cut, row block; the row blocks that read the same rows side by
@@ -89,99 +110,110 @@ template <int KT, int R, bool ITEMS>
 __device__ __forceinline__ bool tree_find(const TreeParams& P, int x, TreeItem& it) {
   const int lane = threadIdx.x & 63;
   const TreeReq r0 = tree_req<KT, R>(P, lane);
-  int64_t total = 0;
+  float total = 0.f;
   int units = 0;
   for (int b0 = 0; b0 < P.B; b0 += 64) {
     const TreeReq r = b0 == 0 ? r0 : tree_req<KT, R>(P, b0 + lane);
-    int u = P.H_kv * r.rbs;
-    int64_t t = (int64_t)u * r.tiles;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      u += __shfl_xor(u, off, 64);
-      t += __shfl_xor(t, off, 64);
-    }
-    units += u;
-    total += t;
+    const int u = P.H_kv * r.rbs;
+    units += lane_of(wave_prefix(u), 63);
+    total += lane_of(wave_prefix((float)u * (float)r.tiles), 63);
   }
-  // sum of ceil(tiles / L) <= total / L + units: a share that fills the GPU once if the units leave room
+  // sum of ceil(tiles / L) <= total / L + units: a share that fills the GPU
+  // once if the units leave room.  The sum has a relative error below 2^-16
+  // (B / 64 + 8 roundings of 2^-24), which the factor covers.
   const int room = P.slots > 2 * units ? P.slots - units : P.slots / 2;
-  const int L = max(P.min_tiles, (int)min((total + room - 1) / room, (int64_t)0x7fffffff));
-  int base = 0;
-  int64_t part = 0;
+  const int L = max(P.min_tiles, (int)fminf(ceilf(total * (1.f + 0x1p-14f) / (float)room), 1e9f));
+  int base = 0, part = 0;
   for (int b0 = 0; b0 < P.B; b0 += 64) {
     const TreeReq r = b0 == 0 ? r0 : tree_req<KT, R>(P, b0 + lane);
-    const int cuts = (int)(((int64_t)r.tiles + L - 1) / L);
+    const int cuts = (int)(((uint32_t)r.tiles + (uint32_t)L - 1) / (uint32_t)L);
     const int u = P.H_kv * r.rbs;
     const int mine = ITEMS ? u * cuts : u;
-    int at = mine;
-    int64_t parts = cuts > 1 ? (int64_t)u * cuts : 0;
-    const int64_t own = parts;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int y = __shfl_up(at, off, 64);
-      const int64_t z = __shfl_up(parts, off, 64);
-      if (lane >= off) {
-        at += y;
-        parts += z;
-      }
-    }
+    const int parts = cuts > 1 ? u * cuts : 0;
+    const int at = wave_prefix(mine), parts_at = wave_prefix(parts);
     const uint64_t past = __ballot(base + at > x);
     if (past != 0) {
       const int w = __builtin_ctzll(past);
-      const int first = uni(base + __shfl(at - mine, w, 64));
       it.b = b0 + w;
-      it.lo = uni(__shfl(r.lo, w, 64));
-      it.ctx = uni(__shfl(r.ctx, w, 64));
-      it.n = uni(__shfl(r.n, w, 64));
-      it.rbs = uni(__shfl(r.rbs, w, 64));
-      it.tiles = uni(__shfl(r.tiles, w, 64));
-      it.cuts = uni(__shfl(cuts, w, 64));
-      part = uni64(part + __shfl(parts - own, w, 64));
-      const int y = x - first;
+      it.lo = lane_of(r.lo, w);
+      it.ctx = lane_of(r.ctx, w);
+      it.n = lane_of(r.n, w);
+      it.rbs = lane_of(r.rbs, w);
+      it.tiles = lane_of(r.tiles, w);
+      it.cuts = lane_of(cuts, w);
+      uint32_t y = (uint32_t)(x - (base + lane_of(at, w) - lane_of(mine, w)));
       it.cut = 0;
+      it.rb = 0;
       if constexpr (ITEMS) {
-        it.rb = y % it.rbs;
-        it.cut = (y / it.rbs) % it.cuts;
-        it.h = y / it.rbs / it.cuts;
+        if (it.rbs > 1) {
+          it.rb = y % (uint32_t)it.rbs;
+          y /= (uint32_t)it.rbs;
+        }
+        if (it.cuts > 1) {
+          it.cut = y % (uint32_t)it.cuts;
+          y /= (uint32_t)it.cuts;
+        }
+        it.h = y;
       } else {
-        it.h = y % P.H_kv;
-        it.rb = y / P.H_kv;
+        it.h = y % (uint32_t)P.H_kv;
+        it.rb = y / (uint32_t)P.H_kv;
       }
-      it.part = part + (int64_t)(it.rb * P.H_kv + it.h) * it.cuts;
+      it.part = part + lane_of(parts_at, w) - lane_of(parts, w) + (it.rb * P.H_kv + it.h) * it.cuts;
       return true;
     }
-    base += uni(__shfl(at, 63, 64));
-    part += uni64(__shfl(parts, 63, 64));
+    base += lane_of(at, 63);
+    part += lane_of(parts_at, 63);
   }
   return false;
 }
 
-// Where row `key` of key tile `t` lies in the pool, in 16-byte pieces from the
-// start of head 0, or kNoRow: behind the committed rows, behind the tree, past
-// the table, or in a block that is not in the pool (a table entry outside
-// [0, blocks): its rows are not attended).  In two steps, so that the table
-// read can be in flight while other tiles are computed.
+// Staging.  An LDS-DMA instruction fills 1 KiB, lane l its piece l, so RPI rows
+// of RB bytes; NJ instructions of a wave fill KEYS rows.  Row key(lane, j) is
+// the one that lane reads for instruction j: a lane's rows lie side by side (or
+// every other one), so where a block holds them all, one look at the block
+// table is enough.  At RB = 128 two rows share the 64 banks; there the parity
+// of the LDS row is kept that of the key.  Both swizzles (which 16-byte piece
+// of a row lies where) go by the key and put every read pass on distinct banks.
 constexpr uint32_t kNoRow = 0xffffffffu;
-template <int KT>
+template <int RB, int NJ>
+struct TreeLanes {
+  static constexpr int SL = RB / 16, RPI = 64 / SL, KEYS = NJ * RPI;
+  static constexpr int STEP = RB == 128 ? 2 : 1;  // keys from one instruction to the next
+  static constexpr int SPAN = NJ * STEP;          // keys, aligned to their number, that a lane's rows lie in
+  __device__ static __forceinline__ int first(int lane) {
+    const int g = lane / SL;
+    return RB == 128 ? SPAN * (g >> 1) + (g & 1) : SPAN * g;
+  }
+  __host__ __device__ static constexpr int lds_row(int key) {  // key < KEYS
+    return RB == 128 ? ((key >> 1) % NJ) * RPI + 2 * (key / SPAN) + (key & 1) : (key % NJ) * RPI + key / NJ;
+  }
+};
+template <int RB>
+__device__ __forceinline__ int tree_kswz(int key) {
+  return RB == 128 ? (key >> 1) & 7 : key & 15;
+}
+template <int RB>
+__device__ __forceinline__ int tree_vswz(int key) {
+  return RB == 128 ? 2 * ((key >> 1) & 1) : 2 * (key & 3);
+}
+
+// The table entry of position `pos` (-1 past the request's rows or the table), and its row in the block.
 struct TreeRow {
   int blk, in_blk;
-  __device__ __forceinline__ void load(const TreeParams& P, const TreeItem& it, int t, int key) {
-    const int nc = (it.ctx + KT - 1) / KT;
-    const int i = t < nc ? t * KT + key : (t - nc) * KT + key;  // committed or tree row
-    const int pos = t < nc ? i : it.ctx + i;
+  __device__ __forceinline__ void load(const TreeParams& P, const TreeItem& it, int pos) {
     const int c = div_by(pos, P.bs);
-    const bool ok = (t < nc ? i < it.ctx : i < it.n) && t < it.tiles && c < P.W;
+    const bool ok = (int)(pos < it.ctx + it.n) & (int)(c < P.W);
     blk = -1;
     if (ok) blk = P.table[it.b * P.table_stride + c];
     in_blk = pos - c * P.bs.d;
   }
+  __device__ __forceinline__ bool there(const TreeParams& P) const { return (uint32_t)blk < (uint32_t)P.blocks; }
+  // in 16-byte pieces from the pool's first row, which stands in for rows that are not there
   __device__ __forceinline__ uint32_t place(const TreeParams& P) const {
-    return blk >= 0 && blk < P.blocks ? (uint32_t)blk * P.sb + (uint32_t)in_blk * P.sr : kNoRow;
+    const uint32_t at = (uint32_t)blk * P.sb + (uint32_t)in_blk * P.sr;
+    return there(P) ? at : 0;
   }
 };
-
-// What rows that are not there read as.
-__device__ uint4 tree_zeros[1];
 
 // 16 bytes a lane from memory into the 1 KiB of LDS at `st` (lane l's piece at 16 l).
 __device__ __forceinline__ void tree_dma(const char* from, char* st) {
@@ -189,29 +221,95 @@ __device__ __forceinline__ void tree_dma(const char* from, char* st) {
                                    (__attribute__((address_space(3))) void*)(st), 16, 0, 0);
 }
 
-// Bits of the 32 tree rows from 32 w on that node i of the item's tree sees.
-__device__ __forceinline__ uint32_t tree_bits(const TreeParams& P, const TreeItem& it, int i, int w) {
-  if (P.mask != nullptr) return P.mask[(int64_t)(it.lo + i) * P.mask_stride + w];
-  const int d = i - 32 * w;
-  return d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1;
+// Bits of the 32 positions from `pos` on that node i of the item's tree sees:
+// committed rows all, tree rows by the node's mask.  In two steps, so that the
+// mask's words can be on their way during other work.
+struct TreeBits {
+  uint32_t lo, hi;
+  __device__ __forceinline__ void load(const TreeParams& P, const TreeItem& it, int i, int pos) {
+    lo = hi = 0xffffffffu;
+    if (P.mask == nullptr) return;
+    const int w = (pos - it.ctx) >> 5, words = (it.n + 31) >> 5;
+    const uint32_t* row = P.mask + (int64_t)(it.lo + i) * P.mask_stride;
+    if (w >= 0) lo = w < words ? row[w] : 0u;
+    if (w >= -1) hi = w + 1 < words ? row[w + 1] : 0u;
+  }
+  __device__ __forceinline__ uint32_t at(const TreeParams& P, const TreeItem& it, int i, int pos) const {
+    if (P.mask == nullptr) {
+      const int d = it.ctx + i - pos;
+      return d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1;
+    }
+    return (uint32_t)((((uint64_t)hi << 32) | lo) >> ((pos - it.ctx) & 31));
+  }
+};
+__device__ __forceinline__ uint32_t tree_bits(const TreeParams& P, const TreeItem& it, int i, int pos) {
+  TreeBits b;
+  b.load(P, it, i, pos);
+  return b.at(P, it, i, pos);
 }
 
-// A 16-bit operand's values that are not finite: which of a word's halves, as
-// 0xffff; and operands with 1 where the value is `inf` or NaN.
+// Bit k set: position pos + k is one of the request's rows (k < 32).
+__device__ __forceinline__ uint32_t tree_rows(const TreeItem& it, int pos) {
+  const int n = it.ctx + it.n - pos;
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+// Which halves of a word hold 16-bit values that are not finite, as 0xffff.
 template <int DT>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
   constexpr uint32_t E = DT == HALO_BF16 ? 0x7f80u : 0x7c00u;
   return ((w & E) == E ? 0xffffu : 0u) | ((w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u);
 }
 template <int DT>
-__device__ __forceinline__ uint32_t is_halves(uint32_t w, bool minus) {
-  constexpr uint32_t E = DT == HALO_BF16 ? 0x7f80u : 0x7c00u;
-  constexpr uint32_t one = DT == HALO_BF16 ? 0x3f80u : 0x3c00u;
-  const uint32_t other = minus ? E : (E | 0x8000u);  // the infinity that does not count
-  const uint32_t odd = odd_halves<DT>(w);
-  const uint32_t lo = (odd & 0xffffu) && (w & 0xffffu) != other ? one : 0u;
-  const uint32_t hi = (odd >> 16) && (w >> 16) != other ? one << 16 : 0u;
-  return lo | hi;
+__device__ __forceinline__ uint4 odd_halves(const uint4& v) {
+  return make_uint4(odd_halves<DT>(v.x), odd_halves<DT>(v.y), odd_halves<DT>(v.z), odd_halves<DT>(v.w));
+}
+
+// Tree rows that some nodes see and others do not: 0 x inf is not 0, so values
+// of V that are not finite must not meet the products.  Whether the staged V
+// tile (`bytes` of 16-bit values) holds any; all lanes take part.
+template <int DT>
+__device__ __forceinline__ bool tree_v_odd(const char* sv, int bytes, int lane) {
+  bool any = false;
+#pragma unroll 1
+  for (int x = lane * 16; x < bytes; x += 1024) {
+    const uint4 o = odd_halves<DT>(*reinterpret_cast<const uint4*>(sv + x));
+    any |= (o.x | o.y | o.z | o.w) != 0;
+  }
+  return __ballot(any) != 0;
+}
+// Zeroes them in LDS, from byte `from` in steps of `step`.
+template <int DT>
+__device__ __forceinline__ void tree_v_clean(char* sv, int bytes, int from, int step) {
+#pragma unroll 1
+  for (int x = from; x < bytes; x += step) {
+    uint4* at = reinterpret_cast<uint4*>(sv + x);
+    const uint4 v = *at, o = odd_halves<DT>(v);
+    *at = make_uint4(v.x & ~o.x, v.y & ~o.y, v.z & ~o.z, v.w & ~o.w);
+  }
+}
+// Adds them to the rows that see them: bit k of `bits` is this lane's row and
+// the tile's key k, whose staged row is at sv + at(k).
+template <int DT, int D, typename AT>
+__device__ __forceinline__ void tree_v_add_odd(pf32x16* o, const char* sv, uint64_t bits, int keys, int hh, AT at) {
+  constexpr int RB = D * 2;
+#pragma unroll 1
+  for (int k = 0; k < keys; ++k) {
+    const bool sees = (bits >> k) & 1;
+    const char* row = sv + at(k);
+#pragma unroll
+    for (int x = 0; x < D / 8; ++x) {
+      const int m = 8 * (x & 3) + 4 * hh;
+      const int byte = ((m >> 4) * (D / 2) + 16 * (x >> 2) + (m & 15)) * 2;  // see tree_channel
+      const uint2 w = *reinterpret_cast<const uint2*>(row + (((byte >> 4) ^ tree_vswz<RB>(k)) << 4) + (byte & 15));
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t half = ((y & 2 ? w.y : w.x) >> (16 * (y & 1))) & 0xffffu;
+        const float f = DT == HALO_BF16 ? __uint_as_float(half << 16) : f16_bits_to_f32((uint16_t)half);
+        o[x >> 2][4 * (x & 3) + y] += sees && !(fabsf(f) < INFINITY) ? f : 0.f;
+      }
+    }
+  }
 }
 
 __device__ __forceinline__ void tree_store4(const TreeParams& P, int64_t at, const float* v4) {
@@ -248,12 +346,94 @@ constexpr int kTreeRows = 32;  // rows of a unit: the columns of one 32x32 produ
 constexpr int kTreeKT = 32;    // rows of a key tile
 constexpr int kTreeWaves = 4;
 
+// Waits until at most N of the wave's vector memory instructions are in flight
+// (they end in order).
+template <int N>
+__device__ __forceinline__ void tree_wait() {
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  else {
+    static_assert(N == 16, "instructions of a tile");
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+  }
+}
+
+// LDS reads of a tile in one block with their wait.  The compiler orders an
+// ordinary LDS read behind every LDS-DMA in flight, since it cannot tell the
+// next K tile from this V tile; these are ordered by tree_wait alone.
+__device__ __forceinline__ uint32_t lds_addr(const char* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)(p);
+}
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+// b128 at a[0 .. N)
+__device__ __forceinline__ void lds_read8(u32x4* v, const uint32_t* a) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %12\n\tds_read_b128 %5, %13\n\tds_read_b128 %6, %14\n\tds_read_b128 %7, %15\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7])
+      : "memory");
+}
+__device__ __forceinline__ void lds_read4(u32x4* v, const uint32_t* a) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+      : "memory");
+}
+__device__ __forceinline__ void lds_read8_b64(u32x2* v, const uint32_t* a) {
+  asm volatile(
+      "ds_read_b64 %0, %8\n\tds_read_b64 %1, %9\n\tds_read_b64 %2, %10\n\tds_read_b64 %3, %11\n\t"
+      "ds_read_b64 %4, %12\n\tds_read_b64 %5, %13\n\tds_read_b64 %6, %14\n\tds_read_b64 %7, %15\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7])
+      : "memory");
+}
+// V^T operands of N d-blocks: for each, transposed reads at a, a + 256, a + 512 and a + 768.
+__device__ __forceinline__ void lds_read_tr2(u32x2* v, const uint32_t* a) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:256\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:512\n\tds_read_b64_tr_b16 %3, %8 offset:768\n\t"
+      "ds_read_b64_tr_b16 %4, %9\n\tds_read_b64_tr_b16 %5, %9 offset:256\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:512\n\tds_read_b64_tr_b16 %7, %9 offset:768\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(a[0]), "v"(a[1])
+      : "memory");
+}
+__device__ __forceinline__ void lds_read_tr4(u32x2* v, const uint32_t* a) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:256\n\t"
+      "ds_read_b64_tr_b16 %2, %16 offset:512\n\tds_read_b64_tr_b16 %3, %16 offset:768\n\t"
+      "ds_read_b64_tr_b16 %4, %17\n\tds_read_b64_tr_b16 %5, %17 offset:256\n\t"
+      "ds_read_b64_tr_b16 %6, %17 offset:512\n\tds_read_b64_tr_b16 %7, %17 offset:768\n\t"
+      "ds_read_b64_tr_b16 %8, %18\n\tds_read_b64_tr_b16 %9, %18 offset:256\n\t"
+      "ds_read_b64_tr_b16 %10, %18 offset:512\n\tds_read_b64_tr_b16 %11, %18 offset:768\n\t"
+      "ds_read_b64_tr_b16 %12, %19\n\tds_read_b64_tr_b16 %13, %19 offset:256\n\t"
+      "ds_read_b64_tr_b16 %14, %19 offset:512\n\tds_read_b64_tr_b16 %15, %19 offset:768\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
+        "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]), "=&v"(v[14]), "=&v"(v[15])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+      : "memory");
+}
+
+// Where a wave leaves piece x of its o (1 KiB, in register order): half of them over its K stage, half over its V stage.
+template <int D>
+__device__ __forceinline__ char* tree_piece(char* k, char* v, int x) {
+  return x < D / 16 ? k + x * 1024 : v + (x - D / 16) * 1024;
+}
+
 // The four waves of a workgroup hold (m, l, o) of the same 32 rows over
-// different tiles.  Each leaves its o in `mine` (16 KiB / 8 KiB at D = 128 / 64,
-// pieces in its own register order) and folds a quarter of the pieces.
-template <int D, bool F32>
+// different tiles; each folds a quarter of the pieces.
+template <int D, bool F32, int TB>
 __device__ __forceinline__ void tree_fold_store(const TreeParams& P, const TreeItem& it, int wave, int lane,
-                                                float2 (*s_ml)[32], const char* const* o_of_wave) {
+                                                float2 (*s_ml)[32], char (*sK)[TB], char (*sV)[TB]) {
   constexpr int PIECES = D / 8, PER = PIECES / kTreeWaves;
   const int qc = lane & 31, hh = lane >> 5;
   float M = -INFINITY;
@@ -277,7 +457,7 @@ __device__ __forceinline__ void tree_fold_store(const TreeParams& P, const TreeI
     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kTreeWaves; ++w) {
-      const float4 a = *reinterpret_cast<const float4*>(o_of_wave[w] + (x * 64 + lane) * 16);
+      const float4 a = *reinterpret_cast<const float4*>(tree_piece<D>(sK[w], sV[w], x) + lane * 16);
       v[0] += a.x * wt[w];
       v[1] += a.y * wt[w];
       v[2] += a.z * wt[w];
@@ -297,21 +477,90 @@ __device__ __forceinline__ void tree_fold_store(const TreeParams& P, const TreeI
   }
 }
 
+// A wave's tile in the narrow kernels: where its rows lie and which are there.
+template <int RB>
+struct TreeTile {
+  static constexpr int NJ = kTreeKT * RB / 1024;
+  typedef TreeLanes<RB, NJ> L;
+  TreeRow row;       // of the lane's first key, where one block holds the lane's rows
+  uint32_t pl[NJ];
+  uint32_t there;    // bit k: key k of the tile
+  __device__ __forceinline__ void look(const TreeParams& P, const TreeItem& it, int t, int lane) {
+    row.load(P, it, t * kTreeKT + L::first(lane));
+  }
+  __device__ __forceinline__ void locate(const TreeParams& P, const TreeItem& it, int t, int lane) {
+    constexpr int GROUPS = kTreeKT / L::SPAN;  // lanes whose rows share a block, 64 / GROUPS of them
+    if (P.bs.d % L::SPAN == 0) {
+      const bool ok = row.there(P);
+      const uint32_t p0 = row.place(P), step = ok ? L::STEP * P.sr : 0;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) pl[j] = p0 + j * step;
+      const uint64_t all = __ballot(ok);
+      there = 0xffffffffu;
+      if (all != ~0ull) {
+        there = 0;
+        constexpr uint32_t part = L::SPAN == 32 ? 0xffffffffu : (1u << L::SPAN) - 1;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) there |= (all >> (g * (64 / GROUPS))) & 1 ? part << (g * L::SPAN) : 0u;
+      }
+    } else {
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int k = L::first(lane) + j * L::STEP;
+        TreeRow r;
+        r.load(P, it, t * kTreeKT + k);
+        pl[j] = r.place(P);
+        mine |= r.there(P) ? 1u << k : 0u;
+      }
+      there = 0;
+#pragma unroll
+      for (int g = 0; g < L::RPI; ++g) there |= (uint32_t)__builtin_amdgcn_readlane(mine, g * L::SL);
+    }
+    there &= tree_rows(it, t * kTreeKT);
+  }
+  // K (swizzled for b128 reads of a row a lane) or V (for transposed reads; fp32 V plain)
+  template <bool V, bool F32>
+  __device__ __forceinline__ void issue(const char* base, char* st, int lane) const {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int k = L::first(lane) + j * L::STEP;
+      const int slot = lane % L::SL;
+      const int piece = !V ? slot ^ tree_kswz<RB>(k) : F32 ? slot : slot ^ tree_vswz<RB>(k);
+      tree_dma(base + (int64_t)pl[j] * 16 + (piece << 4), st + j * 1024);
+    }
+  }
+};
+
+// Zeroes the rows of a wave's staged V tile that are not there: their weights
+// are 0, but what the stand-in row holds need not be finite.
+template <int RB>
+__device__ __forceinline__ void tree_zero_rows(char* sv, uint32_t there, int lane) {
+  typedef typename TreeTile<RB>::L L;
+#pragma unroll 1
+  for (int j = 0; j < TreeTile<RB>::NJ; ++j) {
+    const int k = L::first(lane) + j * L::STEP;
+    if (!((there >> k) & 1)) *reinterpret_cast<uint4*>(sv + j * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // 16-bit queries and pools, products on v_mfma_f32_32x32x16:
 //   scores  S^T[key][row] = sum_d K[key][d] Q[row][d]          (A = K tile, B = Q^T)
 //   output  O^T[d][row]  += sum_key V^T[d][key] P^T[key][row]  (A = V^T, B = P^T)
 // S^T's accumulator gives lane (row, half h) the keys 8i + 4h + j, which are the
 // keys of its P^T operands, so p goes to the second product (rounded to the
 // pool's type, at most half a step of it) without a cross-lane move.  Each wave
-// streams tiles of its own, every fourth of the item's, through two LDS stages
-// of its own: no barrier in the loop.
+// streams tiles of its own, every fourth of the item's, through one LDS stage
+// of its own: the next K tile is asked for once the scores are there, the next
+// V tile once the product is; no barrier in the loop.
 template <int DT, int D>
-__global__ void __launch_bounds__(256) tree_attn_kernel(TreeParams P) {
-  constexpr int KS = D / 16, DB = D / 32, RB = D * 2, SL = RB / 16;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_kernel(TreeParams P) {
+  constexpr int KS = D / 16, DB = D / 32, RB = D * 2;
   constexpr int TB = kTreeKT * RB;  // bytes of a K or V tile
-  constexpr int RPI = 1024 / RB;    // rows of one 1 KiB LDS-DMA instruction
-  constexpr int NI = TB / 1024;
-  __shared__ __attribute__((aligned(16))) char sA[kTreeWaves][2 * TB], sB[kTreeWaves][2 * TB];  // stage: K, then V
+  typedef TreeTile<RB> Tile;
+  typedef typename Tile::L L;
+  constexpr int NJ = Tile::NJ;
+  __shared__ __attribute__((aligned(16))) char sK[kTreeWaves][TB], sV[kTreeWaves][TB];
   __shared__ float2 s_ml[kTreeWaves][32];
   TreeItem it;
   if (!tree_find<kTreeKT, kTreeRows, true>(P, blockIdx.x, it)) return;
@@ -319,8 +568,14 @@ __global__ void __launch_bounds__(256) tree_attn_kernel(TreeParams P) {
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
   const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
-  const int t0 = (int)((int64_t)it.tiles * it.cut / it.cuts) + wave;
-  const int nc = (it.ctx + kTreeKT - 1) / kTreeKT;
+  int t = (int)((int64_t)it.tiles * it.cut / it.cuts) + wave;
+  const int tree0 = it.ctx / kTreeKT;  // first tile with tree rows
+  char* const stK = sK[wave];
+  char* const stV = sV[wave];
+  const char* kh = P.k + (int64_t)it.h * P.sh * 16;
+  const char* vh = P.v + (int64_t)it.h * P.sh * 16;
+  Tile tile;
+  tile.look(P, it, t, lane);
 
   const int r_eff = min(it.rb * kTreeRows + qc, it.n * P.rep - 1);
   const int node = r_eff / P.rep, head = it.h * P.rep + (r_eff - node * P.rep);
@@ -331,184 +586,134 @@ __global__ void __launch_bounds__(256) tree_attn_kernel(TreeParams P) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) qb[s] = *reinterpret_cast<const uint4*>(qrow + (s * 16 + hh * 8) * 2);
   }
-  const char* kh = P.k + (int64_t)it.h * P.sh * 16;
-  const char* vh = P.v + (int64_t)it.h * P.sh * 16;
+  // the mask bits of the wave's first tile with tree rows
+  const int tm = t < tree0 ? t + (tree0 - t + kTreeWaves - 1) / kTreeWaves * kTreeWaves : t;
+  TreeBits first_bits = {0, 0};
+  if (tm < t_end) first_bits.load(P, it, node, tm * kTreeKT);
 
-  auto kswz = [](int r) { return RB == 256 ? (r & 15) : ((r >> 1) & 7); };
-  auto vswz = [](int r) { return RB == 256 ? 2 * (r & 3) : 2 * ((r >> 1) & 1); };
-  // Each instruction fills RPI rows, lane l the slot l % SL of row l / SL with the piece that belongs there.
-  auto issue = [&](uint32_t place, char* st) {
+  uint32_t ka[KS];  // K operands: key qc, channels 16 s + 8 half
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int row = j * RPI + lane / SL, slot = lane % SL;
-      const uint32_t at = __shfl(place, row, 64);
-      const char* k = at == kNoRow ? reinterpret_cast<const char*>(tree_zeros)
-                                   : kh + (int64_t)at * 16 + ((slot ^ kswz(row)) << 4);
-      const char* v = at == kNoRow ? reinterpret_cast<const char*>(tree_zeros)
-                                   : vh + (int64_t)at * 16 + ((slot ^ vswz(row)) << 4);
-      tree_dma(k, st + j * 1024);
-      tree_dma(v, st + TB + j * 1024);
+  for (int s = 0; s < KS; ++s)
+    ka[s] = lds_addr(stK) + L::lds_row(qc) * RB + (((2 * s + hh) ^ tree_kswz<RB>(qc)) << 4);
+  // V^T operands of step u, d-block db: keys 16 u + 4 (lane / 32) + (lane % 16) / 4 and 8 more, 512 bytes a step, 256 to the upper keys
+  static_assert((L::lds_row(8) - L::lds_row(0)) * RB == 256 && (L::lds_row(16) - L::lds_row(0)) * RB == 512, "offsets of the V reads");
+  uint32_t va[DB];
+  {
+    const int vG = lane >> 4, vei = (lane & 15) >> 2, vai = lane & 3;
+    const int k = 4 * (vG >> 1) + vei;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int byte = ((vG & 1) * (D / 2) + 16 * db + 4 * vai) * 2;
+      va[db] = lds_addr(stV) + L::lds_row(k) * RB + (((byte >> 4) ^ tree_vswz<RB>(k)) << 4) + (byte & 15);
     }
-  };
-  auto kread = [&](const char* st, int s) {
-    return *reinterpret_cast<const uint4*>(st + qc * RB + (((2 * s + hh) ^ kswz(qc)) << 4));
-  };
-  const int vG = lane >> 4, vei = (lane & 15) >> 2, vai = lane & 3;
-  auto vread = [&](const char* st, int i) {
-    const int t = i / DB, db = i % DB;
-    const int rlo = 16 * t + 4 * (vG >> 1) + vei, rhi = rlo + 8;
-    const int byte = ((vG & 1) * (D / 2) + 16 * db + 4 * vai) * 2;
-    const int pc = byte >> 4, wi = byte & 15;
-    const uint2 a0 = pf_tr16(st + TB + rlo * RB + ((pc ^ vswz(rlo)) << 4) + wi);
-    const uint2 a1 = pf_tr16(st + TB + rhi * RB + ((pc ^ vswz(rhi)) << 4) + wi);
-    return make_uint4(a0.x, a0.y, a1.x, a1.y);
-  };
+  }
 
   pf32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = pf32x16{};
   float m_run = -INFINITY, l_run = 0.f;
 
-  // a tile's rows that are there, and of those the ones that this lane's row sees
-  struct Tile {
-    uint32_t there, bits;
-  };
-  auto open = [&](const TreeRow<kTreeKT>& row, int t, char* st) {
-    Tile x;
-    const uint32_t place = row.place(P);
-    x.there = (uint32_t)__ballot(place != kNoRow);
-    x.bits = x.there;
-    if (t >= nc) x.bits &= tree_bits(P, it, node, t - nc);
-    issue(place, st);
-    return x;
-  };
-  auto compute = [&](const Tile& x, int t, const char* st) {
-    pf32x16 S = pf32x16{};
+  if (t < t_end) {
+    tile.locate(P, it, t, lane);
+    tile.template issue<false, false>(kh, stK, lane);
+    tile.template issue<true, false>(vh, stV, lane);
+    // q and the mask bits are waited for here, not in the loop behind the DMA in flight there
 #pragma unroll
-    for (int s = 0; s < KS; ++s) S = PMfma<DT>::run(kread(st, s), qb[s], S);
-    const uint32_t mine = x.bits >> (4 * hh);
-    if (__ballot(x.bits != 0xffffffffu)) {
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qb[s].x), "+v"(qb[s].y), "+v"(qb[s].z), "+v"(qb[s].w));
+    asm volatile("" : "+v"(first_bits.lo), "+v"(first_bits.hi));
+    const uint32_t bits0 = first_bits.at(P, it, node, tm * kTreeKT);
+    tile.look(P, it, t + kTreeWaves, lane);
+    for (;;) {
+      const uint32_t there = tile.there;
+      uint32_t bits = there;
+      if (t >= tree0) bits &= t == tm ? bits0 : tree_bits(P, it, node, t * kTreeKT);
+      const int tn = t + kTreeWaves;
+      tree_wait<NJ>();  // K: this tile's V came after it
+      u32x4 kk[KS];
+      if constexpr (KS == 8) lds_read8(kk, ka);
+      else lds_read4(kk, ka);
+      pf32x16 S = pf32x16{};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) S[e] = (mine >> (8 * (e >> 2) + (e & 3))) & 1 ? S[e] : -INFINITY;
-    }
-    float bm = -INFINITY;
+      for (int s = 0; s < KS; ++s) S = PMfma<DT>::run(__builtin_bit_cast(uint4, kk[s]), qb[s], S);
+      // past the last tile the stand-in row is read: the waits below count on NJ instructions
+      tile.locate(P, it, tn, lane);
+      tile.template issue<false, false>(kh, stK, lane);
+      tile.look(P, it, tn + kTreeWaves, lane);
+      const uint32_t mine = bits >> (4 * hh);
+      if (__ballot(bits != 0xffffffffu)) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) bm = fmaxf(bm, S[e]);
-    bm = half_max(bm) * P.scale2;  // scale > 0
-    const float m_old = m_run;
-    m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
-    const float ms = m_run == -INFINITY ? 0.f : m_run;
-    if (__ballot(m_run != m_old)) {
-      const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
-      l_run *= alpha;
+        for (int e = 0; e < 16; ++e) S[e] = (mine >> (8 * (e >> 2) + (e & 3))) & 1 ? S[e] : -INFINITY;
+      }
+      float bm = -INFINITY;
 #pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] *= alpha;
-    }
-    float p[16];
+      for (int e = 0; e < 16; ++e) bm = fmaxf(bm, S[e]);
+      bm = half_max(bm) * P.scale2;  // scale > 0
+      const float m_old = m_run;
+      m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
+      const float ms = m_run == -INFINITY ? 0.f : m_run;
+      if (__ballot(m_run != m_old)) {
+        const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
+        l_run *= alpha;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e], P.scale2, -ms));
-      l_run += p[e];
-    }
-    uint4 pb[2];  // step t: keys 16 t + {4 h + j, 8 + 4 h + j}
+        for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      }
+      float p[16], ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      pb[u] = make_uint4(PMfma<DT>::pack(p[8 * u], p[8 * u + 1]), PMfma<DT>::pack(p[8 * u + 2], p[8 * u + 3]),
-                         PMfma<DT>::pack(p[8 * u + 4], p[8 * u + 5]), PMfma<DT>::pack(p[8 * u + 6], p[8 * u + 7]));
-    // Tree rows that some nodes see and others do not: 0 x inf is not 0, so
-    // values that are not finite are kept out of the product and reach the
-    // rows that see them only.
-    bool odd = false;
-    if (t >= nc) {
-      uint32_t any = 0;
+      for (int e = 0; e < 16; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e], P.scale2, -ms));
+        ps[e & 3] += p[e];
+      }
+      l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      uint4 pb[2];  // step u: keys 16 u + {4 h + j, 8 + 4 h + j}
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        pb[u] = make_uint4(PMfma<DT>::pack(p[8 * u], p[8 * u + 1]), PMfma<DT>::pack(p[8 * u + 2], p[8 * u + 3]),
+                           PMfma<DT>::pack(p[8 * u + 4], p[8 * u + 5]), PMfma<DT>::pack(p[8 * u + 6], p[8 * u + 7]));
+      tree_wait<NJ>();  // V: the next tile's K came after it
+      if (there != 0xffffffffu) {
+        tree_zero_rows<RB>(stV, there, lane);
+        wave_lds_fence();
+      }
+      if (t >= tree0 && tree_v_odd<DT>(stV, TB, lane)) {
+        tree_v_add_odd<DT, D>(o, stV, bits, kTreeKT, hh, [](int k) { return L::lds_row(k) * RB; });
+        wave_lds_fence();
+        tree_v_clean<DT>(stV, TB, lane * 16, 1024);
+        wave_lds_fence();
+      }
+      u32x2 vv[4 * DB];
+      if constexpr (DB == 4) lds_read_tr4(vv, va);
+      else lds_read_tr2(vv, va);
 #pragma unroll
       for (int i = 0; i < 2 * DB; ++i) {
-        const uint4 v = vread(st, i);
-        any |= odd_halves<DT>(v.x) | odd_halves<DT>(v.y) | odd_halves<DT>(v.z) | odd_halves<DT>(v.w);
+        const u32x2 lo = vv[4 * (i % DB) + 2 * (i / DB)], hi = vv[4 * (i % DB) + 2 * (i / DB) + 1];
+        o[i % DB] = PMfma<DT>::run(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[i / DB], o[i % DB]);
       }
-      odd = __ballot(any != 0) != 0;
+      t = tn;
+      if (t >= t_end) break;
+      tile.template issue<true, false>(vh, stV, lane);
     }
-    if (!odd) {
-#pragma unroll
-      for (int i = 0; i < 2 * DB; ++i) o[i % DB] = PMfma<DT>::run(vread(st, i), pb[i / DB], o[i % DB]);
-      return;
-    }
-    uint4 sees[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = (mine >> (8 * ((8 * u + e) >> 2) + (e & 3))) & 1 ? 1.f : 0.f;
-      sees[u] = make_uint4(PMfma<DT>::pack(f[0], f[1]), PMfma<DT>::pack(f[2], f[3]), PMfma<DT>::pack(f[4], f[5]),
-                           PMfma<DT>::pack(f[6], f[7]));
-    }
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      pf32x16 plus = pf32x16{}, minus = pf32x16{};
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint4 v = vread(st, u * DB + db);
-        const uint4 f = make_uint4(v.x & ~odd_halves<DT>(v.x), v.y & ~odd_halves<DT>(v.y),
-                                   v.z & ~odd_halves<DT>(v.z), v.w & ~odd_halves<DT>(v.w));
-        o[db] = PMfma<DT>::run(f, pb[u], o[db]);
-        const uint4 a = make_uint4(is_halves<DT>(v.x, false), is_halves<DT>(v.y, false), is_halves<DT>(v.z, false),
-                                   is_halves<DT>(v.w, false));
-        const uint4 c = make_uint4(is_halves<DT>(v.x, true), is_halves<DT>(v.y, true), is_halves<DT>(v.z, true),
-                                   is_halves<DT>(v.w, true));
-        plus = PMfma<DT>::run(a, sees[u], plus);
-        minus = PMfma<DT>::run(c, sees[u], minus);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[db][e] += (plus[e] > 0.f ? INFINITY : 0.f) + (minus[e] > 0.f ? -INFINITY : 0.f);
-    }
-  };
-
-  TreeRow<kTreeKT> ra, rb;
-  Tile ta = {0, 0}, tb = {0, 0};
-  const int key = lane & 31;
-  char* const stA = sA[wave];
-  char* const stB = sB[wave];
-  ra.load(P, it, t0, key);
-  rb.load(P, it, t0 + kTreeWaves, key);
-  if (t0 < t_end) ta = open(ra, t0, stA);
-  if (t0 + kTreeWaves < t_end) tb = open(rb, t0 + kTreeWaves, stB);
-  for (int t = t0; t < t_end; t += 2 * kTreeWaves) {
-    const int t1 = t + kTreeWaves, t2 = t + 2 * kTreeWaves, t3 = t + 3 * kTreeWaves;
-    ra.load(P, it, t2, key);
-    rb.load(P, it, t3, key);
-    __builtin_amdgcn_s_waitcnt(0);
-    compute(ta, t, stA);
-    if (t2 < t_end) ta = open(ra, t2, stA);
-    if (t1 < t_end) {
-      __builtin_amdgcn_s_waitcnt(0);
-      compute(tb, t1, stB);
-      if (t3 < t_end) tb = open(rb, t3, stB);
-    }
+    tree_wait<0>();  // the stand-in rows have landed: o goes over the stages
   }
-  // o to LDS: the pieces below NI over the stage A, the others over the stage B
   const float lt = half_sum(l_run);
   if (hh == 0) s_ml[wave][qc] = make_float2(m_run, lt);
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<float4*>(stA + ((db * 4 + i) * 64 + lane) * 16) =
-          make_float4(o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]);
+  for (int x = 0; x < D / 8; ++x)
+    *reinterpret_cast<float4*>(tree_piece<D>(stK, stV, x) + lane * 16) =
+        make_float4(o[x / 4][4 * (x & 3)], o[x / 4][4 * (x & 3) + 1], o[x / 4][4 * (x & 3) + 2], o[x / 4][4 * (x & 3) + 3]);
   __syncthreads();
-  const char* ow[kTreeWaves] = {sA[0], sA[1], sA[2], sA[3]};
-  tree_fold_store<D, false>(P, it, wave, lane, s_ml, ow);
+  tree_fold_store<D, false, TB>(P, it, wave, lane, s_ml, sK, sV);
 }
 
 // fp32 queries and pools: the same walk on v_mfma_f32_32x32x2 (fp32 products
 // and sums).  Step s of the score product multiplies channel s (lane half 0)
-// and D/2 + s (half 1).  One LDS stage a wave: K of the next tile is asked for
-// once this tile's scores are there, V once its product is.
+// and D/2 + s (half 1).
 template <int D>
-__global__ void __launch_bounds__(256) tree_attn_f32_kernel(TreeParams P) {
-  constexpr int DB = D / 32, RB = D * 4, SL = RB / 16;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_f32_kernel(TreeParams P) {
+  constexpr int DB = D / 32, RB = D * 4;
   constexpr int TB = kTreeKT * RB;
-  constexpr int RPI = 1024 / RB;
-  constexpr int NI = TB / 1024;
+  typedef TreeTile<RB> Tile;
+  typedef typename Tile::L L;
+  constexpr int NJ = Tile::NJ;
   __shared__ __attribute__((aligned(16))) char sK[kTreeWaves][TB], sV[kTreeWaves][TB];
   __shared__ float2 s_ml[kTreeWaves][32];
   TreeItem it;
@@ -517,8 +722,14 @@ __global__ void __launch_bounds__(256) tree_attn_f32_kernel(TreeParams P) {
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
   const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
-  const int t0 = (int)((int64_t)it.tiles * it.cut / it.cuts) + wave;
-  const int nc = (it.ctx + kTreeKT - 1) / kTreeKT;
+  int t = (int)((int64_t)it.tiles * it.cut / it.cuts) + wave;
+  const int tree0 = it.ctx / kTreeKT;
+  char* const stK = sK[wave];
+  char* const stV = sV[wave];
+  const char* kh = P.k + (int64_t)it.h * P.sh * 16;
+  const char* vh = P.v + (int64_t)it.h * P.sh * 16;
+  Tile tile;
+  tile.look(P, it, t, lane);
 
   const int r_eff = min(it.rb * kTreeRows + qc, it.n * P.rep - 1);
   const int node = r_eff / P.rep, head = it.h * P.rep + (r_eff - node * P.rep);
@@ -536,126 +747,149 @@ __global__ void __launch_bounds__(256) tree_attn_f32_kernel(TreeParams P) {
       qf[4 * s + 3] = x.w;
     }
   }
-  const char* kh = P.k + (int64_t)it.h * P.sh * 16;
-  const char* vh = P.v + (int64_t)it.h * P.sh * 16;
-  // K pieces are swizzled (piece ^ row % 16), V rows are read whole
-  auto issue = [&](const char* base, uint32_t place, char* st, bool is_v) {
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int row = j * RPI + lane / SL, slot = lane % SL;
-      const uint32_t at = __shfl(place, row, 64);
-      const int piece = is_v ? slot : slot ^ (row & 15);
-      tree_dma(at == kNoRow ? reinterpret_cast<const char*>(tree_zeros) : base + (int64_t)at * 16 + (piece << 4),
-               st + j * 1024);
-    }
-  };
+  const int tm = t < tree0 ? t + (tree0 - t + kTreeWaves - 1) / kTreeWaves * kTreeWaves : t;
+  TreeBits first_bits = {0, 0};
+  if (tm < t_end) first_bits.load(P, it, node, tm * kTreeKT);
+
+  typedef __attribute__((ext_vector_type(DB))) float vrow;
+  const uint32_t krow = lds_addr(stK) + L::lds_row(qc) * RB;
+
   pf32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = pf32x16{};
   float m_run = -INFINITY, l_run = 0.f;
-  const int key = lane & 31;
-  char* const stK = sK[wave];
-  char* const stV = sV[wave];
-  TreeRow<kTreeKT> row;
-  row.load(P, it, t0, key);
-  uint32_t place = row.place(P);
-  if (t0 < t_end) {
-    issue(kh, place, stK, false);
-    issue(vh, place, stV, true);
-  }
-  for (int t = t0; t < t_end; t += kTreeWaves) {
-    const uint32_t there = (uint32_t)__ballot(place != kNoRow);
-    uint32_t bits = there;
-    if (t >= nc) bits &= tree_bits(P, it, node, t - nc);
-    row.load(P, it, t + kTreeWaves, key);
-    __builtin_amdgcn_s_waitcnt(0);
-    pf32x16 S = pf32x16{};
+
+  if (t < t_end) {
+    tile.locate(P, it, t, lane);
+    tile.template issue<false, true>(kh, stK, lane);
+    tile.template issue<true, true>(vh, stV, lane);
 #pragma unroll
-    for (int s = 0; s < D / 8; ++s) {
-      const float4 x =
-          *reinterpret_cast<const float4*>(stK + qc * RB + (((hh * (D / 8) + s) ^ (qc & 15)) << 4));
-      S = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, qf[4 * s], S, 0, 0, 0);
-      S = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, qf[4 * s + 1], S, 0, 0, 0);
-      S = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, qf[4 * s + 2], S, 0, 0, 0);
-      S = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, qf[4 * s + 3], S, 0, 0, 0);
-    }
-    place = row.place(P);
-    const bool more = t + kTreeWaves < t_end;
-    if (more) issue(kh, place, stK, false);
-    const uint32_t mine = bits >> (4 * hh);
-    if (__ballot(bits != 0xffffffffu)) {
+    for (int s = 0; s < D / 2; ++s) asm volatile("" : "+v"(qf[s]));
+    asm volatile("" : "+v"(first_bits.lo), "+v"(first_bits.hi));
+    const uint32_t bits0 = first_bits.at(P, it, node, tm * kTreeKT);
+    tile.look(P, it, t + kTreeWaves, lane);
+    for (;;) {
+      const uint32_t there = tile.there;
+      uint32_t bits = there;
+      if (t >= tree0) bits &= t == tm ? bits0 : tree_bits(P, it, node, t * kTreeKT);
+      const int tn = t + kTreeWaves;
+      tree_wait<NJ>();
+      pf32x16 S = pf32x16{};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) S[e] = (mine >> (8 * (e >> 2) + (e & 3))) & 1 ? S[e] : -INFINITY;
-    }
-    float bm = -INFINITY;
+      for (int s0 = 0; s0 < D / 8; s0 += 8) {
+        uint32_t ka[8];
+        u32x4 kk[8];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) bm = fmaxf(bm, S[e]);
-    bm = half_max(bm) * P.scale2;
-    const float m_old = m_run;
-    m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
-    const float ms = m_run == -INFINITY ? 0.f : m_run;
-    if (__ballot(m_run != m_old)) {
-      const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
-      l_run *= alpha;
+        for (int s = 0; s < 8; ++s) ka[s] = krow + (((hh * (D / 8) + s0 + s) ^ tree_kswz<RB>(qc)) << 4);
+        lds_read8(kk, ka);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] *= alpha;
-    }
-    float p[16];
-    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < 8; ++s)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e], P.scale2, -ms));
-      ps[e & 3] += p[e];
-    }
-    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-    typedef __attribute__((ext_vector_type(DB))) float vrow;
-    auto vread = [&](int e) {
-      return *reinterpret_cast<const vrow*>(stV + (8 * (e >> 2) + 4 * hh + (e & 3)) * RB + qc * DB * 4);
-    };
-    // tree rows: values that are not finite reach the rows that see them only
-    bool odd = false;
-    if (t >= nc) {
-      bool bad = false;
+          for (int x = 0; x < 4; ++x)
+            S = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kk[s][x]), qf[4 * (s0 + s) + x], S, 0, 0, 0);
+      }
+      tile.locate(P, it, tn, lane);
+      tile.template issue<false, true>(kh, stK, lane);
+      tile.look(P, it, tn + kTreeWaves, lane);
+      const uint32_t mine = bits >> (4 * hh);
+      if (__ballot(bits != 0xffffffffu)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[e] = (mine >> (8 * (e >> 2) + (e & 3))) & 1 ? S[e] : -INFINITY;
+      }
+      float bm = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bm = fmaxf(bm, S[e]);
+      bm = half_max(bm) * P.scale2;
+      const float m_old = m_run;
+      m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
+      const float ms = m_run == -INFINITY ? 0.f : m_run;
+      if (__ballot(m_run != m_old)) {
+        const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
+        l_run *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      }
+      float p[16], ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const vrow v = vread(e);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) bad |= !(fabsf(v[db]) < INFINITY);
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e], P.scale2, -ms));
+        ps[e & 3] += p[e];
       }
-      odd = __ballot(bad) != 0;
-    }
-    // a tile's products are summed by themselves and then added to O: its rounding error stays below one
-    // accumulator's over all keys
-    pf32x16 tile[DB];
-#pragma unroll
-    for (int db = 0; db < DB; ++db) tile[db] = pf32x16{};
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const vrow v = vread(e);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const float x = odd && !(fabsf(v[db]) < INFINITY) ? 0.f : v[db];
-        tile[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[e], tile[db], 0, 0, 0);
+      l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      tree_wait<NJ>();
+      if (there != 0xffffffffu) {
+        tree_zero_rows<RB>(stV, there, lane);
+        wave_lds_fence();
       }
-    }
+      // tree rows: values that are not finite reach the rows that see them only
+      if (t >= tree0) {
+        bool bad = false;
+#pragma unroll 1
+        for (int x = lane * 16; x < TB; x += 1024) {
+          const float4 y = *reinterpret_cast<const float4*>(stV + x);
+          bad |= (y.x * 0.f + y.y * 0.f) + (y.z * 0.f + y.w * 0.f) != 0.f;  // inf x 0 and NaN x 0 are NaN
+        }
+        if (__ballot(bad)) {
+#pragma unroll 1
+          for (int k = 0; k < kTreeKT; ++k) {
+            const bool sees = (bits >> k) & 1;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[db] += tile[db];
-    if (odd) {
+            for (int e = 0; e < 16; ++e) {
+              const vrow v =
+                  *reinterpret_cast<const vrow*>(stV + L::lds_row(k) * RB + (8 * (e >> 2) + 4 * hh + (e & 3)) * DB * 4);
 #pragma unroll
-      for (int x = 0; x < 2 * DB; ++x) {
-        const float inf = x & 1 ? -INFINITY : INFINITY;
-        pf32x16 n = pf32x16{};
+              for (int db = 0; db < DB; ++db) o[db][e] += sees && !(fabsf(v[db]) < INFINITY) ? v[db] : 0.f;
+            }
+          }
+          wave_lds_fence();
+#pragma unroll 1
+          for (int x = lane * 4; x < TB; x += 256) {
+            float* y = reinterpret_cast<float*>(stV + x);
+            if (!(fabsf(*y) < INFINITY)) *y = 0.f;
+          }
+          wave_lds_fence();
+        }
+      }
+      // a tile's products are summed by themselves and then added to O: its rounding error stays below one
+      // accumulator's over all keys
+      pf32x16 sum[DB];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float v = vread(e)[x >> 1];
-          const float sees = (mine >> (8 * (e >> 2) + (e & 3))) & 1 ? 1.f : 0.f;
-          n = __builtin_amdgcn_mfma_f32_32x32x2f32(v == inf || v != v ? 1.f : 0.f, sees, n, 0, 0, 0);
+      for (int db = 0; db < DB; ++db) sum[db] = pf32x16{};
+#pragma unroll
+      for (int e0 = 0; e0 < 16; e0 += 8) {
+        uint32_t va[8];
+        float v[8][DB];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          va[e] = lds_addr(stV) + L::lds_row(8 * ((e0 + e) >> 2) + 4 * hh + (e & 3)) * RB + qc * DB * 4;
+        if constexpr (DB == 4) {
+          u32x4 w[8];
+          lds_read8(w, va);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) v[e][db] = __uint_as_float(w[e][db]);
+        } else {
+          u32x2 w[8];
+          lds_read8_b64(w, va);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) v[e][db] = __uint_as_float(w[e][db]);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[x >> 1][e] += n[e] > 0.f ? inf : 0.f;
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            sum[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e][db], p[e0 + e], sum[db], 0, 0, 0);
       }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] += sum[db];
+      t = tn;
+      if (t >= t_end) break;
+      tile.template issue<true, true>(vh, stV, lane);
     }
-    if (more) issue(vh, place, stV, true);
+    tree_wait<0>();
   }
   const float lt = half_sum(l_run);
   if (hh == 0) s_ml[wave][qc] = make_float2(m_run, lt);
@@ -670,11 +904,11 @@ __global__ void __launch_bounds__(256) tree_attn_f32_kernel(TreeParams P) {
         const int c = 4 * g + y;
         x[y] = o[c % DB][4 * i + c / DB];
       }
-      *reinterpret_cast<float4*>(stK + ((i * DB + g) * 64 + lane) * 16) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(tree_piece<D>(stK, stV, i * DB + g) + lane * 16) =
+          make_float4(x[0], x[1], x[2], x[3]);
     }
   __syncthreads();
-  const char* ow[kTreeWaves] = {sK[0], sK[1], sK[2], sK[3]};
-  tree_fold_store<D, true>(P, it, wave, lane, s_ml, ow);
+  tree_fold_store<D, true, TB>(P, it, wave, lane, s_ml, sK, sV);
 }
 
 // Merge of a unit's partials: with M the largest of a row's maxima, out = sum_c
@@ -762,10 +996,10 @@ TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows,
   TreeShape s;
   const int64_t rows = (int64_t)max_nodes * (H / H_kv);
   s.units = (int64_t)B * H_kv * ((rows + kTreeRows - 1) / kTreeRows);
-  // LDS of a workgroup: 128 KiB at D = 128, 64 KiB at D = 64, fp32 the same with half the stages
-  s.slots = 256 * (D == 64 ? 2 : 1);
-  s.min_tiles = 2 * kTreeWaves;
-  const int64_t longest = (max_rows + kTreeKT - 1) / kTreeKT + (max_nodes + kTreeKT - 1) / kTreeKT;
+  // by the LDS of a workgroup (16 bits: 64 and 32 KiB at D = 128 and 64, fp32 twice that) and 2 waves a SIMD
+  s.slots = 256 * (dtype == HALO_F32 && D == 128 ? 1 : 2);
+  s.min_tiles = kTreeWaves;
+  const int64_t longest = (max_rows + max_nodes + kTreeKT - 1) / kTreeKT;
   s.merge = longest > s.min_tiles;
   // tree_find: at most `room` items besides one a unit
   s.grid = s.merge ? (s.slots / 2 + s.units > s.slots ? s.slots / 2 + s.units : s.slots) : s.units;
