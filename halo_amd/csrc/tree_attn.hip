@@ -215,6 +215,9 @@ struct TreeRow {
   }
 };
 
+// What rows that are not there read as, where they are not zeroed in LDS.
+__device__ uint4 tree_zeros[1];
+
 // 16 bytes a lane from memory into the 1 KiB of LDS at `st` (lane l's piece at 16 l).
 __device__ __forceinline__ void tree_dma(const char* from, char* st) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),
@@ -345,6 +348,7 @@ __device__ __forceinline__ float tree_weight(float m, float M) {
 constexpr int kTreeRows = 32;  // rows of a unit: the columns of one 32x32 product
 constexpr int kTreeKT = 32;    // rows of a key tile
 constexpr int kTreeWaves = 4;
+constexpr int kTreeWideKT = 64;
 
 // Waits until at most N of the wave's vector memory instructions are in flight
 // (they end in order).
@@ -911,21 +915,328 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   tree_fold_store<D, true, TB>(P, it, wave, lane, s_ml, sK, sV);
 }
 
+// More than 32 rows a unit, 16 bits: NW waves of 32 rows each share every K/V
+// tile, 64 keys staged in LDS (two stages of K and of V), one barrier a tile.
+// K is staged two tiles ahead and V one, so the score products of tile t + 1
+// are issued between the exponentials of tile t, and the maximum of tile t + 1
+// between the output products of tile t: the matrix core and the VALU overlap
+// within a wave.  Lane l of each wave looks up key l of a tile, so one vote gives the
+// rows that are there, and hands the places to the lanes that stage them.
+template <int DT, int D, int NW>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_wide_kernel(TreeParams P) {
+  constexpr int KT = kTreeWideKT, R = 32 * NW;
+  constexpr int KS = D / 16, DB = D / 32, RB = D * 2;
+  constexpr int TB = KT * RB;
+  constexpr int NJ = TB / 1024 / NW;  // LDS-DMA instructions of a wave and tile
+  typedef TreeLanes<RB, NJ> L;
+  static_assert(L::KEYS * NW == KT, "the waves stage the tile");
+  __shared__ __attribute__((aligned(16))) char sK0[TB], sK1[TB], sV0[TB], sV1[TB];
+  TreeItem it;
+  if (!tree_find<KT, R, true>(P, blockIdx.x, it)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = uni((int)(threadIdx.x >> 6));
+  const int qc = lane & 31, hh = lane >> 5;
+  const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
+  const int t0 = (int)((int64_t)it.tiles * it.cut / it.cuts);
+  const int tree0 = it.ctx / KT;  // first tile with tree rows
+  const char* kh = P.k + (int64_t)it.h * P.sh * 16;
+  const char* vh = P.v + (int64_t)it.h * P.sh * 16;
+
+  TreeRow row;  // of key `lane` of the tile looked up last
+  row.load(P, it, t0 * KT + lane);
+
+  const int RG = it.n * P.rep;
+  const int r_lane = it.rb * R + wave * 32 + qc;
+  const bool active = it.rb * R + wave * 32 < RG;  // a wave past the rows only stages tiles
+  const int r_eff = min(r_lane, RG - 1);
+  const int node = r_eff / P.rep, head = it.h * P.rep + (r_eff - node * P.rep);
+  uint4 qb[KS];
+  {
+    const char* qrow =
+        reinterpret_cast<const char*>(P.q) + ((it.lo + node) * P.q_stride_n + head * P.q_stride_h) * 2;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qb[s] = *reinterpret_cast<const uint4*>(qrow + (s * 16 + hh * 8) * 2);
+  }
+
+  // a tile's staged places (of this wave's rows) and which of its keys are there
+  struct Tile {
+    uint32_t pl[NJ];
+    uint64_t there;
+  };
+  int my_key = wave * L::KEYS + L::first(lane);
+  auto locate = [&](int t) {
+    Tile x;
+    const bool ok = row.there(P);
+    const uint32_t place = ok ? row.place(P) : kNoRow;
+    x.there = __ballot(ok);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) x.pl[j] = __shfl(place, my_key + j * L::STEP, 64);
+    row.load(P, it, (t + 1) * KT + lane);
+    return x;
+  };
+  auto issue = [&](const Tile& x, const char* base, char* st, bool is_v) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int k = my_key + j * L::STEP, slot = lane % L::SL;
+      const int piece = slot ^ (is_v ? tree_vswz<RB>(k) : tree_kswz<RB>(k));
+      const char* from = base + (int64_t)x.pl[j] * 16 + (piece << 4);
+      tree_dma(x.pl[j] == kNoRow ? reinterpret_cast<const char*>(tree_zeros) : from, st + (wave * NJ + j) * 1024);
+    }
+  };
+  // Operand addresses: the key's LDS row and, xored, the piece.  lds_row takes
+  // the bits of a key apart, so the rows of key step u are those of the first
+  // by a constant.  kx and vx pass through a register of unknown value in each
+  // tile: the xors are cheaper than keeping all their results.
+  auto lds_row = [](int k) { return k / L::KEYS * L::KEYS + L::lds_row(k % L::KEYS); };
+  const int kx0 = L::lds_row(qc % L::KEYS) * RB + qc / L::KEYS * L::KEYS * RB + ((hh ^ tree_kswz<RB>(qc)) << 4);
+  auto kread = [&](const char* sk, int i, int kx) {  // step i: d-step i / 2, key block i % 2
+    static_assert(32 % L::KEYS == 0, "key block 1 is 32 LDS rows on");
+    return *reinterpret_cast<const uint4*>(sk + (i & 1) * 32 * RB + (kx ^ ((i >> 1) << 5)));
+  };
+  const int vG = lane >> 4, vkey = 4 * (vG >> 1) + ((lane & 15) >> 2), vai = lane & 3;
+  const int vx0 = lds_row(vkey) * RB + ((((vG & 1) * (D / 16) + (vai >> 1)) ^ tree_vswz<RB>(vkey)) << 4) + 8 * (vai & 1);
+  auto vread = [&](const char* sv, int i, int vx) {  // step i: key step i / DB, d-block i % DB
+    const int u = i / DB;
+    const char* at = sv + (vx ^ ((i % DB) << 5));
+    const uint2 a0 = pf_tr16(at + lds_row(16 * u) * RB);
+    const uint2 a1 = pf_tr16(at + lds_row(16 * u + 8) * RB);
+    return make_uint4(a0.x, a0.y, a1.x, a1.y);
+  };
+  constexpr int NKS = 2 * KS;  // score MFMAs per tile
+  constexpr int NPV = 4 * DB;  // output MFMAs per tile
+  constexpr int RING = 4;      // operand reads in flight ahead of their MFMA
+
+  pf32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) o[db] = pf32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+
+  Tile c1, c2;
+  uint64_t there;  // of the tile whose scores are next
+  {
+    const Tile c0 = locate(t0);
+    issue(c0, kh, sK0, false);
+    issue(c0, vh, sV0, true);
+    there = c0.there;
+  }
+  c1 = locate(t0 + 1);
+  if (t0 + 1 < t_end) issue(c1, kh, sK1, false);
+  c2 = locate(t0 + 2);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+
+  // Masks scores by the keys of the tile that this lane's row sees.
+  auto mask_by = [&](uint64_t bits, pf32x16* S) {
+    const uint32_t m_lo = (uint32_t)bits >> (4 * hh), m_hi = (uint32_t)(bits >> 32) >> (4 * hh);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        S[kb][e] = ((kb ? m_hi : m_lo) >> (8 * (e >> 2) + (e & 3))) & 1 ? S[kb][e] : -INFINITY;
+  };
+  uint64_t bits = 0;  // of the tile whose scores were masked last, where it is a tree tile
+  auto mask_tile = [&](int t, pf32x16* S) {
+    if (t >= tree0) {
+      bits = there & (((uint64_t)tree_bits(P, it, node, t * KT + 32) << 32) | tree_bits(P, it, node, t * KT));
+      mask_by(bits, S);
+    } else if (there != ~0ull) {
+      mask_by(there, S);
+    }
+  };
+  float ms = 0.f;  // exponent offset of the current tile: m_run, or 0 while m_run is -inf
+  auto take_max = [&](float bm) {  // the running max takes a tile's max into account, o and l follow
+    bm = half_max(bm) * P.scale2;  // scale > 0
+    const float m_old = m_run;
+    m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
+    ms = m_run == -INFINITY ? 0.f : m_run;
+    if (__ballot(m_run != m_old)) {
+      const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= alpha;
+    }
+  };
+  auto scores = [&](const char* sk, int t, pf32x16* S) {  // not interleaved: the first tile and tree tiles
+    int kx = kx0;
+    asm volatile("" : "+v"(kx));
+#pragma unroll
+    for (int i = 0; i < NKS; ++i) S[i & 1] = PMfma<DT>::run(kread(sk, i, kx), qb[i >> 1], i < 2 ? pf32x16{} : S[i & 1]);
+    mask_tile(t, S);
+    float bm = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bm = fmaxf(bm, S[kb][e]);
+    take_max(bm);
+  };
+
+  pf32x16 S[2], S2[2];
+  int t = t0;
+  if (active) scores(sK0, t, S);
+  __syncthreads();  // K stage 0 is refilled below
+
+  // Stages K(t+2) over K(t) and V(t+1), and moves on the places.
+  auto stage_next = [&](char* kcur, char* vnxt) {
+    asm volatile("" : "+v"(my_key));  // the pieces are worked out anew in each tile
+    if (t + 2 < t_end) issue(c2, kh, kcur, false);
+    if (t + 1 < t_end) issue(c1, vh, vnxt, true);
+    there = c1.there;
+    c1 = c2;
+    c2 = locate(t + 3);
+  };
+  auto end_tile = [&]() {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's loads of K(t+2) and V(t+1) have landed
+    __syncthreads();                // every wave's have; tile t's stages are free
+    ++t;
+  };
+  // A tile whose next one has committed rows only.
+  auto step = [&](auto stage_c, pf32x16* S, pf32x16* Sn) {
+    constexpr int stage = decltype(stage_c)::value;
+    char* const kcur = stage ? sK1 : sK0;  // K(t), scored; receives K(t+2)
+    char* const knxt = stage ? sK0 : sK1;  // K(t+1)
+    char* const vcur = stage ? sV1 : sV0;  // V(t)
+    char* const vnxt = stage ? sV0 : sV1;  // receives V(t+1)
+    stage_next(kcur, vnxt);
+    if (active) {
+      // Both blocks are issued in source order (a scheduling barrier after
+      // each MFMA step): every MFMA's operand was read RING steps earlier, and
+      // the VALU work is spread evenly between the MFMAs.
+      int kx = kx0, vx = vx0;
+      asm volatile("" : "+v"(kx), "+v"(vx));
+      uint4 kr[RING], vr[RING];
+#pragma unroll
+      for (int i = 0; i < RING; ++i) kr[i] = kread(knxt, i, kx);
+      constexpr int EPM = 32 / NKS;  // exponentials per score MFMA
+      uint32_t pw[16];               // P^T: key step 2 kb + u, words 4 (2 kb + u) .., holds keys 16 u + {4 h + j, 8 + 4 h + j} of block kb
+      float psum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NKS; ++i) {
+        Sn[i & 1] = PMfma<DT>::run(kr[i % RING], qb[i >> 1], i < 2 ? pf32x16{} : Sn[i & 1]);
+        if (i + RING < NKS) kr[i % RING] = kread(knxt, i + RING, kx);
+#pragma unroll
+        for (int x = 0; x < EPM; x += 2) {
+          const int w = (i * EPM + x) / 2, e = 2 * (w & 7);
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[w >> 3][e], P.scale2, -ms));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[w >> 3][e + 1], P.scale2, -ms));
+          psum += p0;
+          psum += p1;
+          pw[w] = PMfma<DT>::pack(p0, p1);
+          // keeps the exponentials in this block
+          asm volatile("" : "+v"(pw[w]));
+        }
+        // keeps the additions next to their exponentials
+        asm volatile("" : "+v"(psum));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      l_run += psum;
+      if (there != ~0ull) mask_by(there, Sn);
+
+      constexpr int MPM = 32 / NPV;  // score elements folded into the max per output MFMA
+      float bm = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < RING; ++i) vr[i] = vread(vcur, i, vx);
+#pragma unroll
+      for (int i = 0; i < NPV; ++i) {
+        const uint32_t* pb = pw + 4 * (i / DB);
+        o[i % DB] = PMfma<DT>::run(vr[i % RING], make_uint4(pb[0], pb[1], pb[2], pb[3]), o[i % DB]);
+        if (i + RING < NPV) vr[i % RING] = vread(vcur, i + RING, vx);
+#pragma unroll
+        for (int x = 0; x < MPM; ++x) {
+          const int e = i * MPM + x;
+          bm = fmaxf(bm, Sn[e >> 4][e & 15]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      take_max(bm);
+    }
+    end_tile();
+  };
+  // Steps in pairs, which leaves the stages and the scores where they were.
+  const int t_steps = min(t_end, tree0) - 1;  // tiles before the last one, and before a tree tile
+  while (t + 2 <= t_steps) {
+    step(std::integral_constant<int, 0>(), S, S2);
+    step(std::integral_constant<int, 1>(), S2, S);
+  }
+  // The last tile or two and the tree tiles, one product behind the other.
+  int stage = 0;
+  for (; t < t_end; stage ^= 1) {
+    char* const vcur = stage ? sV1 : sV0;
+    stage_next(stage ? sK1 : sK0, stage ? sV0 : sV1);
+    // Tree rows whose values are not finite reach the rows that see them and are zeroed for the product.
+    // Every wave finds the same: it reads the tile before any of them changes it.
+    if (t >= tree0 && tree_v_odd<DT>(vcur, TB, lane)) {
+      if (active) tree_v_add_odd<DT, D>(o, vcur, bits, KT, hh, [&](int k) { return lds_row(k) * RB; });
+      __syncthreads();
+      tree_v_clean<DT>(vcur, TB, threadIdx.x * 16, NW * 1024);
+      __syncthreads();
+    }
+    if (active) {
+      int vx = vx0;
+      asm volatile("" : "+v"(vx));
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        uint4 pb[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][8 * u + e], P.scale2, -ms));
+            l_run += p[e];
+          }
+          pb[u] = make_uint4(PMfma<DT>::pack(p[0], p[1]), PMfma<DT>::pack(p[2], p[3]), PMfma<DT>::pack(p[4], p[5]),
+                             PMfma<DT>::pack(p[6], p[7]));
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * DB; ++i) o[i % DB] = PMfma<DT>::run(vread(vcur, kb * 2 * DB + i, vx), pb[i / DB], o[i % DB]);
+      }
+      if (t + 1 < t_end) scores(stage ? sK0 : sK1, t + 1, S);
+    }
+    end_tile();
+  }
+
+  if (r_lane >= RG) return;
+  const float lt = half_sum(l_run);
+  if (it.cuts > 1) {
+    const int64_t pw = (int64_t)(it.part + it.cut) * NW + wave;
+    float4* po = P.part_o + pw * (DB * 4 * 64) + lane;
+#pragma unroll
+    for (int x = 0; x < 4 * DB; ++x)
+      po[x * 64] = make_float4(o[x / 4][4 * (x & 3)], o[x / 4][4 * (x & 3) + 1], o[x / 4][4 * (x & 3) + 2],
+                               o[x / 4][4 * (x & 3) + 3]);
+    if (hh == 0) P.part_ml[pw * 32 + qc] = make_float2(m_run, lt);
+    return;
+  }
+  const float inv = tree_inv(lt);
+  const int64_t at = (it.lo + node) * P.o_stride_n + head * P.o_stride_h;
+#pragma unroll
+  for (int x = 0; x < 4 * DB; ++x) {
+    float v4[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v4[j] = o[x / 4][4 * (x & 3) + j] * inv;
+    tree_store4(P, at + tree_channel<D, false>(x, hh), v4);
+  }
+  if (P.lse != nullptr && hh == 0) P.lse[(int64_t)(it.lo + node) * P.H + head] = tree_lse(m_run, lt);
+}
+
 // Merge of a unit's partials: with M the largest of a row's maxima, out = sum_c
 // 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.  One workgroup folds four pieces of
-// a unit, its waves every fourth partial each; the order is fixed.
-template <int D, bool F32>
+// 32 rows, its waves every fourth partial each; the order is fixed.
+template <int D, bool F32, int KT, int NW>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
   constexpr int PIECES = D / 8, PPW = 4;
   __shared__ float4 s_o[kTreeWaves][PPW][64];
   __shared__ float2 s_ml[kTreeWaves][32];
   TreeItem it;
-  if (!tree_find<kTreeKT, kTreeRows, false>(P, blockIdx.x, it) || it.cuts <= 1) return;
+  const int rows32 = NW == 1 ? 0 : blockIdx.x % NW;  // which 32 of the unit's rows
+  if (!tree_find<KT, 32 * NW, false>(P, blockIdx.x / NW, it) || it.cuts <= 1) return;
+  const int row0 = (it.rb * NW + rows32) * 32;
+  if (row0 >= it.n * P.rep) return;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
   const int x0 = blockIdx.y * PPW;
-  const int r = it.rb * kTreeRows + qc;
+  const int r = row0 + qc;
   const bool live = r < it.n * P.rep;
   float m = -INFINITY, l = 0.f;
   float4 acc[PPW];
@@ -934,7 +1245,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
   if (live) {
 #pragma unroll 4
     for (int c = wave; c < it.cuts; c += kTreeWaves) {
-      const int64_t pu = it.part + c;
+      const int64_t pu = (int64_t)(it.part + c) * NW + rows32;
       const float2 ml = P.part_ml[pu * 32 + qc];
       float4 v[PPW];
 #pragma unroll
@@ -986,33 +1297,37 @@ using namespace halo;
 
 namespace {
 
-// How a call is cut: units at most, workgroups that the GPU holds, launch size, partials at most.
+// How a call is cut: 32-row waves that share a unit's tiles (1: the narrow
+// kernel), units at most, workgroups that the GPU holds, launch size, partials
+// at most.
 struct TreeShape {
+  int nw, kt, slots, min_tiles;
   int64_t units, grid, partials;
-  int slots, min_tiles;
   bool merge;
 };
 TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows, int max_nodes) {
   TreeShape s;
   const int64_t rows = (int64_t)max_nodes * (H / H_kv);
-  s.units = (int64_t)B * H_kv * ((rows + kTreeRows - 1) / kTreeRows);
-  // by the LDS of a workgroup (16 bits: 64 and 32 KiB at D = 128 and 64, fp32 twice that) and 2 waves a SIMD
-  s.slots = 256 * (dtype == HALO_F32 && D == 128 ? 1 : 2);
-  s.min_tiles = kTreeWaves;
-  const int64_t longest = (max_rows + max_nodes + kTreeKT - 1) / kTreeKT;
+  s.nw = dtype == HALO_F32 || rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+  s.kt = s.nw == 1 ? kTreeKT : kTreeWideKT;
+  s.units = (int64_t)B * H_kv * ((rows + 32 * s.nw - 1) / (32 * s.nw));
+  // by the LDS of a workgroup (64 KiB at D = 128, 32 KiB at D = 64, the fp32 kernel's twice that) and 2 waves a SIMD
+  s.slots = 256 * (s.nw == 8 || (dtype == HALO_F32 && D == 128) ? 1 : 2);
+  s.min_tiles = s.nw == 1 ? kTreeWaves : 2;
+  const int64_t longest = (max_rows + max_nodes + s.kt - 1) / s.kt;
   s.merge = longest > s.min_tiles;
   // tree_find: at most `room` items besides one a unit
   s.grid = s.merge ? (s.slots / 2 + s.units > s.slots ? s.slots / 2 + s.units : s.slots) : s.units;
-  s.partials = s.merge ? s.slots : 0;
+  s.partials = s.merge ? (int64_t)s.slots * s.nw : 0;
   return s;
 }
 
-int64_t tree_part_bytes(int D) { return (int64_t)kTreeRows * D * 4 + kTreeRows * 8; }
+int64_t tree_part_bytes(int D) { return 32ll * D * 4 + 32 * 8; }
 
 bool tree_sizes_ok(int B, int H, int H_kv, int D, int64_t max_rows, int max_nodes) {
   return B > 0 && H > 0 && H_kv > 0 && H % H_kv == 0 && (D == 64 || D == 128) && max_rows > 0 &&
          max_rows < (1ll << 31) - 1024 && max_nodes > 0 && max_nodes <= 512 && (int64_t)max_nodes * (H / H_kv) < (1 << 24) &&
-         (int64_t)B * H_kv * ((int64_t)max_nodes * (H / H_kv) / kTreeRows + 1) < (1ll << 30);
+         (int64_t)B * H_kv * ((int64_t)max_nodes * (H / H_kv) / 32 + 8) < (1ll << 30);
 }
 
 }  // namespace
@@ -1096,28 +1411,34 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   p.out_vec4 = reinterpret_cast<uintptr_t>(out) % ea == 0 && (out_stride_n * eo) % ea == 0 && (out_stride_h * eo) % ea == 0;
   p.lse = lse;
   p.part_o = reinterpret_cast<float4*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * kTreeRows * (D / 4));
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * 32 * (D / 4));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)s.grid), block(64 * kTreeWaves), mgrid((unsigned)s.units, D / 32);
-#define HALO_TREE(KERNEL, DV, F32V)                                                                       \
-  do {                                                                                                    \
-    hipLaunchKernelGGL((KERNEL), grid, block, 0, st, p);                                                  \
-    if (s.merge) hipLaunchKernelGGL((tree_merge_kernel<DV, F32V>), mgrid, dim3(256), 0, st, p);           \
+  const dim3 grid((unsigned)s.grid), block(64 * (s.nw == 1 ? kTreeWaves : s.nw)), mgrid((unsigned)(s.units * s.nw), D / 32);
+#define HALO_TREE(KERNEL, DV, F32V, KTV, NWV)                                                                      \
+  do {                                                                                                             \
+    hipLaunchKernelGGL((KERNEL), grid, block, 0, st, p);                                                           \
+    if (s.merge) hipLaunchKernelGGL((tree_merge_kernel<DV, F32V, KTV, NWV>), mgrid, dim3(256), 0, st, p);          \
   } while (0)
-#define HALO_TREE16(DTV)                                                  \
-  do {                                                                    \
-    if (D == 128) HALO_TREE((tree_attn_kernel<DTV, 128>), 128, false);    \
-    else HALO_TREE((tree_attn_kernel<DTV, 64>), 64, false);               \
+#define HALO_TREE_WIDE(DTV, DV, NWV) HALO_TREE((tree_attn_wide_kernel<DTV, DV, NWV>), DV, false, kTreeWideKT, NWV)
+#define HALO_TREE16(DTV, DV)                                                                     \
+  do {                                                                                           \
+    if (s.nw == 1) HALO_TREE((tree_attn_kernel<DTV, DV>), DV, false, kTreeKT, 1);                \
+    else if (s.nw == 2) HALO_TREE_WIDE(DTV, DV, 2);                                              \
+    else if (s.nw == 4) HALO_TREE_WIDE(DTV, DV, 4);                                              \
+    else HALO_TREE_WIDE(DTV, DV, 8);                                                             \
   } while (0)
   if (dtype == HALO_F32) {
-    if (D == 128) HALO_TREE((tree_attn_f32_kernel<128>), 128, true);
-    else HALO_TREE((tree_attn_f32_kernel<64>), 64, true);
+    if (D == 128) HALO_TREE((tree_attn_f32_kernel<128>), 128, true, kTreeKT, 1);
+    else HALO_TREE((tree_attn_f32_kernel<64>), 64, true, kTreeKT, 1);
   } else if (dtype == HALO_BF16) {
-    HALO_TREE16(HALO_BF16);
+    if (D == 128) HALO_TREE16(HALO_BF16, 128);
+    else HALO_TREE16(HALO_BF16, 64);
   } else {
-    HALO_TREE16(HALO_F16);
+    if (D == 128) HALO_TREE16(HALO_F16, 128);
+    else HALO_TREE16(HALO_F16, 64);
   }
 #undef HALO_TREE16
+#undef HALO_TREE_WIDE
 #undef HALO_TREE
   HALO_CHECK_HIP(hipGetLastError());
   return HALO_OK;
