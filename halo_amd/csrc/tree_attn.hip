@@ -48,7 +48,7 @@ struct TreeParams {
   float scale2;
   void* out;
   int64_t o_stride_n, o_stride_h;
-  int out_dtype, out_vec4;
+  int out_f32;
   float* lse;
   float4* part_o;
   float2* part_ml;
@@ -315,13 +315,11 @@ __device__ __forceinline__ void tree_v_add_odd(pf32x16* o, const char* sv, uint6
   }
 }
 
+// Four channels of a row of out, which is of the queries' type or fp32.
+template <int DT>
 __device__ __forceinline__ void tree_store4(const TreeParams& P, int64_t at, const float* v4) {
-  if (P.out_vec4) {
-    store_elem4(P.out, at, P.out_dtype, v4);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) store_elem(P.out, at + j, P.out_dtype, v4[j]);
-  }
+  if (DT == HALO_F32 || P.out_f32) store_elem4(P.out, at, HALO_F32, v4);
+  else store_elem4(P.out, at, DT, v4);
 }
 
 // First channel of the four that piece x of lane half hh holds.  16-bit kernel,
@@ -435,7 +433,7 @@ __device__ __forceinline__ char* tree_piece(char* k, char* v, int x) {
 
 // The four waves of a workgroup hold (m, l, o) of the same 32 rows over
 // different tiles; each folds a quarter of the pieces.
-template <int D, bool F32, int TB>
+template <int D, int DT, int TB>
 __device__ __forceinline__ void tree_fold_store(const TreeParams& P, const TreeItem& it, int wave, int lane,
                                                 float2 (*s_ml)[32], char (*sK)[TB], char (*sV)[TB]) {
   constexpr int PIECES = D / 8, PER = PIECES / kTreeWaves;
@@ -472,7 +470,7 @@ __device__ __forceinline__ void tree_fold_store(const TreeParams& P, const TreeI
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] *= inv;
-      tree_store4(P, row * P.o_stride_n + head * P.o_stride_h + tree_channel<D, F32>(x, hh), v);
+      tree_store4<DT>(P, row * P.o_stride_n + head * P.o_stride_h + tree_channel<D, DT == HALO_F32>(x, hh), v);
     }
   }
   if (wave == 0 && hh == 0) {
@@ -705,7 +703,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     *reinterpret_cast<float4*>(tree_piece<D>(stK, stV, x) + lane * 16) =
         make_float4(o[x / 4][4 * (x & 3)], o[x / 4][4 * (x & 3) + 1], o[x / 4][4 * (x & 3) + 2], o[x / 4][4 * (x & 3) + 3]);
   __syncthreads();
-  tree_fold_store<D, false, TB>(P, it, wave, lane, s_ml, sK, sV);
+  tree_fold_store<D, DT, TB>(P, it, wave, lane, s_ml, sK, sV);
 }
 
 // fp32 queries and pools: the same walk on v_mfma_f32_32x32x2 (fp32 products
@@ -912,7 +910,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
           make_float4(x[0], x[1], x[2], x[3]);
     }
   __syncthreads();
-  tree_fold_store<D, true, TB>(P, it, wave, lane, s_ml, sK, sV);
+  tree_fold_store<D, HALO_F32, TB>(P, it, wave, lane, s_ml, sK, sV);
 }
 
 // More than 32 rows a unit, 16 bits: NW waves of 32 rows each share every K/V
@@ -1214,7 +1212,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
     float v4[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v4[j] = o[x / 4][4 * (x & 3) + j] * inv;
-    tree_store4(P, at + tree_channel<D, false>(x, hh), v4);
+    tree_store4<DT>(P, at + tree_channel<D, false>(x, hh), v4);
   }
   if (P.lse != nullptr && hh == 0) P.lse[(int64_t)(it.lo + node) * P.H + head] = tree_lse(m_run, lt);
 }
@@ -1222,7 +1220,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 // Merge of a unit's partials: with M the largest of a row's maxima, out = sum_c
 // 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.  One workgroup folds four pieces of
 // 32 rows, its waves every fourth partial each; the order is fixed.
-template <int D, bool F32, int KT, int NW>
+template <int D, int DT, int KT, int NW>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
   constexpr int PIECES = D / 8, PPW = 4;
   __shared__ float4 s_o[kTreeWaves][PPW][64];
@@ -1287,7 +1285,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
   const float v4[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
   const int node = r / P.rep, head = it.h * P.rep + (r - node * P.rep);
   const int64_t row = it.lo + node;
-  tree_store4(P, row * P.o_stride_n + head * P.o_stride_h + tree_channel<D, F32>(x0 + wave, hh), v4);
+  tree_store4<DT>(P, row * P.o_stride_n + head * P.o_stride_h + tree_channel<D, DT == HALO_F32>(x0 + wave, hh), v4);
   if (P.lse != nullptr && blockIdx.y == 0 && wave == 0 && hh == 0) P.lse[row * P.H + head] = tree_lse(M, l);
 }
 
@@ -1345,7 +1343,7 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   HALO_CHECK_ARG(pool && pool->k && pool->v && table && lengths && cu_nodes, "null pointer argument");
   const int dtype = pool->dtype, D = pool->D, H_kv = pool->H_kv;
   HALO_CHECK_ARG(dtype == HALO_BF16 || dtype == HALO_F16 || dtype == HALO_F32, "dtype must be bf16, f16 or f32");
-  HALO_CHECK_ARG(out_dtype == HALO_F32 || out_dtype == HALO_BF16 || out_dtype == HALO_F16, "bad out_dtype");
+  HALO_CHECK_ARG(out_dtype == HALO_F32 || out_dtype == dtype, "out must be of q's type or fp32");
   HALO_CHECK_ARG(pool->layers == 1 && pool->blocks > 0 && pool->block_size > 0 && W > 0, "need a pool of one layer");
   HALO_CHECK_ARG(D == 64 || D == 128, "head_dim must be 64 or 128");
   HALO_CHECK_ARG(N >= 0, "bad number of nodes");
@@ -1359,6 +1357,9 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   const int64_t lanes = 16 / es;  // elements of a 16-byte piece
   HALO_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(q_stride_n * es) | (uintptr_t)(q_stride_h * es)) % 16 == 0,
                  "q rows must be 16-byte aligned");
+  const int64_t ea = 4 * elem_size(out_dtype);
+  HALO_CHECK_ARG(reinterpret_cast<uintptr_t>(out) % ea == 0 && out_stride_n % 4 == 0 && out_stride_h % 4 == 0,
+                 "out rows must be aligned to four elements");
   HALO_CHECK_ARG((reinterpret_cast<uintptr_t>(pool->k) | reinterpret_cast<uintptr_t>(pool->v)) % 16 == 0 &&
                      pool->stride_b % lanes == 0 && pool->stride_h % lanes == 0 && pool->stride_r % lanes == 0,
                  "pool rows must be 16-byte aligned");
@@ -1406,30 +1407,28 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   p.out = out;
   p.o_stride_n = out_stride_n;
   p.o_stride_h = out_stride_h;
-  p.out_dtype = out_dtype;
-  const int64_t ea = out_dtype == HALO_F32 ? 16 : 8, eo = elem_size(out_dtype);
-  p.out_vec4 = reinterpret_cast<uintptr_t>(out) % ea == 0 && (out_stride_n * eo) % ea == 0 && (out_stride_h * eo) % ea == 0;
+  p.out_f32 = out_dtype == HALO_F32;
   p.lse = lse;
   p.part_o = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * 32 * (D / 4));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)s.grid), block(64 * (s.nw == 1 ? kTreeWaves : s.nw)), mgrid((unsigned)(s.units * s.nw), D / 32);
-#define HALO_TREE(KERNEL, DV, F32V, KTV, NWV)                                                                      \
+#define HALO_TREE(KERNEL, DV, DTV, KTV, NWV)                                                                      \
   do {                                                                                                             \
     hipLaunchKernelGGL((KERNEL), grid, block, 0, st, p);                                                           \
-    if (s.merge) hipLaunchKernelGGL((tree_merge_kernel<DV, F32V, KTV, NWV>), mgrid, dim3(256), 0, st, p);          \
+    if (s.merge) hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV>), mgrid, dim3(256), 0, st, p);          \
   } while (0)
-#define HALO_TREE_WIDE(DTV, DV, NWV) HALO_TREE((tree_attn_wide_kernel<DTV, DV, NWV>), DV, false, kTreeWideKT, NWV)
+#define HALO_TREE_WIDE(DTV, DV, NWV) HALO_TREE((tree_attn_wide_kernel<DTV, DV, NWV>), DV, DTV, kTreeWideKT, NWV)
 #define HALO_TREE16(DTV, DV)                                                                     \
   do {                                                                                           \
-    if (s.nw == 1) HALO_TREE((tree_attn_kernel<DTV, DV>), DV, false, kTreeKT, 1);                \
+    if (s.nw == 1) HALO_TREE((tree_attn_kernel<DTV, DV>), DV, DTV, kTreeKT, 1);                \
     else if (s.nw == 2) HALO_TREE_WIDE(DTV, DV, 2);                                              \
     else if (s.nw == 4) HALO_TREE_WIDE(DTV, DV, 4);                                              \
     else HALO_TREE_WIDE(DTV, DV, 8);                                                             \
   } while (0)
   if (dtype == HALO_F32) {
-    if (D == 128) HALO_TREE((tree_attn_f32_kernel<128>), 128, true, kTreeKT, 1);
-    else HALO_TREE((tree_attn_f32_kernel<64>), 64, true, kTreeKT, 1);
+    if (D == 128) HALO_TREE((tree_attn_f32_kernel<128>), 128, HALO_F32, kTreeKT, 1);
+    else HALO_TREE((tree_attn_f32_kernel<64>), 64, HALO_F32, kTreeKT, 1);
   } else if (dtype == HALO_BF16) {
     if (D == 128) HALO_TREE16(HALO_BF16, 128);
     else HALO_TREE16(HALO_BF16, 64);

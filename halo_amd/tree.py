@@ -91,16 +91,26 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         if qs[2] != 1 or qs[0] % per or qs[1] % per or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
             qs = q.stride()
-        if out is None:
-            out = torch.empty((N, H, D), device=dev, dtype=out_dtype or q.dtype)
+        want = out.dtype if out is not None else out_dtype or q.dtype
+        # the kernel writes q's type or fp32, rows aligned to four elements
+        o = out
+        if out is None or (want != q.dtype and want != torch.float32) or out.data_ptr() % (4 * out.element_size()) \
+                or out.stride(0) % 4 or out.stride(1) % 4:
+            o = torch.empty((N, H, D), device=dev, dtype=want if want == q.dtype else torch.float32)
+            if out is not None:
+                o.copy_(out)  # for the rows that are not written
         if return_lse and lse is None:
             lse = torch.empty((N, H), device=dev, dtype=torch.float32)
         W = block_table.shape[1]
         nbytes = L.halo_tree_workspace_size(nat.dtype_code(q.dtype), B, H, shape[1], D, W * shape[2], max_nodes)
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-        os_ = out.stride()
+        os_ = o.stride()
         nat.check(L.halo_tree_attn(
             pool, q.data_ptr(), qs[0], qs[1], N, H, block_table.data_ptr(), block_table.stride(0) if B > 1 else W, B, W,
-            lengths.data_ptr(), cu_nodes.data_ptr(), max_nodes, nat.ptr(mask), words, scale, out.data_ptr(), os_[0],
-            os_[1], nat.dtype_code(out.dtype), nat.ptr(lse), nat.ptr(ws), nbytes, nat.stream_ptr()), "halo_tree_attn")
+            lengths.data_ptr(), cu_nodes.data_ptr(), max_nodes, nat.ptr(mask), words, scale, o.data_ptr(), os_[0],
+            os_[1], nat.dtype_code(o.dtype), nat.ptr(lse), nat.ptr(ws), nbytes, nat.stream_ptr()), "halo_tree_attn")
+        if out is None:
+            out = o if o.dtype == want else o.to(want)
+        elif o is not out:
+            out.copy_(o)
     return (out, lse) if return_lse else out

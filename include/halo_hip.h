@@ -570,7 +570,8 @@ int halo_tree_layout(const int32_t* parents, const int32_t* cu_nodes, int B, int
 /*
  * Attention of drafted trees over a paged cache.  Node i of request b is row
  * cu_nodes[b] + i of q and out (N, H, D; element strides, q rows 16-byte
- * aligned) and of lse (N, H fp32, or NULL); it attends the request's rows
+ * aligned; out of q's type or fp32, rows aligned to four elements) and of lse
+ * (N, H fp32, or NULL); it attends the request's rows
  * [0, lengths[b]) and the tree rows lengths[b] + j whose bit j is set in its
  * mask row (see halo_tree_layout; NULL: j <= i), each of the request's K/V
  * rows through its block table (B, W; rows table_stride apart).  Rows in a

@@ -218,7 +218,7 @@ def _attn(lib, pool=None, **kw):
     dict(pool=_pool(k=4104)), dict(pool=_pool(sr=68)), dict(pool=_pool(sb=-2048)), dict(pool=_pool(bs=0)),
     dict(pool=_pool(blocks=2 ** 31 - 1, sb=2 ** 40)), dict(H=5), dict(H=0), dict(B=0), dict(W=0), dict(max_nodes=0),
     dict(max_nodes=513), dict(q=4100), dict(q=None), dict(qn=257), dict(table=None), dict(ts=2), dict(W=2 ** 28, ts=2 ** 28),
-    dict(mask=4096, ms=0), dict(scale=0.0), dict(scale=float("nan")), dict(scale=1e-42), dict(out=None), dict(odt=7),
+    dict(mask=4096, ms=0), dict(scale=0.0), dict(scale=float("nan")), dict(scale=1e-42), dict(out=None), dict(odt=7), dict(odt=2), dict(out=4100), dict(on=258), dict(oh=65),
     dict(N=-1), dict(W=3000, ts=3000)])
 def test_tree_attn_entry_refuses(entries, kw):
     assert _attn(entries, **kw) == -1
