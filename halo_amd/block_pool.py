@@ -51,6 +51,41 @@ class BlockUpdate(NamedTuple):
     ok: torch.Tensor
 
 
+def load_calls(path=None):
+    """The prebuilt host extension (halo_amd/_lib/poolcalls_build, made by
+    build()) that checks, allocates and calls in C++, bound to the library; None
+    when it is missing or cannot be loaded.  Its functions return None for a call
+    that they do not take, which then runs (or is refused) here."""
+    import ctypes
+    import importlib.util
+    import os
+    if path is None:
+        path = os.path.join(os.path.dirname(nat.library_path()), "poolcalls_build", "_halo_poolcalls.so")
+    if not os.path.exists(path) or not nat.available():
+        return None
+    try:
+        spec = importlib.util.spec_from_file_location("_halo_poolcalls", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind(*[ctypes.cast(getattr(nat.lib(), "halo_" + n), ctypes.c_void_p).value for n in
+                   ("update_block_tables", "append_rows", "tree_layout", "tree_workspace_size", "tree_attn",
+                    "commit_path")])
+        return mod
+    except (ImportError, OSError, AttributeError):
+        # built against another torch, or not a loadable module: the calls are made in Python (same results, slower)
+        return None
+
+
+calls = load_calls()
+
+
+def called(r, what: str):
+    """What a function of ``calls`` returned, unless it is a status below 0."""
+    if type(r) is int:
+        nat.check(r, what)
+    return r
+
+
 class _Here:
     """Enters nothing: the call's device and stream are the current ones."""
 
@@ -135,6 +170,10 @@ def update_block_tables(block_table: torch.Tensor, n_blocks: torch.Tensor, free_
     it has, its rows' slots are -1 and its ``ok`` is False.  New rows are
     numbered request after request; ``max_rows`` is the room for their slots
     (rows past it get none, places behind the last row are -1)."""
+    if calls is not None and stream is None:
+        r = calls.update_block_tables(block_table, n_blocks, free_blocks, n_free, lengths, first, block_size, max_rows)
+        if r is not None:
+            return BlockUpdate(*called(r, "halo_update_block_tables"))
     L = nat.lib()
     dev = block_table.device
     B = lengths.numel()
@@ -169,6 +208,11 @@ def append_rows(k_new: torch.Tensor, v_new: torch.Tensor, slots: torch.Tensor, k
     ``slots[i]`` (int64) of the pools ([L,] blocks, H_kv, block_size, D), in
     every layer.  Rows whose slot is negative or past the pool are skipped.
     Slots must differ: which of two rows with one slot stays is not defined."""
+    if calls is not None and stream is None:
+        r = calls.append_rows(k_new, v_new, slots, k_pool, v_pool)
+        if r is not None:
+            called(r, "halo_append_rows")
+            return
     L = nat.lib()
     pool = pack_pool(k_pool, v_pool, written=True)
     dev = k_pool.device
@@ -199,6 +243,10 @@ def tree_layout(parents: torch.Tensor, cu_nodes: torch.Tensor, *, max_nodes: int
     j of a node's words set for itself and its ancestors, and ``depth`` (N)
     int32, the number of ancestors.  Entries of no tree (a padded batch) are not
     written; ``mask`` and ``depth`` may be given."""
+    if calls is not None and stream is None and mask is None and depth is None:
+        r = calls.tree_layout(parents, cu_nodes, max_nodes)
+        if r is not None:
+            return called(r, "halo_tree_layout")
     L = nat.lib()
     dev = parents.device
     N, B, words = parents.numel(), cu_nodes.numel() - 1, (max_nodes + 63) // 64
@@ -233,6 +281,10 @@ def commit_path(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     ``path`` (B, P <= 64) int32 rises; it ends at the first entry that does not,
     or whose row the table does not hold.  Returns the new lengths (B) int32,
     in ``out`` if given (not ``lengths`` itself)."""
+    if calls is not None and stream is None:
+        r = calls.commit_path(k_pool, v_pool, block_table, lengths, path, n_path, out)
+        if r is not None:
+            return called(r, "halo_commit_path")
     L = nat.lib()
     pool = pack_pool(k_pool, v_pool, written=True)
     dev = k_pool.device

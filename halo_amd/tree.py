@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from . import _native as nat
+from . import block_pool as pool_calls
 from .block_pool import MAX_NODES, check_ints, check_table, on_stream, overlap, pack_pool
 
 
@@ -45,6 +46,11 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     ``return_lse`` lse (N, H) fp32, both in ``out`` and ``lse`` if given; rows of
     no request are not written.  The softmax and all sums are fp32; for 16-bit
     pools its weights are rounded once to the pool's type."""
+    if pool_calls.calls is not None and stream is None and out_dtype is None:
+        r = pool_calls.calls.tree_attention(q, k_pool, v_pool, block_table, lengths, cu_nodes, max_nodes, mask, scale,
+                                            out, lse, return_lse)
+        if r is not None:
+            return pool_calls.called(r, "halo_tree_attn")
     L = nat.lib()
     if q.dim() != 3:
         raise AssertionError(f"q must be (N, H, D), got {tuple(q.shape)}")
