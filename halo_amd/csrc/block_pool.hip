@@ -16,17 +16,19 @@ namespace {
 // ---------------------------------------------------------------------------
 // Block tables and slots.  need_b = ceil(length_b / block_size); surplus
 // blocks go back first, then requests take theirs in order.  With R_b, G_b
-// and C_b the sums over b' < b of blocks given back, blocks taken and new rows,
+// and C_b the sums over b' < b of blocks given back, blocks wanted and new rows,
 // every moved id and every slot has a place of its own:
-//   entry j of b goes to   free[n_free + R - R_{b+1} + own_b - 1 - j],
+//   entry j of b goes to   free[n_free + R - 1 - (R_b + j - need_b)],
 //   entry j of b comes from free[n_free + R - 1 - (G_b + j - own_b)],
 //   new row r has           b = the last one with C_b <= r.
-// One workgroup, since the free list is one stack: it is bound by the chain
-// lengths -> sums -> ids -> slots, not by bytes.  The ids of a chunk of
-// requests are spread over the threads by a search in the chunk's sums, so one
-// long request does not hold up the others.
+// (Requests that are served and grow come before those that want blocks and are
+// not, so G_b counts no block that stays.)  One workgroup, since the free list
+// is one stack: it is bound by the chain lengths -> sums -> ids -> slots, not by
+// bytes.  The ids of 1024 requests are spread over the threads by a search in
+// their sums, so one long request does not hold up the others.
 // ---------------------------------------------------------------------------
 constexpr int kTabThreads = 1024;
+constexpr int kTabBatch = 4;  // ids a thread has in flight
 
 struct TableParams {
   int32_t* table;
@@ -46,45 +48,57 @@ struct TableParams {
 };
 
 struct TabReq {
-  int own, need, first, len;  // blocks it has and needs, new rows [first, len)
+  int own, need, rows;  // blocks it has and needs, new rows
+  __device__ __forceinline__ int back() const { return max(own - need, 0); }
+  __device__ __forceinline__ int grow(int W) const { return need <= W ? max(need - own, 0) : 0; }
 };
 __device__ __forceinline__ TabReq tab_req(const TableParams& P, int b) {
-  TabReq r = {0, 0, 0, 0};
+  TabReq r = {0, 0, 0};
   if (b < P.B) {
-    r.len = max(P.lengths[b], 0);
-    r.first = max(P.first[b], 0);
+    const int len = max(P.lengths[b], 0);
+    r.rows = max(len - max(P.first[b], 0), 0);
     r.own = min(max(P.n_blocks[b], 0), P.W);
-    r.need = div_by(r.len, P.bs);
-    if (r.need * P.bs.d < r.len) ++r.need;
+    r.need = div_by(len, P.bs);
+    if (r.need * P.bs.d < len) ++r.need;
   }
   return r;
 }
 
-// Exclusive sum over the workgroup's threads; `total` gets the whole sum.
-__device__ __forceinline__ int64_t tab_scan(int64_t v, int64_t* wave_sums, int64_t& total) {
+// Exclusive sums over the workgroup's threads, and the whole sums.  Blocks of
+// all requests number below 2^31, rows may not.
+struct TabSums {
+  int back, grow, all_back, all_grow;
+  int64_t rows, all_rows;
+};
+struct TabWave {
+  int back, grow;
+  int64_t rows;
+};
+__device__ __forceinline__ TabSums tab_scan(int back, int grow, int rows, TabWave* s_wave) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t x = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
+  const int xb = wave_prefix(back), xg = wave_prefix(grow);
+  const int64_t xr = wave_prefix((int64_t)rows);
+  __syncthreads();  // the sums of an earlier scan have been read
+  if (lane == 63) s_wave[wave] = {xb, xg, xr};
   __syncthreads();
-  if (lane == 63) wave_sums[wave] = x;
-  __syncthreads();
-  int64_t base = 0, all = 0;
+  TabSums s = {xb - back, xg - grow, 0, 0, xr - rows, 0};
 #pragma unroll
   for (int w = 0; w < kTabThreads / 64; ++w) {
-    if (w < wave) base += wave_sums[w];
-    all += wave_sums[w];
+    const TabWave t = s_wave[w];
+    if (w < wave) {
+      s.back += t.back;
+      s.grow += t.grow;
+      s.rows += t.rows;
+    }
+    s.all_back += t.back;
+    s.all_grow += t.grow;
+    s.all_rows += t.rows;
   }
-  total = all;
-  return base + x - v;
+  return s;
 }
 
 // The last i in [0, n) with at[i] <= x (at[0] <= x, ascending).
-template <typename T>
-__device__ __forceinline__ int tab_find(const T* at, int n, T x) {
+__device__ __forceinline__ int tab_find(const int* at, int n, int x) {
   int lo = 0, hi = n;  // at[lo] <= x < at[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -107,93 +121,121 @@ __device__ __forceinline__ int64_t tab_slot(const TableParams& P, const int32_t*
 // SLOTS: also the slots, by the same workgroup.
 template <bool SLOTS>
 __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams P) {
-  __shared__ int64_t wave_sums[kTabThreads / 64];
-  __shared__ int s_at[kTabThreads + 1], s_own[kTabThreads], s_cu[kTabThreads + 1];
+  __shared__ TabWave s_wave[kTabThreads / 64];
+  __shared__ int s_at[kTabThreads + 1], s_col[kTabThreads], s_cu[kTabThreads + 1], s_taken;
+  __shared__ bool s_ok[kTabThreads];
   const int tid = threadIdx.x;
   const int nf = min(max(*P.n_free, 0), P.n_cap);
+  const bool one = P.B <= kTabThreads;  // all requests at once: one look at them, one scan
+  TabReq r = tab_req(P, tid);
+  TabSums s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
+  int all_back = s.all_back;
+  for (int b0 = kTabThreads; b0 < P.B; b0 += kTabThreads)
+    all_back += tab_scan(tab_req(P, b0 + tid).back(), 0, 0, s_wave).all_back;
+  if (tid == 0) s_taken = 0;
 
-  int64_t all_back = 0;
-  for (int b0 = 0; b0 < P.B; b0 += kTabThreads) {
-    const TabReq r = tab_req(P, b0 + tid);
-    int64_t t;
-    tab_scan(max(r.own - r.need, 0), wave_sums, t);
-    all_back += t;
-  }
-  // give back: the last request's last block lands lowest
-  int64_t before = 0;
+  int before = 0;
   for (int b0 = 0; all_back > 0 && b0 < P.B; b0 += kTabThreads) {
-    const TabReq r = tab_req(P, b0 + tid);
-    int64_t t;
-    const int64_t at = tab_scan(max(r.own - r.need, 0), wave_sums, t);
-    __syncthreads();
-    s_at[tid] = (int)at;
-    s_own[tid] = r.own;
-    if (tid == 0) s_at[kTabThreads] = (int)t;
-    __syncthreads();
-    for (int x = tid; x < (int)t; x += kTabThreads) {
-      const int i = tab_find(s_at, kTabThreads, x);
-      // x counts the chunk's entries in the order (request, entry from the first surplus one on)
-      int32_t* e = P.table + (int64_t)(b0 + i) * P.table_stride + s_own[i] - (s_at[i + 1] - x);
-      const int64_t to = nf + all_back - 1 - (before + x);
-      const int32_t id = *e;
-      *e = -1;
-      if (to < P.n_cap) P.free_blocks[to] = id;
+    if (!one) {
+      r = tab_req(P, b0 + tid);
+      s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
     }
-    before += t;
+    __syncthreads();
+    s_at[tid] = s.back;
+    s_col[tid] = r.need;
+    __syncthreads();
+    for (int x0 = tid; x0 < s.all_back; x0 += kTabThreads * kTabBatch) {
+      int32_t* e[kTabBatch];
+      int32_t id[kTabBatch];
+#pragma unroll
+      for (int u = 0; u < kTabBatch; ++u) {
+        const int x = x0 + u * kTabThreads;
+        const int i = tab_find(s_at, kTabThreads, x);
+        e[u] = P.table + (int64_t)(b0 + i) * P.table_stride + s_col[i] + (x - s_at[i]);
+        if (x < s.all_back) id[u] = *e[u];
+      }
+#pragma unroll
+      for (int u = 0; u < kTabBatch; ++u) {
+        const int x = x0 + u * kTabThreads;
+        if (x < s.all_back) {
+          const int64_t to = (int64_t)nf + all_back - 1 - (before + x);
+          *e[u] = -1;
+          if (to < P.n_cap) P.free_blocks[to] = id[u];
+        }
+      }
+    }
+    before += s.all_back;
   }
-  __syncthreads();
 
-  const int64_t avail = min(nf + all_back, (int64_t)P.n_cap);
-  int64_t taken_before = 0, rows_before = 0, taken = 0;
+  const int avail = (int)min((int64_t)nf + all_back, (int64_t)P.n_cap);
+  int64_t wanted_before = 0, rows_before = 0;
   for (int b0 = 0; b0 < P.B; b0 += kTabThreads) {
-    const int b = b0 + tid;
-    const TabReq r = tab_req(P, b);
-    const bool fits = r.need <= P.W;
-    const int grow = fits ? max(r.need - r.own, 0) : 0;
-    int64_t t_grow, t_rows, t_take;
-    const int64_t g = taken_before + tab_scan(grow, wave_sums, t_grow);
-    const int64_t c = rows_before + tab_scan(max(r.len - r.first, 0), wave_sums, t_rows);
-    const bool ok = fits && (grow == 0 || g + grow <= avail);
-    // served requests that grow come before the others that do, so their own sums are G_b too
-    const int64_t at = tab_scan(ok ? grow : 0, wave_sums, t_take);
+    if (!one) {
+      r = tab_req(P, b0 + tid);
+      s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
+    }
+    const int grow = r.grow(P.W);
+    const bool ok = r.need <= P.W && (grow == 0 || wanted_before + s.grow + grow <= avail);
     __syncthreads();
-    s_at[tid] = (int)at;
-    s_own[tid] = r.own;
-    if (tid == 0) s_at[kTabThreads] = (int)t_take;
-    if (b < P.B) {
-      const int32_t cu = (int32_t)min(c, (int64_t)0x7fffffff);
-      P.cu_rows[b] = cu;
+    s_at[tid] = s.grow;
+    s_col[tid] = r.own;
+    s_ok[tid] = ok;
+    if (b0 + tid < P.B) {
+      const int32_t cu = (int32_t)min(rows_before + s.rows, (int64_t)0x7fffffff);
+      P.cu_rows[b0 + tid] = cu;
       s_cu[tid] = cu;
-      P.ok[b] = ok;
-      if (ok) P.n_blocks[b] = r.need;
+      P.ok[b0 + tid] = ok;
+      if (ok && r.need != r.own) P.n_blocks[b0 + tid] = r.need;
+      if (ok && grow > 0) atomicMax(&s_taken, (int)(wanted_before + s.grow + grow));
     }
     __syncthreads();
-    for (int x = tid; x < (int)t_take; x += kTabThreads) {
-      const int i = tab_find(s_at, kTabThreads, x);
-      P.table[(int64_t)(b0 + i) * P.table_stride + s_own[i] + (x - s_at[i])] =
-          P.free_blocks[avail - 1 - (taken + x)];
+    const int most = (int)min((int64_t)s.all_grow, avail - wanted_before);
+    for (int x0 = tid; x0 < most; x0 += kTabThreads * kTabBatch) {
+      int32_t id[kTabBatch];
+#pragma unroll
+      for (int u = 0; u < kTabBatch; ++u) {
+        const int x = x0 + u * kTabThreads;
+        if (x < most) id[u] = P.free_blocks[avail - 1 - (wanted_before + x)];
+      }
+#pragma unroll
+      for (int u = 0; u < kTabBatch; ++u) {
+        const int x = x0 + u * kTabThreads;
+        const int i = tab_find(s_at, kTabThreads, x);
+        if (x < most && s_ok[i]) P.table[(int64_t)(b0 + i) * P.table_stride + s_col[i] + (x - s_at[i])] = id[u];
+      }
     }
-    taken_before += t_grow;
-    rows_before += t_rows;
-    taken += t_take;
-    __syncthreads();
+    wanted_before += s.all_grow;
+    rows_before += s.all_rows;
   }
   const int32_t n_rows = (int32_t)min(rows_before, (int64_t)0x7fffffff);
   if (tid == 0) {
     P.cu_rows[P.B] = n_rows;
-    *P.n_free = (int32_t)(avail - taken);
+    *P.n_free = avail - s_taken;
   }
   if constexpr (SLOTS) {
-    if (tid == 0 && P.B <= kTabThreads) s_cu[P.B] = n_rows;
+    if (tid == 0 && one) s_cu[P.B] = n_rows;
     __syncthreads();
-    const int32_t* cu = P.B <= kTabThreads ? s_cu : P.cu_rows;
-    for (int r = tid; r < P.max_rows; r += kTabThreads) P.slots[r] = tab_slot(P, cu, r);
+    const int32_t* cu = one ? s_cu : P.cu_rows;
+    for (int x = tid; x < P.max_rows; x += kTabThreads) P.slots[x] = tab_slot(P, cu, x);
   }
 }
 
-__global__ void __launch_bounds__(256) slots_kernel(TableParams P) {
-  const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r < P.max_rows) P.slots[r] = tab_slot(P, P.cu_rows, r);
+constexpr int kSlotThreads = 256;
+constexpr int kSlotsEach = 4;
+__global__ void __launch_bounds__(kSlotThreads) slots_kernel(TableParams P) {
+  __shared__ int s_cu[kTabThreads + 1];
+  const int32_t* cu = P.cu_rows;
+  if (P.B <= kTabThreads) {  // the search is a chain of reads: in LDS
+    for (int i = threadIdx.x; i <= P.B; i += kSlotThreads) s_cu[i] = P.cu_rows[i];
+    __syncthreads();
+    cu = s_cu;
+  }
+  const int r0 = blockIdx.x * (kSlotThreads * kSlotsEach) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < kSlotsEach; ++u) {
+    const int r = r0 + u * kSlotThreads;
+    if (r < P.max_rows) P.slots[r] = tab_slot(P, cu, r);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -212,7 +254,7 @@ template <int PB>
 struct Piece;
 template <>
 struct Piece<16> {
-  typedef uint4 type;
+  typedef __attribute__((ext_vector_type(4))) uint32_t type;
 };
 template <>
 struct Piece<4> {
@@ -233,44 +275,33 @@ struct AppendParams {
 };
 
 constexpr int kAppThreads = 256;
-constexpr int kAppUnroll = 4;  // rows a thread has in flight
 
+// One piece of one row a thread.  268 MB of rows of 2 KiB read and written:
+// 49 us (5.5 TB/s, a plain copy of as much 50); two, four and eight rows a
+// thread took 51, 56 and 139.
 template <int PB>
 __global__ void __launch_bounds__(kAppThreads) append_rows_kernel(AppendParams P) {
   typedef typename Piece<PB>::type T;
   const int per_head = P.pool.D_bytes / PB;
   const int per_row = P.pool.H_kv * per_head;
   const int cols = min(per_row, kAppThreads);
-  const int at_once = kAppThreads / cols;  // rows of one step
+  const int at_once = kAppThreads / cols;  // rows of a workgroup
   const int row_in = threadIdx.x / cols;
-  if (row_in >= at_once) return;
+  const int r = blockIdx.x * at_once + row_in;
+  if (row_in >= at_once || r >= P.N) return;
+  const int64_t slot = P.slots[r];
+  if (slot < 0 || slot >= (int64_t)P.pool.blocks * P.pool.bs.d) return;
   const int layer = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
-  const char* src = is_v ? P.v + layer * P.vsl : P.k + layer * P.ksl;
-  char* dst = (is_v ? P.pool.v : P.pool.k) + layer * P.pool.sl;
-  const int64_t sn = is_v ? P.vsn : P.ksn, sh = is_v ? P.vsh : P.ksh;
-  const int64_t n_slots = (int64_t)P.pool.blocks * P.pool.bs.d;
-  const int row0 = blockIdx.x * (at_once * kAppUnroll) + row_in;
-  int64_t to[kAppUnroll];
-#pragma unroll
-  for (int u = 0; u < kAppUnroll; ++u) {
-    const int r = row0 + u * at_once;
-    const int64_t slot = r < P.N ? P.slots[r] : -1;
-    to[u] = -1;
-    if (slot >= 0 && slot < n_slots) {
-      const int blk = div_by((int)slot, P.pool.bs);
-      to[u] = blk * P.pool.sb + (slot - (int64_t)blk * P.pool.bs.d) * P.pool.sr;
-    }
-  }
+  const char* src = is_v ? P.v + layer * P.vsl + r * P.vsn : P.k + layer * P.ksl + r * P.ksn;
+  const int64_t sh = is_v ? P.vsh : P.ksh;
+  const int blk = div_by((int)slot, P.pool.bs);
+  char* dst = (is_v ? P.pool.v : P.pool.k) + layer * P.pool.sl + blk * P.pool.sb +
+              (slot - (int64_t)blk * P.pool.bs.d) * P.pool.sr;
   for (int c = threadIdx.x - row_in * cols; c < per_row; c += cols) {
     const int h = c / per_head, x = (c - h * per_head) * PB;
-    T v[kAppUnroll];
-#pragma unroll
-    for (int u = 0; u < kAppUnroll; ++u)
-      if (to[u] >= 0) v[u] = *reinterpret_cast<const T*>(src + (int64_t)(row0 + u * at_once) * sn + h * sh + x);
-#pragma unroll
-    for (int u = 0; u < kAppUnroll; ++u)
-      if (to[u] >= 0) *reinterpret_cast<T*>(dst + to[u] + h * P.pool.sh + x) = v[u];
+    *reinterpret_cast<T*>(dst + h * P.pool.sh + x) =
+        __builtin_nontemporal_load(reinterpret_cast<const T*>(src + h * sh + x));
   }
 }
 
@@ -340,13 +371,11 @@ __global__ void __launch_bounds__(kCommitThreads) commit_path_kernel(CommitParam
   for (int j0 = 0; j0 < n; j0 += U) {
     T v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t f = __shfl(from, (j0 + u) & 63, 64);
-      if (live && j0 + u < n) v[u] = *reinterpret_cast<const T*>(col + f);
-    }
+    for (int u = 0; u < U; ++u)
+      if (live && j0 + u < n) v[u] = *reinterpret_cast<const T*>(col + lane_of(from, min(j0 + u, 63)));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t f = __shfl(from, (j0 + u) & 63, 64), t = __shfl(to, (j0 + u) & 63, 64);
+      const int64_t f = lane_of(from, min(j0 + u, 63)), t = lane_of(to, min(j0 + u, 63));
       if (live && j0 + u < n && f != t) *reinterpret_cast<T*>(col + t) = v[u];
     }
   }
@@ -482,7 +511,8 @@ extern "C" int halo_update_block_tables(int32_t* table, int64_t table_stride, in
   if (here) hipLaunchKernelGGL(update_tables_kernel<true>, dim3(1), dim3(kTabThreads), 0, st, p);
   else {
     hipLaunchKernelGGL(update_tables_kernel<false>, dim3(1), dim3(kTabThreads), 0, st, p);
-    hipLaunchKernelGGL(slots_kernel, dim3((unsigned)((max_rows + 255) / 256)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(slots_kernel, dim3((unsigned)(((int64_t)max_rows + kSlotThreads * kSlotsEach - 1) / (kSlotThreads * kSlotsEach))),
+                       dim3(kSlotThreads), 0, st, p);
   }
   HALO_CHECK_HIP(hipGetLastError());
   return HALO_OK;
@@ -511,7 +541,7 @@ extern "C" int halo_append_rows(const halo_block_pool* pool, const void* k, int6
   const int pb = piece_bytes(p.pool, reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                                          (uint64_t)(p.ksl | p.ksn | p.ksh | p.vsl | p.vsn | p.vsh));
   const int per_row = p.pool.H_kv * (p.pool.D_bytes / pb);
-  const int rows = kAppThreads / (per_row < kAppThreads ? per_row : kAppThreads) * kAppUnroll;
+  const int rows = kAppThreads / (per_row < kAppThreads ? per_row : kAppThreads);
   const dim3 grid((unsigned)((N + rows - 1) / rows), (unsigned)pool->layers, 2), block(kAppThreads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (pb == 16) hipLaunchKernelGGL(append_rows_kernel<16>, grid, block, 0, st, p);

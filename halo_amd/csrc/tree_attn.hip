@@ -81,28 +81,6 @@ struct TreeItem {
   int part;              // partial of the unit's first cut
 };
 
-// Inclusive sums over the 64 lanes, in registers.
-template <typename T, int CTRL, int ROWS>
-__device__ __forceinline__ T tree_dpp(T v) {
-  static_assert(sizeof(T) == 4, "one register");
-  return __builtin_bit_cast(
-      T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-}
-template <typename T>
-__device__ __forceinline__ T wave_prefix(T v) {
-  v += tree_dpp<T, 0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
-  v += tree_dpp<T, 0x112, 0xf>(v);
-  v += tree_dpp<T, 0x114, 0xf>(v);
-  v += tree_dpp<T, 0x118, 0xf>(v);
-  v += tree_dpp<T, 0x142, 0xa>(v);  // lane 15 of each row to the row behind it
-  v += tree_dpp<T, 0x143, 0xc>(v);  // lane 31 to the upper half
-  return v;
-}
-__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ float lane_of(float v, int lane) {
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
-}
-
 // Every lane returns the same; false past the last item.  ITEMS: x counts
 // items (head, cut, row block; the row blocks that read the same rows side by
 // side), else units (row block, head).
@@ -202,12 +180,13 @@ struct TreeRow {
   int blk, in_blk;
   __device__ __forceinline__ void load(const TreeParams& P, const TreeItem& it, int pos) {
     const int c = div_by(pos, P.bs);
-    const bool ok = (int)(pos < it.ctx + it.n) & (int)(c < P.W);
-    blk = -1;
-    if (ok) blk = P.table[it.b * P.table_stride + c];
-    in_blk = pos - c * P.bs.d;
+    // read in any case, from the last column at most: a load behind a branch would be waited for with all others
+    blk = P.table[it.b * P.table_stride + min(c, P.W - 1)];
+    in_blk = pos < it.ctx + it.n && c < P.W ? pos - c * P.bs.d : -1;
   }
-  __device__ __forceinline__ bool there(const TreeParams& P) const { return (uint32_t)blk < (uint32_t)P.blocks; }
+  __device__ __forceinline__ bool there(const TreeParams& P) const {
+    return in_blk >= 0 && (uint32_t)blk < (uint32_t)P.blocks;
+  }
   // in 16-byte pieces from the pool's first row, which stands in for rows that are not there
   __device__ __forceinline__ uint32_t place(const TreeParams& P) const {
     const uint32_t at = (uint32_t)blk * P.sb + (uint32_t)in_blk * P.sr;
@@ -352,13 +331,9 @@ constexpr int kTreeWideKT = 64;
 // (they end in order).
 template <int N>
 __device__ __forceinline__ void tree_wait() {
-  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  else {
-    static_assert(N == 16, "instructions of a tile");
-    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-  }
+  static_assert(N < 64, "6 bits");
+  // the builtin, not asm: the compiler then knows what has landed and adds no waits of its own
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
 // LDS reads of a tile in one block with their wait.  The compiler orders an
@@ -1219,12 +1194,17 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 
 // Merge of a unit's partials: with M the largest of a row's maxima, out = sum_c
 // 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.  One workgroup folds four pieces of
-// 32 rows, its waves every fourth partial each; the order is fixed.
-template <int D, int DT, int KT, int NW>
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
+// 32 rows, its MW waves every MW-th partial each, in batches of 8 whose loads
+// are in flight together; the order is fixed.  Eight waves where few units are
+// cut into many (64 partials in one round trip: 33 of 8 units 4.8 us, with four
+// waves 6.2), two where many units are cut into few (256 of 5 to 15: see
+// tree_shape).
+constexpr int kMergeBatch = 8;
+template <int D, int DT, int KT, int NW, int MW>
+__global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
   constexpr int PIECES = D / 8, PPW = 4;
-  __shared__ float4 s_o[kTreeWaves][PPW][64];
-  __shared__ float2 s_ml[kTreeWaves][32];
+  __shared__ float4 s_o[MW][PPW][64];
+  __shared__ float2 s_ml[MW][32];
   TreeItem it;
   const int rows32 = NW == 1 ? 0 : blockIdx.x % NW;  // which 32 of the unit's rows
   if (!tree_find<KT, 32 * NW, false>(P, blockIdx.x / NW, it) || it.cuts <= 1) return;
@@ -1240,24 +1220,39 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
   float4 acc[PPW];
 #pragma unroll
   for (int x = 0; x < PPW; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) {
-#pragma unroll 4
-    for (int c = wave; c < it.cuts; c += kTreeWaves) {
-      const int64_t pu = (int64_t)(it.part + c) * NW + rows32;
-      const float2 ml = P.part_ml[pu * 32 + qc];
-      float4 v[PPW];
+  for (int c0 = wave; live && c0 < it.cuts; c0 += MW * kMergeBatch) {
+    float2 ml[kMergeBatch];
+    float4 v[kMergeBatch][PPW];
 #pragma unroll
-      for (int x = 0; x < PPW; ++x) v[x] = P.part_o[pu * (PIECES * 64) + (x0 + x) * 64 + lane];
-      const float mn = fmaxf(m, ml.x);
-      const float wo = tree_weight(m, mn), wn = tree_weight(ml.x, mn);
-      m = mn;
-      l = l * wo + ml.y * wn;
+    for (int y = 0; y < kMergeBatch; ++y) {
+      ml[y].x = -INFINITY;
+      if (c0 + y * MW < it.cuts) {
+        const int64_t pu = (int64_t)(it.part + c0 + y * MW) * NW + rows32;
+        ml[y] = P.part_ml[pu * 32 + qc];
 #pragma unroll
-      for (int x = 0; x < PPW; ++x) {
-        acc[x].x = __builtin_fmaf(v[x].x, wn, acc[x].x * wo);
-        acc[x].y = __builtin_fmaf(v[x].y, wn, acc[x].y * wo);
-        acc[x].z = __builtin_fmaf(v[x].z, wn, acc[x].z * wo);
-        acc[x].w = __builtin_fmaf(v[x].w, wn, acc[x].w * wo);
+        for (int x = 0; x < PPW; ++x) v[y][x] = P.part_o[pu * (PIECES * 64) + (x0 + x) * 64 + lane];
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int y = 0; y < kMergeBatch; ++y) mn = fmaxf(mn, ml[y].x);
+    const float wo = tree_weight(m, mn);
+    m = mn;
+    l *= wo;
+#pragma unroll
+    for (int x = 0; x < PPW; ++x) acc[x] = make_float4(acc[x].x * wo, acc[x].y * wo, acc[x].z * wo, acc[x].w * wo);
+#pragma unroll
+    for (int y = 0; y < kMergeBatch; ++y) {
+      if (c0 + y * MW < it.cuts) {
+        const float w = tree_weight(ml[y].x, mn);
+        l = __builtin_fmaf(ml[y].y, w, l);
+#pragma unroll
+        for (int x = 0; x < PPW; ++x) {
+          acc[x].x = __builtin_fmaf(v[y][x].x, w, acc[x].x);
+          acc[x].y = __builtin_fmaf(v[y][x].y, w, acc[x].y);
+          acc[x].z = __builtin_fmaf(v[y][x].z, w, acc[x].z);
+          acc[x].w = __builtin_fmaf(v[y][x].w, w, acc[x].w);
+        }
       }
     }
   }
@@ -1268,24 +1263,32 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams P) {
   if (!live) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kTreeWaves; ++w) M = fmaxf(M, s_ml[w][qc].x);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = 0; w < MW; ++w) M = fmaxf(M, s_ml[w][qc].x);
+  float wt[MW];
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kTreeWaves; ++w) {
-    const float wt = tree_weight(s_ml[w][qc].x, M);
-    const float4 y = s_o[w][wave][lane];
-    l += s_ml[w][qc].y * wt;
-    a.x += y.x * wt;
-    a.y += y.y * wt;
-    a.z += y.z * wt;
-    a.w += y.w * wt;
+  for (int w = 0; w < MW; ++w) {
+    wt[w] = tree_weight(s_ml[w][qc].x, M);
+    l += s_ml[w][qc].y * wt[w];
   }
   const float inv = tree_inv(l);
-  const float v4[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
   const int node = r / P.rep, head = it.h * P.rep + (r - node * P.rep);
   const int64_t row = it.lo + node;
-  tree_store4<DT>(P, row * P.o_stride_n + head * P.o_stride_h + tree_channel<D, DT == HALO_F32>(x0 + wave, hh), v4);
+#pragma unroll
+  for (int x = wave; x < PPW; x += MW) {
+    float v4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < MW; ++w) {
+      const float4 y = s_o[w][x][lane];
+      v4[0] += y.x * wt[w];
+      v4[1] += y.y * wt[w];
+      v4[2] += y.z * wt[w];
+      v4[3] += y.w * wt[w];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v4[j] *= inv;
+    tree_store4<DT>(P, row * P.o_stride_n + head * P.o_stride_h + tree_channel<D, DT == HALO_F32>(x0 + x, hh), v4);
+  }
   if (P.lse != nullptr && blockIdx.y == 0 && wave == 0 && hh == 0) P.lse[row * P.H + head] = tree_lse(M, l);
 }
 
@@ -1299,7 +1302,7 @@ namespace {
 // kernel), units at most, workgroups that the GPU holds, launch size, partials
 // at most.
 struct TreeShape {
-  int nw, kt, slots, min_tiles;
+  int nw, kt, slots, min_tiles, mw;
   int64_t units, grid, partials;
   bool merge;
 };
@@ -1312,6 +1315,7 @@ TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows,
   // by the LDS of a workgroup (64 KiB at D = 128, 32 KiB at D = 64, the fp32 kernel's twice that) and 2 waves a SIMD
   s.slots = 256 * (s.nw == 8 || (dtype == HALO_F32 && D == 128) ? 1 : 2);
   s.min_tiles = s.nw == 1 ? kTreeWaves : 2;
+  s.mw = s.slots >= 16 * s.units ? 8 : 4;
   const int64_t longest = (max_rows + max_nodes + s.kt - 1) / s.kt;
   s.merge = longest > s.min_tiles;
   // tree_find: at most `room` items besides one a unit
@@ -1416,7 +1420,10 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
 #define HALO_TREE(KERNEL, DV, DTV, KTV, NWV)                                                                      \
   do {                                                                                                             \
     hipLaunchKernelGGL((KERNEL), grid, block, 0, st, p);                                                           \
-    if (s.merge) hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV>), mgrid, dim3(256), 0, st, p);          \
+    if (s.merge && s.mw == 8)                                                                                      \
+      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 8>), mgrid, dim3(512), 0, st, p);                   \
+    else if (s.merge)                                                                                              \
+      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 4>), mgrid, dim3(256), 0, st, p);                   \
   } while (0)
 #define HALO_TREE_WIDE(DTV, DV, NWV) HALO_TREE((tree_attn_wide_kernel<DTV, DV, NWV>), DV, DTV, kTreeWideKT, NWV)
 #define HALO_TREE16(DTV, DV)                                                                     \
