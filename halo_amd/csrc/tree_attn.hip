@@ -612,9 +612,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       pf32x16 S = pf32x16{};
 #pragma unroll
       for (int s = 0; s < KS; ++s) S = PMfma<DT>::run(__builtin_bit_cast(uint4, kk[s]), qb[s], S);
-      // past the last tile the stand-in row is read: the waits below count on NJ instructions
+      const bool more = tn < t_end;
       tile.locate(P, it, tn, lane);
-      tile.template issue<false, false>(kh, stK, lane);
+      if (more) tile.template issue<false, false>(kh, stK, lane);
       tile.look(P, it, tn + kTreeWaves, lane);
       const uint32_t mine = bits >> (4 * hh);
       if (__ballot(bits != 0xffffffffu)) {
@@ -646,7 +646,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int u = 0; u < 2; ++u)
         pb[u] = make_uint4(PMfma<DT>::pack(p[8 * u], p[8 * u + 1]), PMfma<DT>::pack(p[8 * u + 2], p[8 * u + 3]),
                            PMfma<DT>::pack(p[8 * u + 4], p[8 * u + 5]), PMfma<DT>::pack(p[8 * u + 6], p[8 * u + 7]));
-      tree_wait<NJ>();  // V: the next tile's K came after it
+      if (more) tree_wait<NJ>();  // V: the next tile's K came after it
+      else tree_wait<0>();
       if (there != 0xffffffffu) {
         tree_zero_rows<RB>(stV, there, lane);
         wave_lds_fence();
@@ -666,10 +667,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         o[i % DB] = PMfma<DT>::run(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[i / DB], o[i % DB]);
       }
       t = tn;
-      if (t >= t_end) break;
+      if (!more) break;
       tile.template issue<true, false>(vh, stV, lane);
     }
-    tree_wait<0>();  // the stand-in rows have landed: o goes over the stages
   }
   const float lt = half_sum(l_run);
   if (hh == 0) s_ml[wave][qc] = make_float2(m_run, lt);
@@ -765,8 +765,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
           for (int x = 0; x < 4; ++x)
             S = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kk[s][x]), qf[4 * (s0 + s) + x], S, 0, 0, 0);
       }
+      const bool more = tn < t_end;
       tile.locate(P, it, tn, lane);
-      tile.template issue<false, true>(kh, stK, lane);
+      if (more) tile.template issue<false, true>(kh, stK, lane);
       tile.look(P, it, tn + kTreeWaves, lane);
       const uint32_t mine = bits >> (4 * hh);
       if (__ballot(bits != 0xffffffffu)) {
@@ -793,7 +794,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         ps[e & 3] += p[e];
       }
       l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-      tree_wait<NJ>();
+      if (more) tree_wait<NJ>();
+      else tree_wait<0>();
       if (there != 0xffffffffu) {
         tree_zero_rows<RB>(stV, there, lane);
         wave_lds_fence();
@@ -863,10 +865,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] += sum[db];
       t = tn;
-      if (t >= t_end) break;
+      if (!more) break;
       tile.template issue<true, true>(vh, stV, lane);
     }
-    tree_wait<0>();
   }
   const float lt = half_sum(l_run);
   if (hh == 0) s_ml[wave][qc] = make_float2(m_run, lt);
