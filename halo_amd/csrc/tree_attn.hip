@@ -81,68 +81,105 @@ struct TreeItem {
   int part;              // partial of the unit's first cut
 };
 
-// Every lane returns the same; false past the last item.  ITEMS: x counts
-// items (head, cut, row block; the row blocks that read the same rows side by
-// side), else units (row block, head).
-template <int KT, int R, bool ITEMS>
-__device__ __forceinline__ bool tree_find(const TreeParams& P, int x, TreeItem& it) {
+// Finds item x, EACH requests a lane at once (one round trip to memory up to 64
+// EACH requests).
+template <int KT, int R, bool ITEMS, int EACH>
+__device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeItem& it) {
   const int lane = threadIdx.x & 63;
-  const TreeReq r0 = tree_req<KT, R>(P, lane);
+  TreeReq r[EACH];
+  auto look = [&](int b0) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) r[k] = tree_req<KT, R>(P, b0 + lane * EACH + k);
+  };
+  look(0);
   float total = 0.f;
   int units = 0;
-  for (int b0 = 0; b0 < P.B; b0 += 64) {
-    const TreeReq r = b0 == 0 ? r0 : tree_req<KT, R>(P, b0 + lane);
-    const int u = P.H_kv * r.rbs;
+  for (int b0 = 0;;) {
+    int u = 0;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      u += P.H_kv * r[k].rbs;
+      t += (float)(P.H_kv * r[k].rbs) * (float)r[k].tiles;
+    }
     units += lane_of(wave_prefix(u), 63);
-    total += lane_of(wave_prefix((float)u * (float)r.tiles), 63);
+    total += lane_of(wave_prefix(t), 63);
+    b0 += 64 * EACH;
+    if (b0 >= P.B) break;
+    look(b0);
   }
   // sum of ceil(tiles / L) <= total / L + units: a share that fills the GPU
   // once if the units leave room.  The sum has a relative error below 2^-16
-  // (B / 64 + 8 roundings of 2^-24), which the factor covers.
+  // (B / 64 + 12 roundings of 2^-24), which the factor covers.
   const int room = P.slots > 2 * units ? P.slots - units : P.slots / 2;
   const int L = max(P.min_tiles, (int)fminf(ceilf(total * (1.f + 0x1p-14f) / (float)room), 1e9f));
   int base = 0, part = 0;
-  for (int b0 = 0; b0 < P.B; b0 += 64) {
-    const TreeReq r = b0 == 0 ? r0 : tree_req<KT, R>(P, b0 + lane);
-    const int cuts = (int)(((uint32_t)r.tiles + (uint32_t)L - 1) / (uint32_t)L);
-    const int u = P.H_kv * r.rbs;
-    const int mine = ITEMS ? u * cuts : u;
-    const int parts = cuts > 1 ? u * cuts : 0;
-    const int at = wave_prefix(mine), parts_at = wave_prefix(parts);
+  if (P.B > 64 * EACH) look(0);
+  for (int b0 = 0;;) {
+    int cuts[EACH], mine[EACH], parts[EACH], sum = 0, psum = 0;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      cuts[k] = (int)(((uint32_t)r[k].tiles + (uint32_t)L - 1) / (uint32_t)L);
+      const int u = P.H_kv * r[k].rbs;
+      parts[k] = cuts[k] > 1 ? u * cuts[k] : 0;
+      mine[k] = ITEMS ? u * cuts[k] : cuts[k] > 1 ? u : 0;
+      sum += mine[k];
+      psum += parts[k];
+    }
+    const int at = wave_prefix(sum), parts_at = wave_prefix(psum);
     const uint64_t past = __ballot(base + at > x);
     if (past != 0) {
       const int w = __builtin_ctzll(past);
-      it.b = b0 + w;
-      it.lo = lane_of(r.lo, w);
-      it.ctx = lane_of(r.ctx, w);
-      it.n = lane_of(r.n, w);
-      it.rbs = lane_of(r.rbs, w);
-      it.tiles = lane_of(r.tiles, w);
-      it.cuts = lane_of(cuts, w);
-      uint32_t y = (uint32_t)(x - (base + lane_of(at, w) - lane_of(mine, w)));
+      int y = x - (base + lane_of(at, w) - lane_of(sum, w));  // among lane w's requests
+      part += lane_of(parts_at, w) - lane_of(psum, w);
+      bool found = false;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int m = lane_of(mine[k], w);
+        if (!found && y < m) {
+          found = true;
+          it.b = b0 + w * EACH + k;
+          it.lo = lane_of(r[k].lo, w);
+          it.ctx = lane_of(r[k].ctx, w);
+          it.n = lane_of(r[k].n, w);
+          it.rbs = lane_of(r[k].rbs, w);
+          it.tiles = lane_of(r[k].tiles, w);
+          it.cuts = lane_of(cuts[k], w);
+        }
+        if (!found) {
+          y -= m;
+          part += lane_of(parts[k], w);
+        }
+      }
       it.cut = 0;
       it.rb = 0;
-      if constexpr (ITEMS) {
-        if (it.rbs > 1) {
-          it.rb = y % (uint32_t)it.rbs;
-          y /= (uint32_t)it.rbs;
-        }
-        if (it.cuts > 1) {
-          it.cut = y % (uint32_t)it.cuts;
-          y /= (uint32_t)it.cuts;
-        }
-        it.h = y;
-      } else {
-        it.h = y % (uint32_t)P.H_kv;
-        it.rb = y / (uint32_t)P.H_kv;
+      uint32_t z = (uint32_t)y;
+      if (it.rbs > 1) {
+        it.rb = z % (uint32_t)it.rbs;
+        z /= (uint32_t)it.rbs;
       }
-      it.part = part + lane_of(parts_at, w) - lane_of(parts, w) + (it.rb * P.H_kv + it.h) * it.cuts;
+      if (ITEMS && it.cuts > 1) {
+        it.cut = z % (uint32_t)it.cuts;
+        z /= (uint32_t)it.cuts;
+      }
+      it.h = z;
+      it.part = part + (it.rb * P.H_kv + it.h) * it.cuts;
       return true;
     }
     base += lane_of(at, 63);
     part += lane_of(parts_at, 63);
+    b0 += 64 * EACH;
+    if (b0 >= P.B) return false;
+    look(b0);
   }
-  return false;
+}
+
+// Every lane returns the same; false past the last one.  ITEMS: x counts items
+// (head, cut, row block; the row blocks that read the same rows side by side),
+// else the units that were cut (head, row block).
+template <int KT, int R, bool ITEMS>
+__device__ __forceinline__ bool tree_find(const TreeParams& P, int x, TreeItem& it) {
+  return P.B <= 64 ? tree_find_of<KT, R, ITEMS, 1>(P, x, it) : tree_find_of<KT, R, ITEMS, 4>(P, x, it);
 }
 
 // Staging.  An LDS-DMA instruction fills 1 KiB, lane l its piece l, so RPI rows
@@ -1208,7 +1245,7 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
   __shared__ float2 s_ml[MW][32];
   TreeItem it;
   const int rows32 = NW == 1 ? 0 : blockIdx.x % NW;  // which 32 of the unit's rows
-  if (!tree_find<KT, 32 * NW, false>(P, blockIdx.x / NW, it) || it.cuts <= 1) return;
+  if (!tree_find<KT, 32 * NW, false>(P, blockIdx.x / NW, it)) return;
   const int row0 = (it.rb * NW + rows32) * 32;
   if (row0 >= it.n * P.rep) return;
   const int lane = threadIdx.x & 63;
@@ -1417,7 +1454,8 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   p.part_o = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * 32 * (D / 4));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)s.grid), block(64 * (s.nw == 1 ? kTreeWaves : s.nw)), mgrid((unsigned)(s.units * s.nw), D / 32);
+  const dim3 grid((unsigned)s.grid), block(64 * (s.nw == 1 ? kTreeWaves : s.nw)), 
+      mgrid((unsigned)((s.units < s.slots / 2 ? s.units : s.slots / 2) * s.nw), D / 32);  // units that can be cut
 #define HALO_TREE(KERNEL, DV, DTV, KTV, NWV)                                                                      \
   do {                                                                                                             \
     hipLaunchKernelGGL((KERNEL), grid, block, 0, st, p);                                                           \
