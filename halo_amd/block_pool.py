@@ -280,7 +280,7 @@ def commit_path(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
 
     ``path`` (B, P <= 64) int32 rises; it ends at the first entry that does not,
     or whose row the table does not hold.  Returns the new lengths (B) int32,
-    in ``out`` if given (not ``lengths`` itself)."""
+    in ``out`` if given (memory of its own, not ``lengths``)."""
     if calls is not None and stream is None:
         r = calls.commit_path(k_pool, v_pool, block_table, lengths, path, n_path, out)
         if r is not None:
@@ -297,8 +297,8 @@ def commit_path(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     check_ints(n_path, "n_path", (B,), dev)
     if out is not None:
         check_ints(out, "out", (B,), dev)
-        if overlap(out, lengths):
-            raise AssertionError("out must not share memory with lengths")
+        if any(overlap(out, t) for t in (lengths, path, n_path, block_table)):
+            raise AssertionError("out must not share memory with what is read")
     with on_stream(dev, stream):
         if out is None:
             out = torch.empty(B, device=dev, dtype=torch.int32)

@@ -97,21 +97,27 @@ __device__ __forceinline__ TabSums tab_scan(int back, int grow, int rows, TabWav
   return s;
 }
 
-// The last i in [0, n) with at[i] <= x (at[0] <= x, ascending).
-__device__ __forceinline__ int tab_find(const int* at, int n, int x) {
-  int lo = 0, hi = n;  // at[lo] <= x < at[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (at[mid] <= x) lo = mid;
-    else hi = mid;
+// For each of U values x: the last i in [0, n) with at[i] <= x (at[0] <= x,
+// ascending).  The searches go side by side: each is a chain of LDS reads.
+template <int U>
+__device__ __forceinline__ void tab_find(const int* at, int n, const int (&x)[U], int (&i)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) i[u] = 0;
+  for (int s = 1 << (31 - __clz(n)); s > 0; s >>= 1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = i[u] + s;
+      if (at[min(c, n - 1)] <= x[u] && c < n) i[u] = c;
+    }
   }
-  return lo;
 }
 
 // Slot of new row r: -1 behind the last row and for rows of requests that were not served.
 __device__ __forceinline__ int64_t tab_slot(const TableParams& P, const int32_t* cu, int r) {
   if (r >= cu[P.B]) return -1;
-  const int b = tab_find(cu, P.B, r);
+  int at[1];
+  tab_find<1>(cu, P.B, {r}, at);
+  const int b = at[0];
   if (!P.ok[b]) return -1;
   const int p = max(P.first[b], 0) + (r - cu[b]);
   const int c = div_by(p, P.bs);
@@ -136,6 +142,7 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
 
   int before = 0;
   for (int b0 = 0; all_back > 0 && b0 < P.B; b0 += kTabThreads) {
+    const int n = min(P.B - b0, kTabThreads);
     if (!one) {
       r = tab_req(P, b0 + tid);
       s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
@@ -147,12 +154,14 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
     for (int x0 = tid; x0 < s.all_back; x0 += kTabThreads * kTabBatch) {
       int32_t* e[kTabBatch];
       int32_t id[kTabBatch];
+      int xs[kTabBatch], is[kTabBatch];
+#pragma unroll
+      for (int u = 0; u < kTabBatch; ++u) xs[u] = x0 + u * kTabThreads;
+      tab_find(s_at, n, xs, is);
 #pragma unroll
       for (int u = 0; u < kTabBatch; ++u) {
-        const int x = x0 + u * kTabThreads;
-        const int i = tab_find(s_at, kTabThreads, x);
-        e[u] = P.table + (int64_t)(b0 + i) * P.table_stride + s_col[i] + (x - s_at[i]);
-        if (x < s.all_back) id[u] = *e[u];
+        e[u] = P.table + (int64_t)(b0 + is[u]) * P.table_stride + s_col[is[u]] + (xs[u] - s_at[is[u]]);
+        if (xs[u] < s.all_back) id[u] = *e[u];
       }
 #pragma unroll
       for (int u = 0; u < kTabBatch; ++u) {
@@ -170,6 +179,7 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
   const int avail = (int)min((int64_t)nf + all_back, (int64_t)P.n_cap);
   int64_t wanted_before = 0, rows_before = 0;
   for (int b0 = 0; b0 < P.B; b0 += kTabThreads) {
+    const int n = min(P.B - b0, kTabThreads);
     if (!one) {
       r = tab_req(P, b0 + tid);
       s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
@@ -185,23 +195,25 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
       P.cu_rows[b0 + tid] = cu;
       s_cu[tid] = cu;
       P.ok[b0 + tid] = ok;
-      if (ok && r.need != r.own) P.n_blocks[b0 + tid] = r.need;
+      if (ok) P.n_blocks[b0 + tid] = r.need;
       if (ok && grow > 0) atomicMax(&s_taken, (int)(wanted_before + s.grow + grow));
     }
     __syncthreads();
     const int most = (int)min((int64_t)s.all_grow, avail - wanted_before);
     for (int x0 = tid; x0 < most; x0 += kTabThreads * kTabBatch) {
       int32_t id[kTabBatch];
+      int xs[kTabBatch], is[kTabBatch];
 #pragma unroll
       for (int u = 0; u < kTabBatch; ++u) {
-        const int x = x0 + u * kTabThreads;
-        if (x < most) id[u] = P.free_blocks[avail - 1 - (wanted_before + x)];
+        xs[u] = x0 + u * kTabThreads;
+        if (xs[u] < most) id[u] = P.free_blocks[avail - 1 - (wanted_before + xs[u])];
       }
+      tab_find(s_at, n, xs, is);
 #pragma unroll
       for (int u = 0; u < kTabBatch; ++u) {
-        const int x = x0 + u * kTabThreads;
-        const int i = tab_find(s_at, kTabThreads, x);
-        if (x < most && s_ok[i]) P.table[(int64_t)(b0 + i) * P.table_stride + s_col[i] + (x - s_at[i])] = id[u];
+        const int i = is[u];
+        if (xs[u] < most && s_ok[i])
+          P.table[(int64_t)(b0 + i) * P.table_stride + s_col[i] + (xs[u] - s_at[i])] = id[u];
       }
     }
     wanted_before += s.all_grow;
@@ -221,7 +233,7 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
 }
 
 constexpr int kSlotThreads = 256;
-constexpr int kSlotsEach = 4;
+constexpr int kSlotsEach = 1;
 __global__ void __launch_bounds__(kSlotThreads) slots_kernel(TableParams P) {
   __shared__ int s_cu[kTabThreads + 1];
   const int32_t* cu = P.cu_rows;
@@ -497,7 +509,7 @@ extern "C" int halo_update_block_tables(int32_t* table, int64_t table_stride, in
                                         int32_t* free_blocks, int n_cap, int32_t* n_free, const int32_t* lengths,
                                         const int32_t* first, int block_size, int max_rows, int32_t* cu_rows,
                                         int64_t* slots, uint8_t* ok, void* stream) {
-  HALO_CHECK_ARG(table && n_blocks && free_blocks && n_free && lengths && first && cu_rows && ok,
+  HALO_CHECK_ARG(table && n_blocks && (free_blocks || n_cap == 0) && n_free && lengths && first && cu_rows && ok,
                  "null pointer argument");
   HALO_CHECK_ARG(B > 0 && W > 0 && n_cap >= 0 && block_size > 0 && max_rows >= 0 && (max_rows == 0 || slots),
                  "bad sizes");

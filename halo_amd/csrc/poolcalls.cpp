@@ -204,7 +204,8 @@ py::object tree_attention(const Tensor& q, const Tensor& k_pool, const Tensor& v
   }
   if (lse) {
     const Tensor& z = *lse;
-    if (z.dim() != 2 || z.size(0) != N || z.size(1) != H || z.scalar_type() != at::kFloat || !on(z, d) || !z.is_contiguous())
+    if (z.dim() != 2 || z.size(0) != N || z.size(1) != H || z.scalar_type() != at::kFloat || !on(z, d) ||
+        !z.is_contiguous() || !apart(z, q) || !apart(z, *out))
       return py::none();
   } else if (return_lse) {
     lse = empty({N, H}, at::kFloat, d);
@@ -235,7 +236,9 @@ py::object commit_path(const Tensor& k_pool, const Tensor& v_pool, const Tensor&
       !path.is_contiguous() || !ints(n_path, B, d))
     return py::none();
   if (out) {
-    if (!ints(*out, B, d) || !apart(*out, lengths)) return py::none();
+    if (!ints(*out, B, d)) return py::none();
+    for (const Tensor* t : {&lengths, &path, &n_path, &table})
+      if (!apart(*out, *t)) return py::none();
   } else {
     out = empty({B}, at::kInt, d);
   }

@@ -91,6 +91,8 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     if lse is not None and (lse.shape != (N, H) or lse.dtype != torch.float32 or lse.device != dev
                             or not lse.is_contiguous()):
         raise AssertionError(f"lse must be contiguous float32 {(N, H)} on {dev}")
+    if lse is not None and (overlap(lse, q) or (out is not None and overlap(lse, out))):
+        raise AssertionError("lse must not share memory with q or out")
     with on_stream(dev, stream):
         qs = q.stride()
         per = 16 // q.element_size()

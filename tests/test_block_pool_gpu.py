@@ -110,6 +110,23 @@ def test_update_there_and_back_restores_the_state(dev):
     assert back[0] == s[0] and back[1] == s[1] and back[3] == s[3]
 
 
+def test_update_without_a_free_list(dev):
+    """An empty free list: lengths that need no new block are served, the others are not."""
+    rng = random.Random(13)
+    table, owned, _, _ = _state(rng, 3, 4, [2, 1, 0], 0)
+    _check_update(dev, (table, owned, [], 0), [16, 9, 0], [14, 8, 0], 8, 4)
+
+
+def test_update_repairs_counts_past_the_table(dev):
+    import halo_amd
+    n = _i32([9, -3], dev)
+    t = _i32([[4, 5, 6], [-1, -1, -1]], dev)
+    free, n_free = _i32([7, -1, -1, -1], dev), _i32([1], dev)
+    up = halo_amd.update_block_tables(t, n, free, n_free, _i32([12, 2], dev), _i32([11, 0], dev), block_size=4, max_rows=3)
+    assert n.tolist() == [3, 1] and t.tolist() == [[4, 5, 6], [7, -1, -1]] and n_free.tolist() == [0]
+    assert up.slots.tolist() == [27, 28, 29]
+
+
 def test_update_strided_table(dev):
     import halo_amd
     base = torch.full((3, 10), -1, dtype=torch.int32, device=dev)

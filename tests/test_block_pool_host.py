@@ -74,6 +74,8 @@ CALLS = dict(update_block_tables=_tables, append_rows=_append, tree_layout=_layo
 _same = torch.zeros(3, 2, 16, 64)
 _lengths = torch.ones(2, dtype=I32)
 _q = torch.zeros(5, 4, 64)
+_out = torch.zeros(5, 4, 64)
+_path = torch.zeros(2, 1, dtype=I32)
 
 REFUSED = [
     ("update_block_tables", dict(block_table=torch.zeros(2, 4, dtype=I64))),
@@ -132,6 +134,8 @@ REFUSED = [
     ("tree_attention", dict(out=torch.zeros(5, 4, 64), out_dtype=torch.float16)),
     ("tree_attention", dict(q=_q, out=_q)),
     ("tree_attention", dict(lse=torch.zeros(4, 5))),
+    ("tree_attention", dict(q=_q, lse=_q.view(-1)[:20].view(5, 4))),
+    ("tree_attention", dict(out=_out, lse=_out.view(-1)[:20].view(5, 4))),
     ("commit_path", dict(path=torch.zeros(2, 65, dtype=I32))),
     ("commit_path", dict(path=torch.zeros(2, 0, dtype=I32))),
     ("commit_path", dict(path=torch.zeros(8, dtype=I32))),
@@ -140,6 +144,8 @@ REFUSED = [
     ("commit_path", dict(block_table=torch.zeros(1, 3, dtype=I32))),
     ("commit_path", dict(lengths=_lengths, out=_lengths)),
     ("commit_path", dict(out=torch.ones(3, dtype=I32))),
+    ("commit_path", dict(path=_path, out=_path.view(-1))),
+    ("commit_path", dict(n_path=_lengths, out=_lengths)),
     ("commit_path", dict(k_pool=_same, v_pool=_same)),
 ]
 
