@@ -44,7 +44,7 @@ struct TreeParams {
   const uint32_t* mask;  // 32-bit words, or null
   int64_t mask_stride;
   int B, H, H_kv, rep, N, max_nodes;
-  int slots, min_tiles;  // workgroups that the GPU holds; shortest item worth its merge
+  int slots, min_tiles;  // workgroups aimed at; shortest item worth its merge
   float scale2;
   void* out;
   int64_t o_stride_n, o_stride_h;
@@ -54,6 +54,10 @@ struct TreeParams {
   float2* part_ml;
 };
 
+// Narrow kernels (up to 32 rows a unit): the columns of one 32x32 product, key
+// tiles of 32, four waves with tiles of their own.  Wide: key tiles of 64.
+constexpr int kTreeRows = 32, kTreeKT = 32, kTreeWaves = 4;
+constexpr int kTreeWideKT = 64;
 // Slack (log2 units) by which a tile's max may exceed the running max before
 // the running max moves (probabilities stay below 2^8).
 constexpr float kTreeLazyMax = 8.0f;
@@ -112,7 +116,9 @@ __device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeIte
   // once if the units leave room.  The sum has a relative error below 2^-16
   // (B / 64 + 12 roundings of 2^-24), which the factor covers.
   const int room = P.slots > 2 * units ? P.slots - units : P.slots / 2;
-  const int L = max(P.min_tiles, (int)fminf(ceilf(total * (1.f + 0x1p-14f) / (float)room), 1e9f));
+  const int share = (int)fminf(ceilf(total * (1.f + 0x1p-14f) / (float)room), 1e9f);
+  constexpr int EVEN = KT == kTreeKT ? kTreeWaves : 1;  // waves that share an item's tiles: none gets one more
+  const int L = max((share + EVEN - 1) / EVEN * EVEN, P.min_tiles);
   int base = 0, part = 0;
   if (P.B > 64 * EACH) look(0);
   for (int b0 = 0;;) {
@@ -359,10 +365,6 @@ __device__ __forceinline__ float tree_weight(float m, float M) {
   return __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
 }
 
-constexpr int kTreeRows = 32;  // rows of a unit: the columns of one 32x32 product
-constexpr int kTreeKT = 32;    // rows of a key tile
-constexpr int kTreeWaves = 4;
-constexpr int kTreeWideKT = 64;
 
 // Waits until at most N of the wave's vector memory instructions are in flight
 // (they end in order).
@@ -1350,8 +1352,13 @@ TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows,
   s.nw = dtype == HALO_F32 || rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   s.kt = s.nw == 1 ? kTreeKT : kTreeWideKT;
   s.units = (int64_t)B * H_kv * ((rows + 32 * s.nw - 1) / (32 * s.nw));
-  // by the LDS of a workgroup (64 KiB at D = 128, 32 KiB at D = 64, the fp32 kernel's twice that) and 2 waves a SIMD
-  s.slots = 256 * (s.nw == 8 || (dtype == HALO_F32 && D == 128) ? 1 : 2);
+  // Two workgroups a CU fit by their LDS (64 KiB at D = 128, 32 KiB at D = 64,
+  // the fp32 kernel's twice that) and 2 waves a SIMD, one of 8 waves.  Few units
+  // are cut into one a CU: half the partials, and the same bandwidth (8 units of
+  // 32768 rows 36.8 -> 34.8 us, of 131072 105 -> 102; 128 units of 8192 would
+  // go from 105 to 121 by the coarser cuts).
+  const bool few = s.nw == 1 && s.units <= 32;
+  s.slots = 256 * (few || s.nw == 8 || (dtype == HALO_F32 && D == 128) ? 1 : 2);
   s.min_tiles = s.nw == 1 ? kTreeWaves : 2;
   s.mw = s.slots >= 16 * s.units ? 8 : 4;
   const int64_t longest = (max_rows + max_nodes + s.kt - 1) / s.kt;
