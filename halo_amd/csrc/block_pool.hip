@@ -25,10 +25,14 @@ namespace {
 // not, so G_b counts no block that stays.)  One workgroup, since the free list
 // is one stack: it is bound by the chain lengths -> sums -> ids -> slots, not by
 // bytes.  The ids of 1024 requests are spread over the threads by a search in
-// their sums, so one long request does not hold up the others.
+// their sums (of the requests that move any), four neighbouring ids a thread for
+// one search, so one long request does not hold up the others; the next ids are
+// on their way meanwhile.  16 requests with a few blocks each: 5.3 us (an empty
+// launch is about 2); the 17 000 blocks of 256 prompts: 11.0 us to hand out, 9.5
+// to take back, with a search for every id 14.4 and 12.4.
 // ---------------------------------------------------------------------------
 constexpr int kTabThreads = 1024;
-constexpr int kTabBatch = 4;  // ids a thread has in flight
+constexpr int64_t kTabNone = -(1ll << 62);  // base of a request that was not served
 
 struct TableParams {
   int32_t* table;
@@ -67,57 +71,92 @@ __device__ __forceinline__ TabReq tab_req(const TableParams& P, int b) {
 // Exclusive sums over the workgroup's threads, and the whole sums.  Blocks of
 // all requests number below 2^31, rows may not.
 struct TabSums {
-  int back, grow, all_back, all_grow;
+  int back, grow, i_back, i_grow;  // i_: how many requests before this one give back, want blocks
+  int all_back, all_grow, n_back, n_grow;
   int64_t rows, all_rows;
 };
 struct TabWave {
-  int back, grow;
+  int back, grow, n;  // n: requests that give back, and in the upper half those that want blocks
   int64_t rows;
 };
 __device__ __forceinline__ TabSums tab_scan(int back, int grow, int rows, TabWave* s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int WAVES = kTabThreads / 64;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int xb = wave_prefix(back), xg = wave_prefix(grow);
   const int64_t xr = wave_prefix((int64_t)rows);
+  const uint64_t hb = __ballot(back > 0), hg = __ballot(grow > 0), below = (1ull << lane) - 1;
   __syncthreads();  // the sums of an earlier scan have been read
-  if (lane == 63) s_wave[wave] = {xb, xg, xr};
+  if (lane == 63) s_wave[wave] = {xb, xg, (int)(__popcll(hb) | __popcll(hg) << 16), xr};
   __syncthreads();
-  TabSums s = {xb - back, xg - grow, 0, 0, xr - rows, 0};
-#pragma unroll
-  for (int w = 0; w < kTabThreads / 64; ++w) {
-    const TabWave t = s_wave[w];
-    if (w < wave) {
-      s.back += t.back;
-      s.grow += t.grow;
-      s.rows += t.rows;
-    }
-    s.all_back += t.back;
-    s.all_grow += t.grow;
-    s.all_rows += t.rows;
-  }
+  TabWave t = {0, 0, 0, 0};
+  if (lane < WAVES) t = s_wave[lane];
+  const int wb = wave_prefix(t.back), wg = wave_prefix(t.grow), wn = wave_prefix(t.n);
+  const int64_t wr = wave_prefix(t.rows);
+  TabSums s;
+  s.all_back = lane_of(wb, WAVES - 1);
+  s.all_grow = lane_of(wg, WAVES - 1);
+  s.n_back = lane_of(wn, WAVES - 1) & 0xffff;
+  s.n_grow = lane_of(wn, WAVES - 1) >> 16;
+  s.all_rows = lane_of(wr, WAVES - 1);
+  const int n_before = lane_of(wn - t.n, wave);
+  s.back = lane_of(wb - t.back, wave) + xb - back;
+  s.grow = lane_of(wg - t.grow, wave) + xg - grow;
+  s.i_back = (n_before & 0xffff) + (int)__popcll(hb & below);
+  s.i_grow = (n_before >> 16) + (int)__popcll(hg & below);
+  s.rows = lane_of(wr - t.rows, wave) + xr - rows;
   return s;
 }
 
-// For each of U values x: the last i in [0, n) with at[i] <= x (at[0] <= x,
-// ascending).  The searches go side by side: each is a chain of LDS reads.
-template <int U>
-__device__ __forceinline__ void tab_find(const int* at, int n, const int (&x)[U], int (&i)[U]) {
-#pragma unroll
-  for (int u = 0; u < U; ++u) i[u] = 0;
+// The last i in [0, n) with at[i] <= x (at[0] <= x, ascending).
+__device__ __forceinline__ int tab_find(const int* at, int n, int x) {
+  int i = 0;
   for (int s = 1 << (31 - __clz(n)); s > 0; s >>= 1) {
+    const int c = i + s;
+    if (at[min(c, n - 1)] <= x && c < n) i = c;
+  }
+  return i;
+}
+
+// Blocks x .. x + 3 of those that the listed requests move: entry i of the list
+// moves blocks at[i] .. at[i + 1] - 1, at least one, to or from table[base[i] + x],
+// or nowhere where its base is kTabNone.  e: where they stand in the table, less
+// than 0 for one that does not move; true where the four lie side by side.
+__device__ __forceinline__ bool tab_places(const int* at, const int64_t* base, int n, int all, int x,
+                                           int64_t (&e)[4]) {
+  int i = tab_find(at, n, x);
+  const bool same = x + 3 < all && (i + 1 == n || at[i + 1] > x + 3);
+  e[0] = base[i] + x;
+  if (!same) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = i[u] + s;
-      if (at[min(c, n - 1)] <= x[u] && c < n) i[u] = c;
+    for (int u = 1; u < 4; ++u) {
+      if (i + 1 < n && at[i + 1] <= x + u) ++i;
+      e[u] = x + u < all ? base[i] + x + u : -1;
     }
   }
+  return same;
 }
+
+// Four ids on the stack, the first on top, `left` of them there.
+struct TabIds {
+  int32_t id[4];
+  __device__ __forceinline__ void load(const int32_t* top, int left) {
+    if (left >= 4) {
+      int32_t v[4];
+      __builtin_memcpy(v, top - 3, 16);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) id[u] = v[3 - u];
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < left) id[u] = top[-u];
+    }
+  }
+};
 
 // Slot of new row r: -1 behind the last row and for rows of requests that were not served.
 __device__ __forceinline__ int64_t tab_slot(const TableParams& P, const int32_t* cu, int r) {
   if (r >= cu[P.B]) return -1;
-  int at[1];
-  tab_find<1>(cu, P.B, {r}, at);
-  const int b = at[0];
+  const int b = tab_find(cu, P.B, r);
   if (!P.ok[b]) return -1;
   const int p = max(P.first[b], 0) + (r - cu[b]);
   const int c = div_by(p, P.bs);
@@ -128,8 +167,8 @@ __device__ __forceinline__ int64_t tab_slot(const TableParams& P, const int32_t*
 template <bool SLOTS>
 __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams P) {
   __shared__ TabWave s_wave[kTabThreads / 64];
-  __shared__ int s_at[kTabThreads + 1], s_col[kTabThreads], s_cu[kTabThreads + 1], s_taken;
-  __shared__ bool s_ok[kTabThreads];
+  __shared__ int s_at[kTabThreads], s_cu[kTabThreads + 1], s_taken;
+  __shared__ int64_t s_base[kTabThreads];
   const int tid = threadIdx.x;
   const int nf = min(max(*P.n_free, 0), P.n_cap);
   const bool one = P.B <= kTabThreads;  // all requests at once: one look at them, one scan
@@ -142,35 +181,40 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
 
   int before = 0;
   for (int b0 = 0; all_back > 0 && b0 < P.B; b0 += kTabThreads) {
-    const int n = min(P.B - b0, kTabThreads);
     if (!one) {
       r = tab_req(P, b0 + tid);
       s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
     }
     __syncthreads();
-    s_at[tid] = s.back;
-    s_col[tid] = r.need;
+    if (r.back() > 0) {
+      s_at[s.i_back] = s.back;
+      s_base[s.i_back] = (int64_t)(b0 + tid) * P.table_stride + r.need - s.back;
+    }
     __syncthreads();
-    for (int x0 = tid; x0 < s.all_back; x0 += kTabThreads * kTabBatch) {
-      int32_t* e[kTabBatch];
-      int32_t id[kTabBatch];
-      int xs[kTabBatch], is[kTabBatch];
+    for (int x0 = tid * 4; x0 < s.all_back; x0 += kTabThreads * 4) {
+      int64_t e[4];
+      int32_t id[4];
+      const bool same = tab_places(s_at, s_base, s.n_back, s.all_back, x0, e);
+      const int64_t to = (int64_t)nf + all_back - 1 - (before + x0);  // of the first, the others below it
+      if (same) {
+        __builtin_memcpy(id, P.table + e[0], 16);
+        const int32_t gone[4] = {-1, -1, -1, -1};
+        __builtin_memcpy(P.table + e[0], gone, 16);
+      } else {
 #pragma unroll
-      for (int u = 0; u < kTabBatch; ++u) xs[u] = x0 + u * kTabThreads;
-      tab_find(s_at, n, xs, is);
+        for (int u = 0; u < 4; ++u)
+          if (e[u] >= 0) id[u] = P.table[e[u]];
 #pragma unroll
-      for (int u = 0; u < kTabBatch; ++u) {
-        e[u] = P.table + (int64_t)(b0 + is[u]) * P.table_stride + s_col[is[u]] + (xs[u] - s_at[is[u]]);
-        if (xs[u] < s.all_back) id[u] = *e[u];
+        for (int u = 0; u < 4; ++u)
+          if (e[u] >= 0) P.table[e[u]] = -1;
       }
+      if (same && to < P.n_cap) {
+        const int32_t v[4] = {id[3], id[2], id[1], id[0]};
+        __builtin_memcpy(P.free_blocks + to - 3, v, 16);
+      } else {
 #pragma unroll
-      for (int u = 0; u < kTabBatch; ++u) {
-        const int x = x0 + u * kTabThreads;
-        if (x < s.all_back) {
-          const int64_t to = (int64_t)nf + all_back - 1 - (before + x);
-          *e[u] = -1;
-          if (to < P.n_cap) P.free_blocks[to] = id[u];
-        }
+        for (int u = 0; u < 4; ++u)
+          if ((same || e[u] >= 0) && to - u < P.n_cap) P.free_blocks[to - u] = id[u];
       }
     }
     before += s.all_back;
@@ -179,7 +223,6 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
   const int avail = (int)min((int64_t)nf + all_back, (int64_t)P.n_cap);
   int64_t wanted_before = 0, rows_before = 0;
   for (int b0 = 0; b0 < P.B; b0 += kTabThreads) {
-    const int n = min(P.B - b0, kTabThreads);
     if (!one) {
       r = tab_req(P, b0 + tid);
       s = tab_scan(r.back(), r.grow(P.W), r.rows, s_wave);
@@ -187,9 +230,10 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
     const int grow = r.grow(P.W);
     const bool ok = r.need <= P.W && (grow == 0 || wanted_before + s.grow + grow <= avail);
     __syncthreads();
-    s_at[tid] = s.grow;
-    s_col[tid] = r.own;
-    s_ok[tid] = ok;
+    if (grow > 0) {
+      s_at[s.i_grow] = s.grow;
+      s_base[s.i_grow] = ok ? (int64_t)(b0 + tid) * P.table_stride + r.own - s.grow : kTabNone;
+    }
     if (b0 + tid < P.B) {
       const int32_t cu = (int32_t)min(rows_before + s.rows, (int64_t)0x7fffffff);
       P.cu_rows[b0 + tid] = cu;
@@ -200,21 +244,21 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
     }
     __syncthreads();
     const int most = (int)min((int64_t)s.all_grow, avail - wanted_before);
-    for (int x0 = tid; x0 < most; x0 += kTabThreads * kTabBatch) {
-      int32_t id[kTabBatch];
-      int xs[kTabBatch], is[kTabBatch];
+    TabIds ids, next;  // the next ones are on their way during the search
+    const int32_t* top = P.free_blocks + (avail - 1 - wanted_before);
+    ids.load(top - tid * 4, most - tid * 4);
+    for (int x0 = tid * 4; x0 < most; x0 += kTabThreads * 4) {
+      next.load(top - (x0 + kTabThreads * 4), most - (x0 + kTabThreads * 4));
+      int64_t e[4];
+      const bool same = tab_places(s_at, s_base, s.n_grow, most, x0, e);
+      if (same && e[0] >= 0) {
+        __builtin_memcpy(P.table + e[0], ids.id, 16);
+      } else if (!same) {
 #pragma unroll
-      for (int u = 0; u < kTabBatch; ++u) {
-        xs[u] = x0 + u * kTabThreads;
-        if (xs[u] < most) id[u] = P.free_blocks[avail - 1 - (wanted_before + xs[u])];
+        for (int u = 0; u < 4; ++u)
+          if (e[u] >= 0) P.table[e[u]] = ids.id[u];
       }
-      tab_find(s_at, n, xs, is);
-#pragma unroll
-      for (int u = 0; u < kTabBatch; ++u) {
-        const int i = is[u];
-        if (xs[u] < most && s_ok[i])
-          P.table[(int64_t)(b0 + i) * P.table_stride + s_col[i] + (xs[u] - s_at[i])] = id[u];
-      }
+      ids = next;
     }
     wanted_before += s.all_grow;
     rows_before += s.all_rows;
@@ -227,26 +271,24 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
   if constexpr (SLOTS) {
     if (tid == 0 && one) s_cu[P.B] = n_rows;
     __syncthreads();
-    const int32_t* cu = one ? s_cu : P.cu_rows;
-    for (int x = tid; x < P.max_rows; x += kTabThreads) P.slots[x] = tab_slot(P, cu, x);
+    for (int x = tid; x < P.max_rows; x += kTabThreads)
+      P.slots[x] = one ? tab_slot(P, s_cu, x) : tab_slot(P, P.cu_rows, x);
   }
 }
 
+// Slots of long batches, one a thread over the whole GPU: each is a search in
+// the sums and one read of the table (a quarter of a million in 3.9 us, 0.5 TB/s
+// of slots written: launch and latency).
 constexpr int kSlotThreads = 256;
-constexpr int kSlotsEach = 1;
 __global__ void __launch_bounds__(kSlotThreads) slots_kernel(TableParams P) {
   __shared__ int s_cu[kTabThreads + 1];
-  const int32_t* cu = P.cu_rows;
+  const int r = blockIdx.x * kSlotThreads + threadIdx.x;
   if (P.B <= kTabThreads) {  // the search is a chain of reads: in LDS
     for (int i = threadIdx.x; i <= P.B; i += kSlotThreads) s_cu[i] = P.cu_rows[i];
     __syncthreads();
-    cu = s_cu;
-  }
-  const int r0 = blockIdx.x * (kSlotThreads * kSlotsEach) + threadIdx.x;
-#pragma unroll
-  for (int u = 0; u < kSlotsEach; ++u) {
-    const int r = r0 + u * kSlotThreads;
-    if (r < P.max_rows) P.slots[r] = tab_slot(P, cu, r);
+    if (r < P.max_rows) P.slots[r] = tab_slot(P, s_cu, r);
+  } else if (r < P.max_rows) {
+    P.slots[r] = tab_slot(P, P.cu_rows, r);
   }
 }
 
@@ -288,9 +330,10 @@ struct AppendParams {
 
 constexpr int kAppThreads = 256;
 
-// One piece of one row a thread.  268 MB of rows of 2 KiB read and written:
-// 49 us (5.5 TB/s, a plain copy of as much 50); two, four and eight rows a
-// thread took 51, 56 and 139.
+// One piece of one row a thread.  32768 rows of 2 KiB, K and V (268 MB read and
+// written): 49 to 54 us by the card (5.0 to 5.5 TB/s; a plain copy of as much
+// 50 to 52).  Two, four and eight rows a thread took 51, 56 and 139 where one
+// took 49.  203 rows: 2.6 us, the launch.
 template <int PB>
 __global__ void __launch_bounds__(kAppThreads) append_rows_kernel(AppendParams P) {
   typedef typename Piece<PB>::type T;
@@ -347,7 +390,10 @@ __device__ __forceinline__ int64_t row_offset(const PoolView& pool, const int32_
 // path rises, so path[j] >= j and a row is written only after every move that
 // reads it: a thread takes one column of all rows in order and needs no other.
 // Lane j of each wave finds move j; the path ends at the first entry that does
-// not rise or whose rows the table does not hold.
+// not rise or whose rows the table does not hold.  Eight rows are in flight a
+// thread.  One request, 32 layers of 2 KiB rows, 5 accepted nodes: 4.0 us, the
+// chain path -> table -> rows; 32 requests, 28 layers of 1 KiB rows, up to 8
+// nodes: 7.8 us (2.8 TB/s of rows of 256 bytes).
 template <int PB>
 __global__ void __launch_bounds__(kCommitThreads) commit_path_kernel(CommitParams P) {
   typedef typename Piece<PB>::type T;
@@ -396,7 +442,8 @@ __global__ void __launch_bounds__(kCommitThreads) commit_path_kernel(CommitParam
 // ---------------------------------------------------------------------------
 // Ancestor masks.  With M_i the set of node i and its ancestors at most s - 1
 // steps up and a_i the ancestor s steps up, M_i | M_{a_i} reaches 2 s - 1
-// steps: log2(depth) rounds, one workgroup per tree, the sets in LDS.
+// steps: log2(depth) rounds, one workgroup per tree, the sets in LDS.  Bound by
+// the launch and two reads: 4 trees of 16 nodes 2.8 us, 256 of 200 4.6.
 // ---------------------------------------------------------------------------
 constexpr int kMaxNodes = 512;
 constexpr int kTreeThreads = 256;
@@ -513,7 +560,9 @@ extern "C" int halo_update_block_tables(int32_t* table, int64_t table_stride, in
                  "null pointer argument");
   HALO_CHECK_ARG(B > 0 && W > 0 && n_cap >= 0 && block_size > 0 && max_rows >= 0 && (max_rows == 0 || slots),
                  "bad sizes");
-  HALO_CHECK_ARG(table_stride >= W && (int64_t)B * W < (1ll << 31) && (int64_t)W * block_size < (1ll << 31),
+  // counts of blocks, and a step of the loops over them past the last, in 31 bits
+  HALO_CHECK_ARG(table_stride >= W && (int64_t)B * W < (1ll << 31) - kTabThreads * 4 &&
+                     (int64_t)W * block_size < (1ll << 31),
                  "table too large, or its rows overlap");
   TableParams p = {table, table_stride, n_blocks, B, W, free_blocks, n_cap, n_free, lengths, first,
                    make_div(block_size), max_rows, cu_rows, slots, ok};
@@ -523,7 +572,7 @@ extern "C" int halo_update_block_tables(int32_t* table, int64_t table_stride, in
   if (here) hipLaunchKernelGGL(update_tables_kernel<true>, dim3(1), dim3(kTabThreads), 0, st, p);
   else {
     hipLaunchKernelGGL(update_tables_kernel<false>, dim3(1), dim3(kTabThreads), 0, st, p);
-    hipLaunchKernelGGL(slots_kernel, dim3((unsigned)(((int64_t)max_rows + kSlotThreads * kSlotsEach - 1) / (kSlotThreads * kSlotsEach))),
+    hipLaunchKernelGGL(slots_kernel, dim3((unsigned)(((int64_t)max_rows + kSlotThreads - 1) / kSlotThreads)),
                        dim3(kSlotThreads), 0, st, p);
   }
   HALO_CHECK_HIP(hipGetLastError());

@@ -568,7 +568,12 @@ __device__ __forceinline__ void tree_zero_rows(char* sv, uint32_t there, int lan
 // pool's type, at most half a step of it) without a cross-lane move.  Each wave
 // streams tiles of its own, every fourth of the item's, through one LDS stage
 // of its own: the next K tile is asked for once the scores are there, the next
-// V tile once the product is; no barrier in the loop.
+// V tile once the product is; no barrier in the loop.  One stage leaves room for
+// two workgroups a CU, whose loads overlap each other's products.  Long
+// requests run at the memory's rate (16 of 8192 rows, 8 KV heads: 105 us,
+// 5.1 TB/s; one of 131072: 102); 8 nodes over 4096 rows take 11.2 us where
+// their bytes need 3.3: one chain of launch, item search, table look, K, V and the
+// fold of the four waves.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_kernel(TreeParams P) {
   constexpr int KS = D / 16, DB = D / 32, RB = D * 2;
@@ -722,7 +727,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 // fp32 queries and pools: the same walk on v_mfma_f32_32x32x2 (fp32 products
 // and sums).  Step s of the score product multiplies channel s (lane half 0)
-// and D/2 + s (half 1).
+// and D/2 + s (half 1).  3 requests of up to 1500 rows: 9.8 us, the same chain of
+// search, loads and fold as in the 16-bit kernel, with eight times its MFMA steps.
 template <int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_f32_kernel(TreeParams P) {
   constexpr int DB = D / 32, RB = D * 4;
@@ -935,6 +941,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // between the output products of tile t: the matrix core and the VALU overlap
 // within a wave.  Lane l of each wave looks up key l of a tile, so one vote gives the
 // rows that are there, and hands the places to the lanes that stage them.
+// 64 nodes of 4 heads (256 rows a unit) over 32768 rows, 8 KV heads: 50 to 57 us by
+// the card, 34.4 GFLOP at 600 to 690 TFLOP/s with the matrix cores busy 39 % of
+// the cycles: the exponentials, one instruction stream for both, bound it.
+// 16 requests of 1024 to 32768 rows, 84 rows a unit: 52 to 58 us, 4.0 to 4.5 TB/s.
+// Four stages of K and V took 57.7 where two took 55.7; finding a tile's places
+// in the step that stages it cost 5 us of 52.
 template <int DT, int D, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_wide_kernel(TreeParams P) {
   constexpr int KT = kTreeWideKT, R = 32 * NW;
@@ -1235,10 +1247,9 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 // Merge of a unit's partials: with M the largest of a row's maxima, out = sum_c
 // 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.  One workgroup folds four pieces of
 // 32 rows, its MW waves every MW-th partial each, in batches of 8 whose loads
-// are in flight together; the order is fixed.  Eight waves where few units are
-// cut into many (64 partials in one round trip: 33 of 8 units 4.8 us, with four
-// waves 6.2), two where many units are cut into few (256 of 5 to 15: see
-// tree_shape).
+// are in flight together; the order is fixed.  Bound by the launch and one or
+// two round trips: 8 units of 32 partials 4.0 us; 32 partials of 256 rows of 8
+// heads (34 MB) 8.8.  For MW see tree_shape.
 constexpr int kMergeBatch = 8;
 template <int D, int DT, int KT, int NW, int MW>
 __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
@@ -1349,6 +1360,9 @@ struct TreeShape {
 TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows, int max_nodes) {
   TreeShape s;
   const int64_t rows = (int64_t)max_nodes * (H / H_kv);
+  // As few waves as hold the rows.  48 rows, one request of 32768: two waves
+  // 40.8 us, four 39.8, two blocks of the narrow kernel 48.4; 64 rows, 16 of
+  // 8192: 120, 117 and 155; 48 rows, 64 of 1024: 65.6, 74.6 and 83.6.
   s.nw = dtype == HALO_F32 || rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   s.kt = s.nw == 1 ? kTreeKT : kTreeWideKT;
   s.units = (int64_t)B * H_kv * ((rows + 32 * s.nw - 1) / (32 * s.nw));
@@ -1359,7 +1373,13 @@ TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows,
   // go from 105 to 121 by the coarser cuts).
   const bool few = s.nw == 1 && s.units <= 32;
   s.slots = 256 * (few || s.nw == 8 || (dtype == HALO_F32 && D == 128) ? 1 : 2);
+  // No item shorter than this many tiles: one a wave, or two for the pipeline.
+  // With 4, 8 and 16 in the narrow kernel 1000 rows took 12.5, 13.3 and 15.0
+  // us, in fp32 3 requests of 900 12.8, 15.0 and 20.2.
   s.min_tiles = s.nw == 1 ? kTreeWaves : 2;
+  // 8 waves of the merge have 64 partials in one round trip (33 partials of 8
+  // units: 4.7 us, with four waves 6.2); many units of few partials need the
+  // workgroups side by side (64 units of 4 blocks: four waves 8.5, eight 13).
   s.mw = s.slots >= 16 * s.units ? 8 : 4;
   const int64_t longest = (max_rows + max_nodes + s.kt - 1) / s.kt;
   s.merge = longest > s.min_tiles;
@@ -1461,7 +1481,7 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   p.part_o = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * 32 * (D / 4));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)s.grid), block(64 * (s.nw == 1 ? kTreeWaves : s.nw)), 
+  const dim3 grid((unsigned)s.grid), block(64 * (s.nw == 1 ? kTreeWaves : s.nw)),
       mgrid((unsigned)((s.units < s.slots / 2 ? s.units : s.slots / 2) * s.nw), D / 32);  // units that can be cut
 #define HALO_TREE(KERNEL, DV, DTV, KTV, NWV)                                                                      \
   do {                                                                                                             \

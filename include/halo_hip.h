@@ -537,6 +537,7 @@ typedef struct halo_block_pool {
  * table (B, W) rows table_stride apart, n_blocks (B), free_blocks[0 .. *n_free)
  * the stack of free blocks in a buffer of n_cap entries (ids pushed past it
  * are dropped), all changed in place; lengths and first below 0 count as 0.
+ * B * W must be below 2^31 - 4096 and W * block_size below 2^31.
  * cu_rows (B+1), slots (max_rows), ok (B) are written whole.  One launch, or
  * two where there are many slots.
  */

@@ -63,6 +63,18 @@ def test_update_of_long_rows_takes_the_wide_slot_launch(dev):
     _check_update(dev, _state(rng, 3, 700, [5, 0, 300], 1200), [11000, 9000, 20], [80, 0, 0], 16, 20000)
 
 
+@pytest.mark.parametrize("B,W,part", [(90, 200, 0.7), (700, 40, 0.4), (1100, 30, 1.0)])
+def test_update_of_thousands_of_blocks(dev, B, W, part):
+    """More blocks than one step of the kernel moves, given back past the end of the free list and taken
+    until the list is empty."""
+    rng = random.Random(B)
+    owned = [rng.choice([0, 1, W, rng.randint(0, W)]) for _ in range(B)]
+    table, owned, free, n_free = _state(rng, B, W, owned, int(part * sum(owned) / 4))
+    lengths = [4 * rng.choice([0, 1, 2, W, rng.randint(0, W)]) for _ in range(B)]
+    _check_update(dev, (table, owned, free[:n_free + int(part * sum(owned) / 3)], n_free), lengths,
+                  [max(x - 3, 0) for x in lengths], 4, 4 * B)
+
+
 @pytest.mark.parametrize("spare", [0, 1, 2, 5, 6, 40])
 def test_update_serves_in_order_while_blocks_last(dev, spare):
     rng = random.Random(spare)
