@@ -279,7 +279,8 @@ def commit_path(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     ``lengths[b] + path[b, j]`` held, for ``j < n_path[b]``.
 
     ``path`` (B, P <= 64) int32 rises; it ends at the first entry that does not,
-    or whose row the table does not hold.  Returns the new lengths (B) int32,
+    or whose row the table does not hold.  Rows behind the committed ones lie in
+    blocks that no other request has (committed blocks may be shared).  Returns the new lengths (B) int32,
     in ``out`` if given (memory of its own, not ``lengths``)."""
     if calls is not None and stream is None:
         r = calls.commit_path(k_pool, v_pool, block_table, lengths, path, n_path, out)

@@ -197,7 +197,7 @@ py::object tree_attention(const Tensor& q, const Tensor& k_pool, const Tensor& v
     const Tensor& o = *out;
     if (o.sizes() != q.sizes() || !on(o, d) || o.scalar_type() != q.scalar_type() || o.stride(2) != 1 || o.stride(0) % 4 ||
         o.stride(1) % 4 || reinterpret_cast<uintptr_t>(o.data_ptr()) % (4 * o.element_size()) || !apart(o, q) ||
-        !apart(o, k_pool) || !apart(o, v_pool))
+        !apart(o, k_pool) || !apart(o, v_pool) || (N > 1 && o.stride(0) == 0) || (H > 1 && o.stride(1) == 0))
       return py::none();
   } else {
     out = empty({N, H, D}, q.scalar_type(), d);
@@ -205,7 +205,7 @@ py::object tree_attention(const Tensor& q, const Tensor& k_pool, const Tensor& v
   if (lse) {
     const Tensor& z = *lse;
     if (z.dim() != 2 || z.size(0) != N || z.size(1) != H || z.scalar_type() != at::kFloat || !on(z, d) ||
-        !z.is_contiguous() || !apart(z, q) || !apart(z, *out))
+        !z.is_contiguous() || !apart(z, q) || !apart(z, k_pool) || !apart(z, v_pool) || !apart(z, *out))
       return py::none();
   } else if (return_lse) {
     lse = empty({N, H}, at::kFloat, d);

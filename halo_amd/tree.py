@@ -45,7 +45,7 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     Returns out (N, H, D) in ``out_dtype`` (default q.dtype), and with
     ``return_lse`` lse (N, H) fp32, both in ``out`` and ``lse`` if given; rows of
     no request are not written.  The softmax and all sums are fp32; for 16-bit
-    pools its weights are rounded once to the pool's type."""
+    pools its weights are rounded once to the pool's type.  No gradient is kept."""
     if pool_calls.calls is not None and stream is None and out_dtype is None:
         r = pool_calls.calls.tree_attention(q, k_pool, v_pool, block_table, lengths, cu_nodes, max_nodes, mask, scale,
                                             out, lse, return_lse)
@@ -84,15 +84,16 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     if not 0 < scale < math.inf:
         raise AssertionError(f"scale must be positive and finite, got {scale}")
     if out is not None and (out.shape != q.shape or out.device != dev or out.stride(-1) != 1
-                            or out.dtype != (out_dtype or out.dtype)):
-        raise AssertionError(f"out must be {tuple(q.shape)} on {dev} with unit last stride")
+                            or out.dtype != (out_dtype or out.dtype)
+                            or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
+        raise AssertionError(f"out must be {tuple(q.shape)} on {dev} with unit last stride, not expanded")
     if out is not None and (overlap(out, q) or overlap(out, k_pool) or overlap(out, v_pool)):
         raise AssertionError("out must not share memory with q or the pools")
     if lse is not None and (lse.shape != (N, H) or lse.dtype != torch.float32 or lse.device != dev
                             or not lse.is_contiguous()):
         raise AssertionError(f"lse must be contiguous float32 {(N, H)} on {dev}")
-    if lse is not None and (overlap(lse, q) or (out is not None and overlap(lse, out))):
-        raise AssertionError("lse must not share memory with q or out")
+    if lse is not None and any(overlap(lse, t) for t in (q, k_pool, v_pool, out) if t is not None):
+        raise AssertionError("lse must not share memory with q, the pools or out")
     with on_stream(dev, stream):
         qs = q.stride()
         per = 16 // q.element_size()

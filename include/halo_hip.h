@@ -599,7 +599,8 @@ int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_
  * held, for the j < n_path[b] (<= n_path_max <= 64) in front of the first entry
  * that is not above the one before it or whose rows the table does not hold;
  * new_lengths[b] = lengths[b] + their number (lengths below 0 count as 0).
- * Nothing else of the pool changes.  new_lengths must not be lengths.
+ * Nothing else of the pool changes.  Rows from lengths[b] on lie in blocks of
+ * one request only.  new_lengths must not be lengths.
  */
 int halo_commit_path(const halo_block_pool* pool, const int32_t* table, int64_t table_stride, int B, int W,
                      const int32_t* lengths, const int32_t* path, int64_t path_stride, int n_path_max,

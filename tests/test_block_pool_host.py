@@ -133,7 +133,11 @@ REFUSED = [
     ("tree_attention", dict(out=torch.zeros(5, 4, 32))),
     ("tree_attention", dict(out=torch.zeros(5, 4, 64), out_dtype=torch.float16)),
     ("tree_attention", dict(q=_q, out=_q)),
+    ("tree_attention", dict(out=torch.zeros(1, 4, 64).expand(5, 4, 64))),
+    ("tree_attention", dict(out=torch.zeros(5, 1, 64).expand(5, 4, 64))),
     ("tree_attention", dict(lse=torch.zeros(4, 5))),
+    ("tree_attention", dict(k_pool=_same, v_pool=torch.zeros(3, 2, 16, 64), lse=_same.view(-1)[:20].view(5, 4))),
+    ("tree_attention", dict(k_pool=torch.zeros(3, 2, 16, 64), v_pool=_same, lse=_same.view(-1)[:20].view(5, 4))),
     ("tree_attention", dict(q=_q, lse=_q.view(-1)[:20].view(5, 4))),
     ("tree_attention", dict(out=_out, lse=_out.view(-1)[:20].view(5, 4))),
     ("commit_path", dict(path=torch.zeros(2, 65, dtype=I32))),
