@@ -307,8 +307,9 @@ class TieredStorage:
 
     def pool(self, tier="gpu", layer: Optional[int] = None):
         """K and V of a memory tier as a block pool, (L, max_blocks, H_kv,
-        block_size, D) or one layer's (max_blocks, H_kv, block_size, D): what
-        ``halo_amd.append_rows``, ``tree_attention`` and ``commit_path`` take."""
+        block_size, D) or one layer's (max_blocks, H_kv, block_size, D): of the
+        GPU tier, what ``halo_amd.append_rows``, ``tree_attention`` and
+        ``commit_path`` take (they refuse host memory)."""
         t = MemoryTier.from_name(tier)
         if t is MemoryTier.NVME:
             raise ValueError("the NVMe tier is a file, not a pool")
