@@ -113,8 +113,12 @@ __device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeIte
     look(b0);
   }
   // sum of ceil(tiles / L) <= total / L + units: a share that fills the GPU
-  // once if the units leave room.  The sum has a relative error below 2^-16
-  // (B / 64 + 12 roundings of 2^-24), which the factor covers.
+  // once if the units leave room.  Items, cut units and partials stay within
+  // the launch and the workspace whatever the batch: a rounded sum of terms
+  // that are not negative is never below the rounded sum of some of them alone,
+  // and of the (at most 2 P.slots, were there more) cut units each goes through
+  // 16 roundings in its wave and one for each wave with another of them, so
+  // total >= (the cut units' tiles) (1 - 1040 2^-24), which the factor covers.
   const int room = P.slots > 2 * units ? P.slots - units : P.slots / 2;
   const int share = (int)fminf(ceilf(total * (1.f + 0x1p-14f) / (float)room), 1e9f);
   constexpr int EVEN = KT == kTreeKT ? kTreeWaves : 1;  // waves that share an item's tiles: none gets one more
