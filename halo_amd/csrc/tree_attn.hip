@@ -61,6 +61,21 @@ constexpr int kTreeWideKT = 64;
 // Slack (log2 units) by which a tile's max may exceed the running max before
 // the running max moves (probabilities stay below 2^8).
 constexpr float kTreeLazyMax = 8.0f;
+// The running max of the 16-bit kernels is held kTreeLift (log2 units) below the
+// one found, which lifts all weights and sums alike and leaves their quotients.
+// fp16 has no exponents below 2^-14: as they are, weights of 2^-25 of the
+// largest and less would vanish from the products while l still counts them (a
+// first row of large score and 9000 rows of 2^-25.6 behind it gave 0 for
+// 1.8e-4).  Lifted by 2^7 they are off by 2^-32 of the largest at most, and stay
+// below 2^15 for exponents up to 2^30: the tile's max is taken a step up there,
+// since an exponent's exact product may lie half a step above its rounded one,
+// and the step is 32 at 2^28.  bf16 has fp32's exponents.
+template <int DT>
+__device__ __forceinline__ float tree_new_max(float m_old, float bm) {
+  constexpr float kLift = DT == HALO_F16 ? 7.0f : 0.0f;
+  if constexpr (DT == HALO_F16) bm = __builtin_fmaf(fabsf(bm), 0x1.01p-24f, bm);  // of -inf NaN, which is not above
+  return bm - m_old > kTreeLazyMax + kLift ? bm - kLift : m_old;
+}
 
 struct TreeReq {
   int lo, ctx, n, rbs, tiles;
@@ -569,7 +584,8 @@ __device__ __forceinline__ void tree_zero_rows(char* sv, uint32_t there, int lan
 //   output  O^T[d][row]  += sum_key V^T[d][key] P^T[key][row]  (A = V^T, B = P^T)
 // S^T's accumulator gives lane (row, half h) the keys 8i + 4h + j, which are the
 // keys of its P^T operands, so p goes to the second product (rounded to the
-// pool's type, at most half a step of it) without a cross-lane move.  Each wave
+// pool's type: half a step of it at most, fp16's below 2^-21 of the largest
+// off by 2^-32 of that) without a cross-lane move.  Each wave
 // streams tiles of its own, every fourth of the item's, through one LDS stage
 // of its own: the next K tile is asked for once the scores are there, the next
 // V tile once the product is; no barrier in the loop.  One stage leaves room for
@@ -674,7 +690,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int e = 0; e < 16; ++e) bm = fmaxf(bm, S[e]);
       bm = half_max(bm) * P.scale2;  // scale > 0
       const float m_old = m_run;
-      m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
+      m_run = tree_new_max<DT>(m_old, bm);
       const float ms = m_run == -INFINITY ? 0.f : m_run;
       if (__ballot(m_run != m_old)) {
         const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
@@ -1076,7 +1092,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
   auto take_max = [&](float bm) {  // the running max takes a tile's max into account, o and l follow
     bm = half_max(bm) * P.scale2;  // scale > 0
     const float m_old = m_run;
-    m_run = bm > m_old + kTreeLazyMax ? bm : m_old;
+    m_run = tree_new_max<DT>(m_old, bm);
     ms = m_run == -INFINITY ? 0.f : m_run;
     if (__ballot(m_run != m_old)) {
       const float alpha = m_run != m_old ? __builtin_amdgcn_exp2f(m_old - m_run) : 1.f;
