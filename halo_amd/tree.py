@@ -21,7 +21,7 @@ import torch
 
 from . import _native as nat
 from . import block_pool as pool_calls
-from .block_pool import MAX_NODES, check_ints, check_table, on_stream, overlap, pack_pool
+from .block_pool import _DTYPES, MAX_NODES, check_ints, check_table, on_stream, overlap, pack_pool
 
 
 def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -42,11 +42,12 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     attends nothing has out 0 and lse -inf, and what a node does not attend has
     no part in its output, NaN and infinities included.
 
-    Returns out (N, H, D) in ``out_dtype`` (default q.dtype), and with
-    ``return_lse`` lse (N, H) fp32, both in ``out`` and ``lse`` if given; rows of
-    no request are not written.  The softmax and all sums are fp32; for 16-bit
-    pools its weights are rounded once to the pool's type (fp16 weights below
-    2^-21 of the largest are off by at most 2^-32 of it).  No gradient is kept."""
+    Returns out (N, H, D) in ``out_dtype`` (bf16, fp16 or fp32; default
+    q.dtype), and with ``return_lse`` lse (N, H) fp32, both in ``out`` and ``lse``
+    if given; rows of no request keep what they hold there.  The softmax and all
+    sums are fp32; for 16-bit pools its weights are rounded once to the pool's
+    type (fp16 weights below 2^-21 of the largest are off by at most 2^-32 of
+    it).  No gradient is kept."""
     if pool_calls.calls is not None and stream is None and out_dtype is None:
         r = pool_calls.calls.tree_attention(q, k_pool, v_pool, block_table, lengths, cu_nodes, max_nodes, mask, scale,
                                             out, lse, return_lse)
@@ -84,6 +85,11 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0 < scale < math.inf:
         raise AssertionError(f"scale must be positive and finite, got {scale}")
+    if out_dtype is not None and out_dtype not in _DTYPES:
+        raise AssertionError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
+    if out is not None and out.dtype not in _DTYPES:
+        # its copy in fp32 could not hold the rows that are not written
+        raise AssertionError(f"out must be bf16, fp16 or fp32, got {out.dtype}")
     if out is not None and (out.shape != q.shape or out.device != dev or out.stride(-1) != 1
                             or out.dtype != (out_dtype or out.dtype)
                             or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
