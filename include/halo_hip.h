@@ -583,8 +583,9 @@ int halo_tree_layout(const int32_t* parents, const int32_t* cu_nodes, int B, int
  * scale > 0.  The pool has one layer, rows 16-byte aligned, at most 64 GiB of
  * K; D in {64, 128}; H a multiple of H_kv.  workspace: 16-byte aligned, at
  * least halo_tree_workspace_size(max_rows = W * block_size) bytes; calls that
- * may overlap need their own.  Results do not depend on the batch's order in
- * time: partials are merged in a fixed order.
+ * may overlap need their own.  Equal calls give equal bits: partials are
+ * merged in a fixed order.  Where a request's rows are cut goes by all the
+ * requests of the call, and so do its last bits.
  */
 size_t halo_tree_workspace_size(int dtype, int B, int H, int H_kv, int D, int64_t max_rows, int max_nodes);
 int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int N, int H,

@@ -1,13 +1,14 @@
-"""Tree attention's forms of output on the GPU."""
+"""Tree attention's forms of output, and requests in other company, on the GPU.
+Tolerances as in test_tree_pipeline_gpu.py."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 import tree_launch
+from test_tree_pipeline_gpu import BF16, F16, F32, check
 
 pytestmark = pytest.mark.gpu
-BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -31,3 +32,20 @@ def test_rows_of_no_request_keep_what_they_hold(dev, dtype, out_dtype, form):
     assert torch.equal(lse[:8], want[1])
     full = b.run(out_dtype=torch.float32)[0]
     assert torch.equal(out[:8], full.to(out_dtype)) and torch.equal(full.to(dtype), want[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_a_request_alone_and_among_others(dev, dtype):
+    """Each is right by itself; their last bits may differ, since the cuts go by all the requests of a call."""
+    b = tree_launch.Batch(dev, lengths=[3000, 17, 1200, 0, 5000], nodes=[5, 9, 2, 12, 7], H=8, Hk=2, D=128, bs=16, dtype=dtype, seed=4)
+    out, lse = b.run()
+    for i in (0, 1, 3, 4):
+        lo, hi = sum(b.nodes[:i]), sum(b.nodes[:i + 1])
+        one = tree_launch.Batch.__new__(tree_launch.Batch)
+        one.__dict__.update(b.__dict__, lengths=[b.lengths[i]], nodes=[b.nodes[i]], max_nodes=b.nodes[i])
+        a = b.args
+        one.args = dict(a, q=a["q"][lo:hi], mask=a["mask"][lo:hi], block_table=a["block_table"][i:i + 1], lengths=a["lengths"][i:i + 1],
+                        cu_nodes=a["cu_nodes"].new_tensor([0, hi - lo]))
+        exact = one.exact()
+        check(one, *one.run(), exact)
+        check(one, out, lse, exact, rows=slice(lo, hi))
