@@ -309,7 +309,13 @@ class TieredStorage:
         """K and V of a memory tier as a block pool, (L, max_blocks, H_kv,
         block_size, D) or one layer's (max_blocks, H_kv, block_size, D): of the
         GPU tier, what ``halo_amd.append_rows``, ``tree_attention`` and
-        ``commit_path`` take (they refuse host memory)."""
+        ``commit_path`` take (they refuse host memory).
+
+        The memory is handed out as it is: these calls neither read nor write
+        the directory.  A block that was moved to another tier keeps its rows
+        here and can be attended, but rows written to it through the pool are
+        lost to ``read_block`` and to the next move back; where blocks move,
+        ``write_rows`` writes them."""
         t = MemoryTier.from_name(tier)
         if t is MemoryTier.NVME:
             raise ValueError("the NVMe tier is a file, not a pool")
@@ -334,6 +340,27 @@ class TieredStorage:
         t = MemoryTier.from_name(tier)
         self._buffer(t).write(layer, block, keys, values)
         self.directory()[layer, block] = _TIER_CODE[t]
+
+    def write_rows(self, *, slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                   layer: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> None:
+        """``halo_amd.append_rows`` to the GPU tier's pool, rows (N, H_kv, D) of
+        one layer or (L, N, H_kv, D) of all, after which the directory names the
+        GPU tier for the blocks they lie in, in stream order (slots outside the
+        pool are skipped).  The other rows of such a block are those that the GPU
+        tier holds: a block whose rows were written in another tier is moved here
+        first.  Moves of the same blocks on other streams are waited for before
+        (``HALORefetcher.wait``, ``HALODemoter.wait``)."""
+        from .block_pool import append_rows, on_stream
+        append_rows(keys, values, slots, *self.pool("gpu", layer), stream=stream)
+        n = slots.numel()
+        rows = self.directory() if layer is None else self.directory()[layer][None]
+        with on_stream(rows.device, stream):
+            blocks = torch.div(slots, self.block_size, rounding_mode="floor")
+            blocks = torch.where((blocks >= 0) & (blocks < self.max_blocks), blocks, -1).to(torch.int32)
+            strm = nat.stream_ptr()
+            for r in rows:
+                nat.check(nat.lib().halo_set_tier(r.data_ptr(), blocks.data_ptr(), n, self.max_blocks, -1,
+                                                  _TIER_CODE[MemoryTier.GPU], strm), "halo_set_tier")
 
     def read_block(self, *, layer: int, block: int):
         t = MemoryTier.from_name(self.locate_block(layer=layer, block=block))
