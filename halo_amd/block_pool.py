@@ -55,7 +55,8 @@ def load_calls(path=None):
     """The prebuilt host extension (halo_amd/_lib/poolcalls_build, made by
     build()) that checks, allocates and calls in C++, bound to the library; None
     when it is missing or cannot be loaded.  Its functions return None for a call
-    that they do not take, which then runs (or is refused) here."""
+    that they do not take, which then runs (or is refused) here; an argument that
+    is no tensor or number where one belongs is a TypeError there."""
     import ctypes
     import importlib.util
     import os
