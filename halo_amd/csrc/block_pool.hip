@@ -22,14 +22,14 @@ namespace {
 //   entry j of b comes from free[n_free + R - 1 - (G_b + j - own_b)],
 //   new row r has           b = the last one with C_b <= r.
 // (Requests that are served and grow come before those that want blocks and are
-// not, so G_b counts no block that stays.)  One workgroup, since the free list
-// is one stack: it is bound by the chain lengths -> sums -> ids -> slots, not by
-// bytes.  The ids of 1024 requests are spread over the threads by a search in
-// their sums (of the requests that move any), four neighbouring ids a thread for
-// one search, so one long request does not hold up the others; the next ids are
-// on their way meanwhile.  16 requests with a few blocks each: 5.3 us (an empty
-// launch is about 2); the 17 000 blocks of 256 prompts: 11.0 us to hand out, 9.5
-// to take back, with a search for every id 14.4 and 12.4.
+// not, so G_b counts no block that stays.)  One workgroup: a call of a few blocks
+// is bound by the chain lengths -> sums -> ids -> slots, not by bytes.  The ids of
+// 1024 requests are spread over the threads by a search in their sums (of the
+// requests that move any), four neighbouring ids a thread for one search, so one
+// long request does not hold up the others; the next ids are on their way
+// meanwhile.  16 requests with a few blocks each: 5.3 us (an empty launch is about
+// 2); the 11 600 blocks of 256 prompts: 11.2 us to hand out, 9.6 to take back,
+// where the one CU's moves bound it (with a search for every id 14.4 and 12.4).
 // ---------------------------------------------------------------------------
 constexpr int kTabThreads = 1024;
 constexpr int64_t kTabNone = -(1ll << 62);  // base of a request that was not served
@@ -277,8 +277,8 @@ __global__ void __launch_bounds__(kTabThreads) update_tables_kernel(TableParams 
 }
 
 // Slots of long batches, one a thread over the whole GPU: each is a search in
-// the sums and one read of the table (a quarter of a million in 3.9 us, 0.5 TB/s
-// of slots written: launch and latency).
+// the sums and one read of the table (183 000 in 3.9 us, 0.4 TB/s of slots
+// written: launch and latency).
 constexpr int kSlotThreads = 256;
 __global__ void __launch_bounds__(kSlotThreads) slots_kernel(TableParams P) {
   __shared__ int s_cu[kTabThreads + 1];
@@ -331,7 +331,7 @@ struct AppendParams {
 constexpr int kAppThreads = 256;
 
 // One piece of one row a thread.  32768 rows of 2 KiB, K and V (268 MB read and
-// written): 49 to 54 us by the card (5.0 to 5.5 TB/s; a plain copy of as much
+// written): 51 to 56 us by the card (4.8 to 5.3 TB/s; a plain copy of as much
 // 50 to 52).  Two, four and eight rows a thread took 51, 56 and 139 where one
 // took 49.  203 rows: 2.6 us, the launch.
 template <int PB>
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kCommitThreads) commit_path_kernel(CommitParam
 // Ancestor masks.  With M_i the set of node i and its ancestors at most s - 1
 // steps up and a_i the ancestor s steps up, M_i | M_{a_i} reaches 2 s - 1
 // steps: log2(depth) rounds, one workgroup per tree, the sets in LDS.  Bound by
-// the launch and two reads: 4 trees of 16 nodes 2.8 us, 256 of 200 4.6.
+// the launch and two reads: 4 trees of 16 nodes 2.9 us, 256 of 200 4.7.
 // ---------------------------------------------------------------------------
 constexpr int kMaxNodes = 512;
 constexpr int kTreeThreads = 256;

@@ -44,7 +44,7 @@ struct TreeParams {
   const uint32_t* mask;  // 32-bit words, or null
   int64_t mask_stride;
   int B, H, H_kv, rep, N, max_nodes;
-  int slots, min_tiles;  // workgroups aimed at; shortest item worth its merge
+  int slots, min_tiles;  // workgroups aimed at; the least that an item's largest number of tiles may be
   float scale2;
   void* out;
   int64_t o_stride_n, o_stride_h;
@@ -590,10 +590,10 @@ __device__ __forceinline__ void tree_zero_rows(char* sv, uint32_t there, int lan
 // of its own: the next K tile is asked for once the scores are there, the next
 // V tile once the product is; no barrier in the loop.  One stage leaves room for
 // two workgroups a CU, whose loads overlap each other's products.  Long
-// requests run at the memory's rate (16 of 8192 rows, 8 KV heads: 105 us,
-// 5.1 TB/s; one of 131072: 102); 8 nodes over 4096 rows take 11.2 us where
-// their bytes need 3.3: one chain of launch, item search, table look, K, V and the
-// fold of the four waves.
+// requests run at the memory's rate (16 of 8192 rows, 8 KV heads: 106 us,
+// 5.0 TB/s; one of 131072: 101); 8 nodes over 4096 rows take 11 us where their
+// bytes need 3.3: one chain of launch, item search, table look, K, V, the second
+// tile's K and V behind the first's products, and the fold of the four waves.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_kernel(TreeParams P) {
   constexpr int KS = D / 16, DB = D / 32, RB = D * 2;
@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 // fp32 queries and pools: the same walk on v_mfma_f32_32x32x2 (fp32 products
 // and sums).  Step s of the score product multiplies channel s (lane half 0)
-// and D/2 + s (half 1).  3 requests of up to 1500 rows: 9.8 us, the same chain of
+// and D/2 + s (half 1).  3 requests of up to 1500 rows: 10.2 us, the same chain of
 // search, loads and fold as in the 16-bit kernel, with eight times its MFMA steps.
 template <int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_f32_kernel(TreeParams P) {
@@ -961,10 +961,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // between the output products of tile t: the matrix core and the VALU overlap
 // within a wave.  Lane l of each wave looks up key l of a tile, so one vote gives the
 // rows that are there, and hands the places to the lanes that stage them.
-// 64 nodes of 4 heads (256 rows a unit) over 32768 rows, 8 KV heads: 50 to 57 us by
-// the card, 34.4 GFLOP at 600 to 690 TFLOP/s with the matrix cores busy 39 % of
-// the cycles: the exponentials, one instruction stream for both, bound it.
-// 16 requests of 1024 to 32768 rows, 84 rows a unit: 52 to 58 us, 4.0 to 4.5 TB/s.
+// 64 nodes of 4 heads (256 rows a unit) over 32768 rows, 8 KV heads: 57 us (51 to
+// 66 by the card), 34.4 GFLOP at 600 TFLOP/s.  The matrix cores are busy 39 % of
+// the cycles and the waves wait 39 % of theirs: products and exponentials are one
+// instruction stream, and each tile ends in a full wait and a barrier with one
+// workgroup a CU.  16 requests of 1024 to 32768 rows, 84 rows a unit: 55 us (52 to
+// 63), 4.3 TB/s, the waves waiting 57 % of their cycles.
 // Four stages of K and V took 57.7 where two took 55.7; finding a tile's places
 // in the step that stages it cost 5 us of 52.
 template <int DT, int D, int NW>
@@ -1268,8 +1270,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 // 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.  One workgroup folds four pieces of
 // 32 rows, its MW waves every MW-th partial each, in batches of 8 whose loads
 // are in flight together; the order is fixed.  Bound by the launch and one or
-// two round trips: 8 units of 32 partials 4.0 us; 32 partials of 256 rows of 8
-// heads (34 MB) 8.8.  For MW see tree_shape.
+// two round trips: 8 units of 17 partials 4.0 us, of 29 5.1; 31 partials of 256 rows
+// of 8 heads (33 MB) 8.9.  For MW see tree_shape.
 constexpr int kMergeBatch = 8;
 template <int D, int DT, int KT, int NW, int MW>
 __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
@@ -1381,25 +1383,29 @@ TreeShape tree_shape(int dtype, int B, int H, int H_kv, int D, int64_t max_rows,
   TreeShape s;
   const int64_t rows = (int64_t)max_nodes * (H / H_kv);
   // As few waves as hold the rows.  48 rows, one request of 32768: two waves
-  // 40.8 us, four 39.8, two blocks of the narrow kernel 48.4; 64 rows, 16 of
-  // 8192: 120, 117 and 155; 48 rows, 64 of 1024: 65.6, 74.6 and 83.6.
+  // 40.7 us, four 39.6, two blocks of the narrow kernel 49.4; 64 rows, 16 of
+  // 8192: 120, 116 and 156; 48 rows, 64 of 1024: 65.7, 67.6 and 78.7.  128 rows,
+  // 16 of 8192: four waves 124, eight 175, two blocks of two 176; 32 rows, 16 of
+  // 8192: the narrow kernel 106, two waves 118.
   s.nw = dtype == HALO_F32 || rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   s.kt = s.nw == 1 ? kTreeKT : kTreeWideKT;
   s.units = (int64_t)B * H_kv * ((rows + 32 * s.nw - 1) / (32 * s.nw));
   // Two workgroups a CU fit by their LDS (64 KiB at D = 128, 32 KiB at D = 64,
   // the fp32 kernel's twice that) and 2 waves a SIMD, one of 8 waves.  Few units
   // are cut into one a CU: half the partials, and the same bandwidth (8 units of
-  // 32768 rows 36.8 -> 34.8 us, of 131072 105 -> 102; 128 units of 8192 would
-  // go from 105 to 121 by the coarser cuts).
+  // 32768 rows 36.3 -> 34.2 us, of 131072 105 -> 101, 32 units of 8192 34.7 ->
+  // 34.0; 128 units of 8192 would go from 106 to 120 by the coarser cuts).
   const bool few = s.nw == 1 && s.units <= 32;
   s.slots = 256 * (few || s.nw == 8 || (dtype == HALO_F32 && D == 128) ? 1 : 2);
-  // No item shorter than this many tiles: one a wave, or two for the pipeline.
-  // With 4, 8 and 16 in the narrow kernel 1000 rows took 12.5, 13.3 and 15.0
-  // us, in fp32 3 requests of 900 12.8, 15.0 and 20.2.
+  // The least L: a tile a wave, or two for the pipeline.  A unit of more tiles is
+  // cut into ceil(tiles / L) even items, which may be about half as long (5 tiles
+  // become 2 and 3).  With 4, 8 and 16 in the narrow kernel 1000 rows took 12.2,
+  // 12.9 and 14.6 us, in fp32 3 requests of 900 13.4, 15.4 and 20.3.
   s.min_tiles = s.nw == 1 ? kTreeWaves : 2;
-  // 8 waves of the merge have 64 partials in one round trip (33 partials of 8
-  // units: 4.7 us, with four waves 6.2); many units of few partials need the
-  // workgroups side by side (64 units of 4 blocks: four waves 8.5, eight 13).
+  // 8 waves of the merge have 64 partials in one round trip (129 partials of one
+  // unit 8.7 us, with four waves 9.5; 52 of 4 units 5.7 and 6.0; 29 of 8 units 5.1
+  // both); many units of few partials need the workgroups side by side (128 units
+  // of 3 partials of 64 rows: four waves 7.7, eight 12.5).
   s.mw = s.slots >= 16 * s.units ? 8 : 4;
   const int64_t longest = (max_rows + max_nodes + s.kt - 1) / s.kt;
   s.merge = longest > s.min_tiles;
