@@ -351,16 +351,17 @@ class TieredStorage:
         first.  Moves of the same blocks on other streams are waited for before
         (``HALORefetcher.wait``, ``HALODemoter.wait``)."""
         from .block_pool import append_rows, on_stream
-        append_rows(keys, values, slots, *self.pool("gpu", layer), stream=stream)
-        n = slots.numel()
-        rows = self.directory() if layer is None else self.directory()[layer][None]
-        with on_stream(rows.device, stream):
+        if self._dir is None and self.on_device and torch.cuda.is_current_stream_capturing():
+            raise AssertionError("the directory must exist before a graph is captured, whose replays would clear it")
+        k_pool, v_pool = self.pool("gpu", layer)
+        append_rows(keys, values, slots, k_pool, v_pool, stream=stream)
+        with on_stream(k_pool.device, stream):
+            rows = self.directory() if layer is None else self.directory()[layer][None]
             blocks = torch.div(slots, self.block_size, rounding_mode="floor")
             blocks = torch.where((blocks >= 0) & (blocks < self.max_blocks), blocks, -1).to(torch.int32)
-            strm = nat.stream_ptr()
             for r in rows:
-                nat.check(nat.lib().halo_set_tier(r.data_ptr(), blocks.data_ptr(), n, self.max_blocks, -1,
-                                                  _TIER_CODE[MemoryTier.GPU], strm), "halo_set_tier")
+                nat.check(nat.lib().halo_set_tier(r.data_ptr(), blocks.data_ptr(), slots.numel(), self.max_blocks, -1,
+                                                  _TIER_CODE[MemoryTier.GPU], nat.stream_ptr()), "halo_set_tier")
 
     def read_block(self, *, layer: int, block: int):
         t = MemoryTier.from_name(self.locate_block(layer=layer, block=block))

@@ -113,3 +113,33 @@ def test_a_speculative_step_over_moved_blocks(dev, store):
         _fetch(store, i)
         kb, vb = store.read_block(layer=i, block=0)
         assert torch.equal(kb.transpose(0, 1), k[i, [0, 2, 3, 5]]) and torch.equal(vb.transpose(0, 1), v[i, [0, 2, 3, 5]])
+
+
+def test_a_graph_does_not_make_the_directory(dev, monkeypatch):
+    from halo_amd import TieredStorage
+    st = TieredStorage(tiers=["gpu"], num_layers=L, num_kv_heads=H, head_dim=D, block_size=BS, dtype=torch.bfloat16,
+                       device=dev, max_blocks=BLOCKS)
+    k, v = _rows(dev, L, 2)
+    call = lambda: st.write_rows(slots=torch.tensor([28, 29], device=dev), keys=k, values=v)  # noqa: E731
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(AssertionError, match="captured"):
+            call()
+    call()
+    assert not st.directory().any()
+
+
+def test_no_rows(dev, store):
+    k, v = _rows(dev, L, 0)
+    store.write_rows(slots=torch.empty(0, dtype=torch.int64, device=dev), keys=k, values=v)
+    assert store.directory().tolist() == [[0] + [1] * (BLOCKS - 1)] * L
+
+
+@pytest.mark.parametrize("bad", [dict(slots=torch.arange(2, dtype=torch.int32)), dict(keys=torch.zeros(L, 2, H, D)),
+                                 dict(values=torch.zeros(2, H, D).bfloat16()), dict(layer=0)])
+def test_refused_calls_change_nothing(dev, store, bad):
+    k, v = _rows(dev, L, 2)
+    args = dict(slots=torch.tensor([28, 29], device=dev), keys=k, values=v)
+    with pytest.raises(AssertionError):
+        store.write_rows(**{**args, **{n: t.to(dev) if torch.is_tensor(t) else t for n, t in bad.items()}})
+    assert store.directory().tolist() == [[0] + [1] * (BLOCKS - 1)] * L
