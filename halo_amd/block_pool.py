@@ -15,6 +15,9 @@ One speculative step of a batch, all of it on the device::
                tree_attention(q, k_pool[layer], v_pool[layer], block_table, lengths, up.cu_rows, mask=mask, ...)
     lengths = commit_path(k_pool, v_pool, block_table, lengths, path, n_path)   # all layers
 
+The calls know blocks, not tiers: where a store moves blocks between tiers,
+``TieredStorage.write_rows`` is ``append_rows`` with the tier directory kept.
+
 No call waits for the device, so a step can be captured in a HIP graph; the
 tensors a call changes are the caller's.  The calls run on ``stream`` (default:
 the current stream of the tensors' device).

@@ -46,9 +46,10 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     q.dtype), and with ``return_lse`` lse (N, H) fp32, both in ``out`` and ``lse``
     if given; rows of no request keep what they hold there.  The softmax and all
     sums are fp32; for 16-bit pools its weights are rounded once to the pool's
-    type (fp16 weights below 2^-21 of the largest are off by at most 2^-32 of
-    it).  Equal calls give equal bits; where a request's rows are cut, and so its
-    last bits, goes by all the requests of the call.  No gradient is kept."""
+    type (fp16 weights below 2^-21 of the largest are off by at most 2^-32 of it;
+    fp16 scores beyond 2^29 are not covered).  Equal calls give equal bits; where
+    a request's rows are cut, and so its last bits, goes by all the requests of
+    the call.  No gradient is kept."""
     if pool_calls.calls is not None and stream is None and out_dtype is None:
         r = pool_calls.calls.tree_attention(q, k_pool, v_pool, block_table, lengths, cu_nodes, max_nodes, mask, scale,
                                             out, lse, return_lse)
