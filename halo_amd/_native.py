@@ -177,6 +177,40 @@ _SIGNATURES = {
     ]),
     "halo_commit_path": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
                                 _c_void_p, _c_void_p]),
+    "halo_chunk_workspace_size": (_size_t, [_i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32]),
+    "halo_chunk_attn": (_i32, [
+        _c_void_p, _c_void_p, _i64, _i64, _i32, _i32,    # pool (halo_block_pool), q, strides, N, H
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i32,  # table, stride, B, W, lengths, cu_rows, max_rows
+        _f32, _c_void_p, _i64, _i64, _i32, _c_void_p,    # scale, out, strides, out_dtype, lse
+        _c_void_p, _size_t, _c_void_p,                   # workspace, bytes, stream
+    ]),
+    "halo_rotate_rows": (_i32, [
+        _c_void_p, _c_void_p, _i64, _i64, _i32,          # pool (halo_block_pool), q, strides, H
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,    # k, v, strides
+        _c_void_p, _i64, _i64, _i32,                     # out, strides, N
+        _c_void_p, _i32, _c_void_p, _c_void_p, _i64, _i64, _i32, _i32,  # positions, pos64, cos, sin, stride, rows, R, interleaved
+        _c_void_p, _i32, _c_void_p, _i32, _f32,          # q_norm, fp32, k_norm, fp32, eps
+        _c_void_p, _c_void_p,                            # slots, stream
+    ]),
+    "halo_fork_workspace_size": (_size_t, [_i32, _i32, _i32]),
+    "halo_fork_blocks": (_i32, [
+        _c_void_p, _c_void_p, _i64, _c_void_p, _i32, _i32,       # pool, table, stride, n_blocks, B, W
+        _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # free, cap, n_free, shared, lengths, source
+        _c_void_p, _c_void_p, _c_void_p, _size_t, _c_void_p,     # new_lengths, ok, workspace, bytes, stream
+    ]),
+    "halo_compact_workspace_size": (_size_t, [_i32]),
+    "halo_compact_blocks": (_i32, [
+        _c_void_p, _c_void_p, _i64, _c_void_p, _i32, _i32,       # pool, table, stride, n_blocks, B, W
+        _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # free, cap, n_free, shared, new_id, n_used
+        _c_void_p, _size_t, _c_void_p,                           # workspace, bytes, stream
+    ]),
+    "halo_verify_workspace_size": (_size_t, [_i32, _i32]),
+    "halo_verify_tree": (_i32, [
+        _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32,  # tokens, parents, cu_nodes, B, N, max_nodes, V, dtype
+        _c_void_p, _i64, _c_void_p, _i64, _i32,          # probs, stride, draft_probs, stride, replacement
+        _c_void_p, _c_void_p, _i32,                      # accept, sample, max_path
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size_t, _c_void_p,  # path, n_path, token, workspace, bytes, stream
+    ]),
     "halo_copy_blocks": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32, _i64,
                                 _c_void_p, _i32, _c_void_p]),
     "halo_set_tier": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _c_void_p]),

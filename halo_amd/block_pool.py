@@ -312,3 +312,101 @@ def commit_path(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
                                      lengths.data_ptr(), path.data_ptr(), path.shape[1], path.shape[1],
                                      n_path.data_ptr(), out.data_ptr(), nat.stream_ptr()), "halo_commit_path")
     return out
+
+
+def _changed_apart(changed, read) -> None:
+    """Changed tensors share no memory with each other or with what is read."""
+    for i, (t, name) in enumerate(changed):
+        if any(overlap(t, u) for u, _ in changed[i + 1:]) or any(overlap(t, u) for u in read):
+            raise AssertionError(f"{name} is changed: it must not share memory with the call's other tensors")
+
+
+def _check_owners(block_table, n_blocks, free_blocks, n_free, shared, k_pool, B: int):
+    dev = k_pool.device
+    if B < 1:
+        raise AssertionError("no requests")
+    check_table(block_table, B, dev)
+    check_ints(n_blocks, "n_blocks", (B,), dev)
+    check_ints(n_free, "n_free", (1,), dev)
+    check_ints(free_blocks, "free_blocks", (free_blocks.numel(),), dev)
+    check_ints(shared, "shared", (k_pool.shape[-4],), dev)
+    return [(block_table, "block_table"), (n_blocks, "n_blocks"), (free_blocks, "free_blocks"), (n_free, "n_free"),
+            (shared, "shared")]
+
+
+def fork_blocks(block_table: torch.Tensor, n_blocks: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor,
+                shared: torch.Tensor, lengths: torch.Tensor, source: torch.Tensor, k_pool: torch.Tensor,
+                v_pool: torch.Tensor, *, stream=None):
+    """Requests that go on with other requests' blocks: beams, samples of one
+    prompt, a common beginning; and requests that give theirs up.
+
+    Row b of the tables becomes what row ``source[b]`` (B, int32) was before the
+    call; a value outside [0, B) gives b's blocks up.  The full blocks of a
+    row's ``lengths`` are shared by all that go on with it, and the partly filled
+    one behind them is copied, in every layer of the pools, for all but one: the
+    row's heir, which is the row itself if it stays, else the lowest b, has all
+    its blocks (those beyond its rows too).  ``shared`` (blocks of the pool)
+    int32, 0 at first, counts how many requests beyond the first have a block.
+    Changed in place, as ``update_block_tables`` takes them: ``block_table`` (B,
+    W), ``n_blocks``, ``free_blocks``, ``n_free``; and ``shared`` and the pools.
+    Blocks that nobody has any more go on the free list, in the order of their
+    ids, before the copies' blocks come from it, in the order of b.
+
+    Returns the new lengths (B) int32 (0 for rows given up, at most the rows of
+    a request's blocks) and ``ok`` (1) bool: False where the free list does not
+    cover the copies, and then nothing has changed.
+
+    A request that shares blocks is given up here, not by a length of 0 in
+    ``update_block_tables``, which knows no ``shared``: there its length may grow
+    and fall, but not below the rows of its shared blocks.  B <= 4096."""
+    L = nat.lib()
+    pool = pack_pool(k_pool, v_pool, written=True)
+    dev = k_pool.device
+    B = lengths.numel()
+    changed = _check_owners(block_table, n_blocks, free_blocks, n_free, shared, k_pool, B)
+    check_ints(lengths, "lengths", (B,), dev)
+    check_ints(source, "source", (B,), dev)
+    _changed_apart(changed + [(k_pool, "k_pool"), (v_pool, "v_pool")], (lengths, source))
+    W = block_table.shape[1]
+    with on_stream(dev, stream):
+        new = torch.empty(B, device=dev, dtype=torch.int32)
+        ok = torch.empty(1, device=dev, dtype=torch.bool)
+        nbytes = L.halo_fork_workspace_size(B, W, shared.numel())
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        nat.check(L.halo_fork_blocks(pool, block_table.data_ptr(), block_table.stride(0) if B > 1 else W,
+                                     n_blocks.data_ptr(), B, W, free_blocks.data_ptr(), free_blocks.numel(),
+                                     n_free.data_ptr(), shared.data_ptr(), lengths.data_ptr(), source.data_ptr(),
+                                     new.data_ptr(), ok.data_ptr(), ws.data_ptr(), nbytes, nat.stream_ptr()),
+                  "halo_fork_blocks")
+    return new, ok
+
+
+def compact_blocks(block_table: torch.Tensor, n_blocks: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor,
+                   shared: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, *, stream=None):
+    """Moves the used blocks of the pools ([L,] blocks, H_kv, block_size, D) to
+    their front: of the blocks in the tables and in the free list the first in
+    the order of ids are the used ones afterwards, so that the pool's end can be
+    given back or handed on.  Blocks behind these move, in order, into the free
+    ones among them; other blocks stay.
+
+    ``block_table``, ``free_blocks`` (the lowest id on top), ``n_free`` and
+    ``shared`` (see ``fork_blocks``; zeros where no blocks are shared) are changed
+    in place.  Returns ``new_id`` (blocks) int32, where each block is now, for
+    what else names blocks (slots not written yet), and ``n_used`` (1) int32."""
+    L = nat.lib()
+    pool = pack_pool(k_pool, v_pool, written=True)
+    dev = k_pool.device
+    B = n_blocks.numel()
+    changed = _check_owners(block_table, n_blocks, free_blocks, n_free, shared, k_pool, B)
+    _changed_apart(changed + [(k_pool, "k_pool"), (v_pool, "v_pool")], ())
+    W = block_table.shape[1]
+    with on_stream(dev, stream):
+        new_id = torch.empty(shared.numel(), device=dev, dtype=torch.int32)
+        n_used = torch.empty(1, device=dev, dtype=torch.int32)
+        nbytes = L.halo_compact_workspace_size(shared.numel())
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        nat.check(L.halo_compact_blocks(pool, block_table.data_ptr(), block_table.stride(0) if B > 1 else W,
+                                        n_blocks.data_ptr(), B, W, free_blocks.data_ptr(), free_blocks.numel(),
+                                        n_free.data_ptr(), shared.data_ptr(), new_id.data_ptr(), n_used.data_ptr(),
+                                        ws.data_ptr(), nbytes, nat.stream_ptr()), "halo_compact_blocks")
+    return new_id, n_used

@@ -296,29 +296,6 @@ __global__ void __launch_bounds__(kSlotThreads) slots_kernel(TableParams P) {
 // Rows to their slots and along an accepted path: copies of whole rows, PB
 // bytes a thread (16 where everything is aligned for it).
 // ---------------------------------------------------------------------------
-struct PoolView {
-  char* k;
-  char* v;
-  int64_t sl, sb, sh, sr;  // strides in bytes
-  int layers, blocks, H_kv, D_bytes;
-  Div bs;
-};
-
-template <int PB>
-struct Piece;
-template <>
-struct Piece<16> {
-  typedef __attribute__((ext_vector_type(4))) uint32_t type;
-};
-template <>
-struct Piece<4> {
-  typedef uint32_t type;
-};
-template <>
-struct Piece<2> {
-  typedef uint16_t type;
-};
-
 struct AppendParams {
   PoolView pool;
   const char* k;
@@ -457,7 +434,7 @@ __global__ void __launch_bounds__(kTreeThreads)
   __shared__ uint64_t s_bits[NODES][WORDS];
   __shared__ int s_up[NODES];
   const int lo = max(cu[blockIdx.x], 0);
-  const int n = min(min(cu[blockIdx.x + 1], N) - lo, max_nodes);
+  const int n = min(min(max(cu[blockIdx.x + 1], 0), N) - lo, max_nodes);
   if (n <= 0) return;
   uint64_t bits[PER][WORDS];
   int up[PER];
@@ -519,38 +496,6 @@ __global__ void __launch_bounds__(kTreeThreads)
 }  // namespace halo
 
 using namespace halo;
-
-namespace {
-
-int check_pool(const halo_block_pool* pool, PoolView* out) {
-  HALO_CHECK_ARG(pool && pool->k && pool->v, "null pool");
-  HALO_CHECK_ARG(pool->dtype == HALO_F32 || pool->dtype == HALO_BF16 || pool->dtype == HALO_F16, "bad pool dtype");
-  HALO_CHECK_ARG(pool->layers > 0 && pool->blocks > 0 && pool->H_kv > 0 && pool->block_size > 0 && pool->D > 0,
-                 "pool sizes must be positive");
-  HALO_CHECK_ARG((int64_t)pool->blocks * pool->block_size < (1ll << 31), "a pool holds at most 2^31 - 1 rows");
-  const int64_t es = elem_size(pool->dtype);
-  out->k = static_cast<char*>(pool->k);
-  out->v = static_cast<char*>(pool->v);
-  out->sl = pool->stride_l * es;
-  out->sb = pool->stride_b * es;
-  out->sh = pool->stride_h * es;
-  out->sr = pool->stride_r * es;
-  out->layers = pool->layers;
-  out->blocks = pool->blocks;
-  out->H_kv = pool->H_kv;
-  out->D_bytes = (int)(pool->D * es);
-  out->bs = make_div(pool->block_size);
-  return HALO_OK;
-}
-
-// The widest piece that every row start is a multiple of.
-int piece_bytes(const PoolView& p, uint64_t more) {
-  const uint64_t all = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | (uint64_t)p.sl |
-                       (uint64_t)p.sb | (uint64_t)p.sh | (uint64_t)p.sr | (uint64_t)p.D_bytes | more;
-  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
-}
-
-}  // namespace
 
 extern "C" int halo_update_block_tables(int32_t* table, int64_t table_stride, int32_t* n_blocks, int B, int W,
                                         int32_t* free_blocks, int n_cap, int32_t* n_free, const int32_t* lengths,

@@ -1,4 +1,4 @@
-// What the block-pool kernels share: positions to blocks and rows.
+// What the block-pool kernels share: pools, positions to blocks and rows.
 #pragma once
 
 #include "common.hpp"
@@ -55,6 +55,58 @@ __device__ __forceinline__ float lane_of(float v, int lane) {
 __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | lo);
+}
+
+// A pool as the kernels address it.
+struct PoolView {
+  char* k;
+  char* v;
+  int64_t sl, sb, sh, sr;  // strides in bytes
+  int layers, blocks, H_kv, D_bytes;
+  Div bs;
+};
+
+template <int PB>
+struct Piece;
+template <>
+struct Piece<16> {
+  typedef __attribute__((ext_vector_type(4))) uint32_t type;
+};
+template <>
+struct Piece<4> {
+  typedef uint32_t type;
+};
+template <>
+struct Piece<2> {
+  typedef uint16_t type;
+};
+
+inline int check_pool(const halo_block_pool* pool, PoolView* out) {
+  HALO_CHECK_ARG(pool && pool->k && pool->v, "null pool");
+  HALO_CHECK_ARG(pool->dtype == HALO_F32 || pool->dtype == HALO_BF16 || pool->dtype == HALO_F16, "bad pool dtype");
+  HALO_CHECK_ARG(pool->layers > 0 && pool->blocks > 0 && pool->H_kv > 0 && pool->block_size > 0 && pool->D > 0,
+                 "pool sizes must be positive");
+  HALO_CHECK_ARG((int64_t)pool->blocks * pool->block_size < (1ll << 31), "a pool holds at most 2^31 - 1 rows");
+  const int64_t es = elem_size(pool->dtype);
+  out->k = static_cast<char*>(pool->k);
+  out->v = static_cast<char*>(pool->v);
+  out->sl = pool->stride_l * es;
+  out->sb = pool->stride_b * es;
+  out->sh = pool->stride_h * es;
+  out->sr = pool->stride_r * es;
+  out->layers = pool->layers;
+  out->blocks = pool->blocks;
+  out->H_kv = pool->H_kv;
+  out->D_bytes = (int)(pool->D * es);
+  out->bs = make_div(pool->block_size);
+  return HALO_OK;
+}
+
+// The widest piece that every row start is a multiple of.
+inline int piece_bytes(const PoolView& p, uint64_t more) {
+  const uint64_t all = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | (uint64_t)p.sl |
+                       (uint64_t)p.sb | (uint64_t)p.sh | (uint64_t)p.sr | (uint64_t)p.D_bytes | more;
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
 }
 
 }  // namespace halo

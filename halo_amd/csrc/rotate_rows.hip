@@ -1,0 +1,222 @@
+// Rows on their way into a paged cache (gfx950, wave64): heads of queries and
+// keys normed and rotated, keys and values written to their slots of the pool.
+//
+//   y = x w / sqrt(mean(x^2) + eps)                       (with a weight w, else y = x)
+//   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s)          c, s: cosine and sine of the row's position and the pair
+// for the pairs (i, i + R/2), or (2i, 2i + 1), of a head's first R channels;
+// all of it in fp32, rounded once.  The model library rounds after the norm and
+// after the rotation; here the row is read and written once.  The reference
+// leaves both to the model and attends what it is handed.
+//
+// A head's D channels are D / 16 lanes of two 8-channel pieces.  For the pairs
+// (i, i + R/2) the pieces of a lane are R/2 channels apart, so both of a pair
+// are in one lane, and its cosines and sines are 8 floats in a row either way.
+#include "block_pool.hpp"
+
+namespace halo {
+namespace {
+
+struct RotateParams {
+  PoolView pool;
+  const char* q;
+  const char* k;
+  const char* v;
+  char* out;
+  int64_t qsn, qsh, ksn, ksh, vsn, vsh, osn, osh;  // strides in bytes
+  int H, H_kv, N, parts;
+  Div per_row;  // parts
+  const void* positions;
+  int pos64;
+  const float* cos;
+  const float* sin;
+  int64_t trig_stride;
+  int64_t trig_rows;
+  int R, interleaved;
+  const void* q_norm;
+  const void* k_norm;
+  int q_norm_f32, k_norm_f32;
+  float eps;
+  const int64_t* slots;
+};
+
+constexpr int kRotThreads = 256;
+
+template <int DT>
+__device__ __forceinline__ void load8(const char* p, float* f) {
+  if constexpr (DT == HALO_F32) {
+    unpack16<DT>(*reinterpret_cast<const uint4*>(p), f);
+    unpack16<DT>(*reinterpret_cast<const uint4*>(p + 16), f + 4);
+  } else {
+    unpack16<DT>(*reinterpret_cast<const uint4*>(p), f);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store8(char* p, const float* f) {
+  store_elem4(p, 0, DT, f);
+  store_elem4(p, 4, DT, f + 4);
+}
+
+// Sum over the G = 4 or 8 lanes of a head.
+template <int G>
+__device__ __forceinline__ float head_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false));  // lane ^ 1
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false));  // lane ^ 2
+  if (G == 8) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, false));  // 7 - lane
+  return v;
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P) {
+  constexpr int G = D / 16;  // lanes of a head
+  constexpr int ES = DT == HALO_F32 ? 4 : 2;
+  const int lane = threadIdx.x & (G - 1);
+  const int unit = blockIdx.x * (kRotThreads / G) + threadIdx.x / G;
+  const int n = div_by(unit, P.per_row);
+  if (n >= P.N) return;
+  const int part = unit - n * P.parts;
+  const int R = P.R, heads = P.H + 2 * P.H_kv;
+  const bool halves = !P.interleaved && 16 * lane < R;
+  const int ca = halves ? 8 * lane : 16 * lane, cb = halves ? R / 2 + 8 * lane : 16 * lane + 8;
+
+  float c[8], s[8];
+  if (16 * lane < R) {
+    int64_t pos = P.pos64 ? reinterpret_cast<const int64_t*>(P.positions)[n] : reinterpret_cast<const int32_t*>(P.positions)[n];
+    const bool there = pos >= 0 && pos < P.trig_rows;
+    pos = there ? pos : 0;
+    const float* cr = P.cos + pos * P.trig_stride + 8 * lane;
+    const float* sr = P.sin + pos * P.trig_stride + 8 * lane;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = there ? cr[i] : __uint_as_float(0x7fc00000u);
+      s[i] = sr[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+  }
+  const int64_t slot = P.slots[n];
+  const bool kept = slot >= 0 && slot < (int64_t)P.pool.blocks * P.pool.bs.d;
+  const int blk = kept ? div_by((int)slot, P.pool.bs) : 0;
+  const int64_t place = blk * P.pool.sb + (slot - (int64_t)blk * P.pool.bs.d) * P.pool.sr;
+
+  for (int h = part; h < heads; h += P.parts) {
+    const bool is_q = h < P.H, is_v = h >= P.H + P.H_kv;
+    if (!is_q && !kept) continue;
+    const int hk = h - P.H - (is_v ? P.H_kv : 0);
+    const char* src = is_q ? P.q + n * P.qsn + h * P.qsh : is_v ? P.v + n * P.vsn + hk * P.vsh : P.k + n * P.ksn + hk * P.ksh;
+    char* dst = is_q ? P.out + n * P.osn + h * P.osh : (is_v ? P.pool.v : P.pool.k) + place + hk * P.pool.sh;
+    float a[8], b[8];
+    load8<DT>(src + ca * ES, a);
+    load8<DT>(src + cb * ES, b);
+    if (!is_v) {
+      const void* w = is_q ? P.q_norm : P.k_norm;
+      if (w != nullptr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a[i], a[i], __builtin_fmaf(b[i], b[i], sum));
+        const float inv = 1.f / sqrtf(head_sum<G>(sum) * (1.f / D) + P.eps);
+        const int wdt = (is_q ? P.q_norm_f32 : P.k_norm_f32) ? HALO_F32 : DT;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[i] = a[i] * inv * load_elem(w, ca + i, wdt);
+          b[i] = b[i] * inv * load_elem(w, cb + i, wdt);
+        }
+      }
+      if (16 * lane < R) {
+        if (P.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
+            a[i] = a0 * c[i / 2] - a1 * s[i / 2];
+            a[i + 1] = a1 * c[i / 2] + a0 * s[i / 2];
+            b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
+            b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = a[i], y = b[i];
+            a[i] = x * c[i] - y * s[i];
+            b[i] = y * c[i] + x * s[i];
+          }
+        }
+      }
+    }
+    store8<DT>(dst + ca * ES, a);
+    store8<DT>(dst + cb * ES, b);
+  }
+}
+
+}  // namespace
+}  // namespace halo
+
+using namespace halo;
+
+extern "C" int halo_rotate_rows(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int H,
+                                const void* k, int64_t k_stride_n, int64_t k_stride_h, const void* v,
+                                int64_t v_stride_n, int64_t v_stride_h, void* out, int64_t out_stride_n,
+                                int64_t out_stride_h, int N, const void* positions, int pos64, const float* cos,
+                                const float* sin, int64_t trig_stride, int64_t trig_rows, int R, int interleaved,
+                                const void* q_norm, int q_norm_f32, const void* k_norm, int k_norm_f32, float eps,
+                                const int64_t* slots, void* stream) {
+  RotateParams p;
+  const int rc = check_pool(pool, &p.pool);
+  if (rc != HALO_OK) return rc;
+  HALO_CHECK_ARG(pool->layers == 1, "need a pool of one layer");
+  HALO_CHECK_ARG(pool->D == 64 || pool->D == 128, "head_dim must be 64 or 128");
+  HALO_CHECK_ARG(R > 0 && R <= pool->D && R % 16 == 0, "need 16 <= R <= D in steps of 16");
+  HALO_CHECK_ARG(N >= 0 && H > 0, "bad sizes");
+  HALO_CHECK_ARG(eps >= 0.f && std::isfinite(eps), "eps must be finite and not negative");
+  if (N == 0) return HALO_OK;
+  HALO_CHECK_ARG(q && k && v && out && positions && cos && sin && slots, "null pointer argument");
+  HALO_CHECK_ARG(trig_rows > 0 && trig_stride >= R / 2 && trig_stride % 4 == 0 &&
+                     (reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16 == 0,
+                 "rows of cosines and sines must be 16-byte aligned and not overlap");
+  const int64_t es = elem_size(pool->dtype);
+  HALO_CHECK_ARG(piece_bytes(p.pool, 0) == 16, "pool rows must be 16-byte aligned");
+  p.q = static_cast<const char*>(q);
+  p.k = static_cast<const char*>(k);
+  p.v = static_cast<const char*>(v);
+  p.out = static_cast<char*>(out);
+  p.qsn = q_stride_n * es, p.qsh = q_stride_h * es, p.ksn = k_stride_n * es, p.ksh = k_stride_h * es;
+  p.vsn = v_stride_n * es, p.vsh = v_stride_h * es, p.osn = out_stride_n * es, p.osh = out_stride_h * es;
+  HALO_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                  reinterpret_cast<uintptr_t>(out) | (uint64_t)(p.qsn | p.qsh | p.ksn | p.ksh | p.vsn | p.vsh | p.osn | p.osh)) %
+                         16 == 0,
+                 "rows must be 16-byte aligned");
+  const int64_t heads = (int64_t)H + 2 * (int64_t)pool->H_kv;
+  HALO_CHECK_ARG(heads * N < (1ll << 31) - kRotThreads, "heads of all rows in 31 bits");
+  p.H = H;
+  p.H_kv = pool->H_kv;
+  p.N = N;
+  p.parts = (int)heads;
+  p.per_row = make_div(p.parts);
+  p.positions = positions;
+  p.pos64 = pos64;
+  p.cos = cos;
+  p.sin = sin;
+  p.trig_stride = trig_stride;
+  p.trig_rows = trig_rows;
+  p.R = R;
+  p.interleaved = interleaved;
+  p.q_norm = q_norm;
+  p.k_norm = k_norm;
+  p.q_norm_f32 = q_norm_f32;
+  p.k_norm_f32 = k_norm_f32;
+  p.eps = eps;
+  p.slots = slots;
+  const int per = kRotThreads / (pool->D / 16);
+  const dim3 grid((unsigned)(((int64_t)p.parts * N + per - 1) / per)), block(kRotThreads);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+#define HALO_ROTATE(DTV)                                                                            \
+  do {                                                                                              \
+    if (pool->D == 128) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128>), grid, block, 0, st, p);  \
+    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64>), grid, block, 0, st, p);                  \
+  } while (0)
+  if (pool->dtype == HALO_F32) HALO_ROTATE(HALO_F32);
+  else if (pool->dtype == HALO_BF16) HALO_ROTATE(HALO_BF16);
+  else HALO_ROTATE(HALO_F16);
+#undef HALO_ROTATE
+  HALO_CHECK_HIP(hipGetLastError());
+  return HALO_OK;
+}

@@ -52,6 +52,10 @@ struct TreeParams {
   float* lse;
   float4* part_o;
   float2* part_ml;
+  // chunks: see chunk_plan_kernel
+  const int32_t* plan;  // items, units that were cut
+  const int4* items;
+  const int32_t* cut_units;
 };
 
 // Narrow kernels (up to 32 rows a unit): the columns of one 32x32 product, key
@@ -69,7 +73,10 @@ constexpr float kTreeLazyMax = 8.0f;
 // 1.8e-4).  Lifted by 2^7 they are off by 2^-32 of the largest at most, and stay
 // below 2^15 for exponents up to 2^30: the tile's max is taken a step up there,
 // since an exponent's exact product may lie half a step above its rounded one,
-// and the step is 32 at 2^28.  bf16 has fp32's exponents.
+// and the step is 32 at 2^28.  The lifted maximum is rounded to such a step too: up
+// to exponents of 2^25 (steps of 2) the largest weight stays above 2^4, from 2^28 on
+// it may fall below fp16's normal range, where the quotients lose their accuracy.
+// bf16 has fp32's exponents.
 template <int DT>
 __device__ __forceinline__ float tree_new_max(float m_old, float bm) {
   constexpr float kLift = DT == HALO_F16 ? 7.0f : 0.0f;
@@ -85,7 +92,7 @@ __device__ __forceinline__ TreeReq tree_req(const TreeParams& P, int b) {
   TreeReq r = {0, 0, 0, 0, 0};
   if (b < P.B) {
     r.lo = max(P.cu[b], 0);
-    r.n = max(min(min(P.cu[b + 1], P.N) - r.lo, P.max_nodes), 0);
+    r.n = max(min(min(max(P.cu[b + 1], 0), P.N) - r.lo, P.max_nodes), 0);  // (a difference of values below 0 could wrap)
     r.ctx = min(max(P.lengths[b], 0), P.W * P.bs.d);
     r.rbs = (r.n * P.rep + R - 1) / R;
     if (r.n > 0) r.tiles = (r.ctx + r.n + KT - 1) / KT;
@@ -98,6 +105,7 @@ struct TreeItem {
   int b, lo, ctx, n, rbs, tiles;
   int h, rb, cut, cuts;  // the cut-th of `cuts` cuts of the unit (h, rb)
   int part;              // partial of the unit's first cut
+  int seen;              // rows from the first on that all rows of the unit see
 };
 
 // Finds item x, EACH requests a lane at once (one round trip to memory up to 64
@@ -189,6 +197,7 @@ __device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeIte
       }
       it.h = z;
       it.part = part + (it.rb * P.H_kv + it.h) * it.cuts;
+      it.seen = it.ctx;
       return true;
     }
     base += lane_of(at, 63);
@@ -205,6 +214,34 @@ __device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeIte
 template <int KT, int R, bool ITEMS>
 __device__ __forceinline__ bool tree_find(const TreeParams& P, int x, TreeItem& it) {
   return P.B <= 64 ? tree_find_of<KT, R, ITEMS, 1>(P, x, it) : tree_find_of<KT, R, ITEMS, 4>(P, x, it);
+}
+
+// The same from the plan of a call of chunks; the heads of an item side by side.
+constexpr int kItemInts4 = 3;
+template <int R, bool ITEMS>
+__device__ __forceinline__ bool chunk_find(const TreeParams& P, int x, TreeItem& it) {
+  const int i = x / P.H_kv;
+  if (i >= P.plan[ITEMS ? 0 : 1]) return false;
+  const int4* at = P.items + (int64_t)(ITEMS ? i : P.cut_units[i]) * kItemInts4;
+  const int4 a = at[0], b = at[1], c = at[2];
+  it.h = x - i * P.H_kv;
+  it.b = uni(a.x);
+  it.rb = uni(a.y);
+  it.cut = uni(a.z);
+  it.cuts = uni(a.w);
+  it.tiles = uni(b.x);
+  it.part = uni(b.y) + it.h * it.cuts;
+  it.lo = uni(b.z);
+  it.ctx = uni(b.w);
+  it.n = uni(c.x);
+  it.rbs = 0;
+  it.seen = it.ctx + it.rb * R / P.rep + 1;
+  return true;
+}
+template <int KT, int R, bool ITEMS, bool CHUNK>
+__device__ __forceinline__ bool find_item(const TreeParams& P, int x, TreeItem& it) {
+  if constexpr (CHUNK) return chunk_find<R, ITEMS>(P, x, it);
+  else return tree_find<KT, R, ITEMS>(P, x, it);
 }
 
 // Staging.  An LDS-DMA instruction fills 1 KiB, lane l its piece l, so RPI rows
@@ -749,7 +786,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // and sums).  Step s of the score product multiplies channel s (lane half 0)
 // and D/2 + s (half 1).  3 requests of up to 1500 rows: 10.2 us, the same chain of
 // search, loads and fold as in the 16-bit kernel, with eight times its MFMA steps.
-template <int D>
+template <int D, bool CHUNK>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_f32_kernel(TreeParams P) {
   constexpr int DB = D / 32, RB = D * 4;
   constexpr int TB = kTreeKT * RB;
@@ -759,13 +796,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __attribute__((aligned(16))) char sK[kTreeWaves][TB], sV[kTreeWaves][TB];
   __shared__ float2 s_ml[kTreeWaves][32];
   TreeItem it;
-  if (!tree_find<kTreeKT, kTreeRows, true>(P, blockIdx.x, it)) return;
+  if (!find_item<kTreeKT, kTreeRows, true, CHUNK>(P, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
   const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
   int t = (int)((int64_t)it.tiles * it.cut / it.cuts) + wave;
-  const int tree0 = it.ctx / kTreeKT;
+  const int tree0 = it.seen / kTreeKT;
   char* const stK = sK[wave];
   char* const stV = sV[wave];
   const char* kh = P.k + (int64_t)it.h * P.sh * 16;
@@ -969,7 +1006,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // 63), 4.3 TB/s, the waves waiting 57 % of their cycles.
 // Four stages of K and V took 57.7 where two took 55.7; finding a tile's places
 // in the step that stages it cost 5 us of 52.
-template <int DT, int D, int NW>
+template <int DT, int D, int NW, bool CHUNK>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) tree_attn_wide_kernel(TreeParams P) {
   constexpr int KT = kTreeWideKT, R = 32 * NW;
   constexpr int KS = D / 16, DB = D / 32, RB = D * 2;
@@ -979,13 +1016,13 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
   static_assert(L::KEYS * NW == KT, "the waves stage the tile");
   __shared__ __attribute__((aligned(16))) char sK0[TB], sK1[TB], sV0[TB], sV1[TB];
   TreeItem it;
-  if (!tree_find<KT, R, true>(P, blockIdx.x, it)) return;
+  if (!find_item<KT, R, true, CHUNK>(P, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
   const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
   const int t0 = (int)((int64_t)it.tiles * it.cut / it.cuts);
-  const int tree0 = it.ctx / KT;  // first tile with tree rows
+  const int tree0 = it.seen / KT;  // first tile with rows that not all see
   const char* kh = P.k + (int64_t)it.h * P.sh * 16;
   const char* vh = P.v + (int64_t)it.h * P.sh * 16;
 
@@ -1273,14 +1310,14 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 // two round trips: 8 units of 17 partials 4.0 us, of 29 5.1; 31 partials of 256 rows
 // of 8 heads (33 MB) 8.9.  For MW see tree_shape.
 constexpr int kMergeBatch = 8;
-template <int D, int DT, int KT, int NW, int MW>
+template <int D, int DT, int KT, int NW, int MW, bool CHUNK>
 __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
   constexpr int PIECES = D / 8, PPW = 4;
   __shared__ float4 s_o[MW][PPW][64];
   __shared__ float2 s_ml[MW][32];
   TreeItem it;
   const int rows32 = NW == 1 ? 0 : blockIdx.x % NW;  // which 32 of the unit's rows
-  if (!tree_find<KT, 32 * NW, false>(P, blockIdx.x / NW, it)) return;
+  if (!find_item<KT, 32 * NW, false, CHUNK>(P, blockIdx.x / NW, it)) return;
   const int row0 = (it.rb * NW + rows32) * 32;
   if (row0 >= it.n * P.rep) return;
   const int lane = threadIdx.x & 63;
@@ -1365,6 +1402,148 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
   if (P.lse != nullptr && blockIdx.y == 0 && wave == 0 && hh == 0) P.lse[row * P.H + head] = tree_lse(M, l);
 }
 
+// ---------------------------------------------------------------------------
+// Chunks: any number of new rows a request, row i sees the rows up to length + i.
+// A unit (request, block of R rows) walks the tiles up to its last row, so units
+// differ, and one workgroup plans the call: with tiles_u the tiles of unit u and
+// H_kv workgroups for each, it weighs cutting the longest unit into c = 1 .. 32
+// and all others into pieces no longer than those,
+//   rounds of 256 workgroups x (mean item + kItemCost) + kPartCost x partials,
+// against the longest item alone, takes the cheapest c whose partials fit the
+// workspace, and lists the items, last rows (most tiles) first.
+// ---------------------------------------------------------------------------
+constexpr int kChunkMaxB = 4096, kPlanThreads = 1024, kCandidates = 32;
+// In tiles: what an item costs besides its tiles (staging its first tiles, its
+// output), and a partial (written and read by all workgroups together).
+constexpr float kItemCost = 3.0f, kPartCost = 0.025f;
+
+struct ChunkPlanParams {
+  TreeParams t;
+  int32_t* plan;
+  int4* items;
+  int32_t* cut_units;
+  int R, KT, min_tiles, unit_cap, part_cap;  // room for units, and for partials (of R rows, all heads)
+};
+
+__global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(ChunkPlanParams C) {
+  const TreeParams& P = C.t;
+  __shared__ int s_at[kChunkMaxB + 1], s_sum[kPlanThreads / 64], s_max, s_best;
+  __shared__ float s_cost[kCandidates];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  auto rows_of = [&](int b, int& lo, int& ctx) {
+    lo = max(P.cu[b], 0);
+    ctx = (int)min((int64_t)max(P.lengths[b], 0), (int64_t)P.W * P.bs.d);
+    return max(min(min(max(P.cu[b + 1], 0), P.N) - lo, P.max_nodes), 0);  // (a difference of values below 0 could wrap)
+  };
+  // Sum over the threads before this one, and of all.
+  auto scan = [&](int x, int& all) {
+    const int in = wave_prefix(x);
+    __syncthreads();
+    if (lane == 63) s_sum[wave] = in;
+    __syncthreads();
+    const int t = lane < kPlanThreads / 64 ? s_sum[lane] : 0;
+    const int ws = wave_prefix(t);
+    all = lane_of(ws, kPlanThreads / 64 - 1);
+    return lane_of(ws - t, wave) + in - x;
+  };
+  auto tiles_at = [&](int ctx, int n, int rb) {
+    const int last = min((int)min((int64_t)(rb + 1) * C.R, (int64_t)n * P.rep) - 1, n * P.rep - 1) / P.rep;
+    return (ctx + last + C.KT) / C.KT;
+  };
+  if (tid == 0) s_max = 0;
+  __syncthreads();
+  const int per = (P.B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(tid * per, P.B), b1 = min(b0 + per, P.B);
+  int mine = 0, pairs, longest = 0;
+  for (int b = b0; b < b1; ++b) {
+    int lo, ctx;
+    const int n = rows_of(b, lo, ctx), rbs = (int)(((int64_t)n * P.rep + C.R - 1) / C.R);
+    mine += rbs;
+    if (n > 0) longest = max(longest, tiles_at(ctx, n, rbs - 1));
+  }
+  int at = scan(mine, pairs);
+  for (int b = b0; b < b1; ++b) {
+    int lo, ctx;
+    s_at[b] = at;
+    at += (int)(((int64_t)rows_of(b, lo, ctx) * P.rep + C.R - 1) / C.R);
+  }
+  if (tid == 0) s_at[P.B] = pairs;
+  atomicMax(&s_max, longest);
+  __syncthreads();
+  longest = s_max;
+  pairs = min(pairs, C.unit_cap);  // more only if the requests' rows overlap
+  if (pairs == 0) {
+    if (tid == 0) C.plan[0] = C.plan[1] = 0;
+    return;
+  }
+  auto find = [&](int u) {  // the request of unit u
+    int b = 0;
+    for (int s = 1 << (31 - __clz(P.B)); s > 0; s >>= 1)
+      if (b + s < P.B && s_at[b + s] <= u) b += s;
+    return b;  // the last that starts at or before u, which has rows
+  };
+  auto tiles_of = [&](int u, int& b, int& n, int& lo, int& ctx) {
+    b = find(u);
+    n = rows_of(b, lo, ctx);
+    return tiles_at(ctx, n, u - s_at[b]);
+  };
+  for (int c = wave; c < kCandidates; c += kPlanThreads / 64) {
+    const int L = max((longest + c) / (c + 1), C.min_tiles);
+    int64_t items = 0, parts = 0;
+    float total = 0.f;
+    for (int u = lane; u < pairs; u += 64) {
+      int b, n, lo, ctx;
+      const int t = tiles_of(u, b, n, lo, ctx), cuts = (t + L - 1) / L;
+      items += cuts;
+      parts += cuts > 1 ? cuts : 0;
+      total += (float)t;
+    }
+    items = lane_of(wave_prefix(items), 63) * P.H_kv;
+    parts = lane_of(wave_prefix(parts), 63) * P.H_kv;
+    total = lane_of(wave_prefix(total), 63) * (float)P.H_kv;
+    const float mean = total / (float)items;
+    const float rounds = (float)((items + 255) / 256) * (mean + kItemCost);
+    const float cost = fmaxf(rounds, (float)min(L, longest) + kItemCost) + kPartCost * (float)parts;
+    if (lane == 0) s_cost[c] = parts <= C.part_cap ? cost : INFINITY;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int best = 0;
+    for (int c = 1; c < kCandidates; ++c)
+      if (s_cost[c] < s_cost[best]) best = c;
+    s_best = best;
+  }
+  __syncthreads();
+  const int L = max((longest + s_best) / (s_best + 1), C.min_tiles);
+  int base = 0, part = 0, cut_base = 0;
+  for (int u0 = 0; u0 < pairs; u0 += kPlanThreads) {
+    const int u = pairs - 1 - (u0 + tid);
+    int b = 0, n = 0, lo = 0, ctx = 0, t = 0, cuts = 0;
+    if (u >= 0) {
+      t = tiles_of(u, b, n, lo, ctx);
+      cuts = (t + L - 1) / L;
+    }
+    int all, all_parts, all_cut;
+    const int i0 = base + scan(cuts, all);
+    const int p0 = part + scan(cuts > 1 ? cuts * P.H_kv : 0, all_parts);
+    const int c0 = cut_base + scan(cuts > 1, all_cut);
+    for (int k = 0; k < cuts; ++k) {
+      int4* it = C.items + (int64_t)(i0 + k) * kItemInts4;
+      it[0] = make_int4(b, u - s_at[b], k, cuts);
+      it[1] = make_int4(t, p0, lo, ctx);
+      it[2] = make_int4(n, 0, 0, 0);
+    }
+    if (cuts > 1) C.cut_units[c0] = i0;
+    base += all;
+    part += all_parts;
+    cut_base += all_cut;
+  }
+  if (tid == 0) {
+    C.plan[0] = base;
+    C.plan[1] = cut_base;
+  }
+}
+
 }  // namespace halo
 
 using namespace halo;
@@ -1430,11 +1609,14 @@ extern "C" size_t halo_tree_workspace_size(int dtype, int B, int H, int H_kv, in
   return (size_t)tree_shape(dtype, B, H, H_kv, D, max_rows, max_nodes).partials * (size_t)tree_part_bytes(D);
 }
 
-extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h,
-                              int N, int H, const int32_t* table, int64_t table_stride, int B, int W,
-                              const int32_t* lengths, const int32_t* cu_nodes, int max_nodes, const int64_t* mask,
-                              int64_t mask_stride, float scale, void* out, int64_t out_stride_n, int64_t out_stride_h,
-                              int out_dtype, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+namespace {
+
+// Checks what calls of trees and of chunks have in common, and enters it.
+// `size_nodes`: the rows of a request that the launch's sizes are made for.
+int tree_params(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int N, int H,
+                const int32_t* table, int64_t table_stride, int B, int W, const int32_t* lengths, const int32_t* cu_nodes,
+                int max_nodes, int size_nodes, const int64_t* mask, int64_t mask_stride, float scale, void* out,
+                int64_t out_stride_n, int64_t out_stride_h, int out_dtype, float* lse, TreeParams* p) {
   HALO_CHECK_ARG(pool && pool->k && pool->v && table && lengths && cu_nodes, "null pointer argument");
   const int dtype = pool->dtype, D = pool->D, H_kv = pool->H_kv;
   HALO_CHECK_ARG(dtype == HALO_BF16 || dtype == HALO_F16 || dtype == HALO_F32, "dtype must be bf16, f16 or f32");
@@ -1442,9 +1624,10 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   HALO_CHECK_ARG(pool->layers == 1 && pool->blocks > 0 && pool->block_size > 0 && W > 0, "need a pool of one layer");
   HALO_CHECK_ARG(D == 64 || D == 128, "head_dim must be 64 or 128");
   HALO_CHECK_ARG(N >= 0, "bad number of nodes");
+  p->N = 0;
   if (N == 0) return HALO_OK;
   HALO_CHECK_ARG(q && out, "null pointer argument");
-  HALO_CHECK_ARG(tree_sizes_ok(B, H, H_kv, D, (int64_t)W * pool->block_size, max_nodes),
+  HALO_CHECK_ARG(tree_sizes_ok(B, H, H_kv, D, (int64_t)W * pool->block_size, size_nodes),
                  "need H % H_kv == 0, 1 <= max_nodes <= 512 and positive sizes in 31 bits");
   HALO_CHECK_ARG(table_stride >= W, "rows of the block table overlap");
   HALO_CHECK_ARG(mask == nullptr || mask_stride >= (max_nodes + 63) / 64, "mask rows are shorter than max_nodes bits");
@@ -1463,6 +1646,57 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   const int64_t last = ((int64_t)(pool->blocks - 1) * pool->stride_b + (pool->block_size - 1) * pool->stride_r) / lanes;
   HALO_CHECK_ARG(last < 0xffffffffll && pool->stride_h / lanes * (H_kv - 1) < 0xffffffffll, "pool larger than 64 GiB");
   HALO_CHECK_ARG(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
+  p->q = q;
+  p->q_stride_n = q_stride_n;
+  p->q_stride_h = q_stride_h;
+  p->k = static_cast<const char*>(pool->k);
+  p->v = static_cast<const char*>(pool->v);
+  p->sb = (uint32_t)(pool->stride_b / lanes);
+  p->sh = (uint32_t)(pool->stride_h / lanes);
+  p->sr = (uint32_t)(pool->stride_r / lanes);
+  p->blocks = pool->blocks;
+  p->bs = make_div(pool->block_size);
+  p->table = table;
+  p->table_stride = table_stride;
+  p->W = W;
+  p->lengths = lengths;
+  p->cu = cu_nodes;
+  p->mask = reinterpret_cast<const uint32_t*>(mask);
+  p->mask_stride = 2 * mask_stride;
+  p->B = B;
+  p->H = H;
+  p->H_kv = H_kv;
+  p->rep = H / H_kv;
+  p->N = N;
+  p->max_nodes = max_nodes;
+  p->slots = p->min_tiles = 0;
+  p->scale2 = (float)((double)scale * 1.4426950408889634);
+  HALO_CHECK_ARG(p->scale2 >= 0x1p-126f && std::isfinite(p->scale2), "scale out of range");
+  p->out = out;
+  p->o_stride_n = out_stride_n;
+  p->o_stride_h = out_stride_h;
+  p->out_f32 = out_dtype == HALO_F32;
+  p->lse = lse;
+  p->part_o = nullptr;
+  p->part_ml = nullptr;
+  p->plan = nullptr;
+  p->items = nullptr;
+  p->cut_units = nullptr;
+  return HALO_OK;
+}
+
+}  // namespace
+
+extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h,
+                              int N, int H, const int32_t* table, int64_t table_stride, int B, int W,
+                              const int32_t* lengths, const int32_t* cu_nodes, int max_nodes, const int64_t* mask,
+                              int64_t mask_stride, float scale, void* out, int64_t out_stride_n, int64_t out_stride_h,
+                              int out_dtype, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  TreeParams p;
+  const int rc = tree_params(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_nodes, max_nodes,
+                             max_nodes, mask, mask_stride, scale, out, out_stride_n, out_stride_h, out_dtype, lse, &p);
+  if (rc != HALO_OK || N == 0) return rc;
+  const int dtype = pool->dtype, D = pool->D, H_kv = pool->H_kv;
   const TreeShape s = tree_shape(dtype, B, H, H_kv, D, (int64_t)W * pool->block_size, max_nodes);
   const size_t need = (size_t)s.partials * (size_t)tree_part_bytes(D);
   HALO_CHECK_ARG(need == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
@@ -1471,39 +1705,8 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
     set_error("workspace too small");
     return HALO_E_WORKSPACE;
   }
-  TreeParams p;
-  p.q = q;
-  p.q_stride_n = q_stride_n;
-  p.q_stride_h = q_stride_h;
-  p.k = static_cast<const char*>(pool->k);
-  p.v = static_cast<const char*>(pool->v);
-  p.sb = (uint32_t)(pool->stride_b / lanes);
-  p.sh = (uint32_t)(pool->stride_h / lanes);
-  p.sr = (uint32_t)(pool->stride_r / lanes);
-  p.blocks = pool->blocks;
-  p.bs = make_div(pool->block_size);
-  p.table = table;
-  p.table_stride = table_stride;
-  p.W = W;
-  p.lengths = lengths;
-  p.cu = cu_nodes;
-  p.mask = reinterpret_cast<const uint32_t*>(mask);
-  p.mask_stride = 2 * mask_stride;
-  p.B = B;
-  p.H = H;
-  p.H_kv = H_kv;
-  p.rep = H / H_kv;
-  p.N = N;
-  p.max_nodes = max_nodes;
   p.slots = s.slots;
   p.min_tiles = s.min_tiles;
-  p.scale2 = (float)((double)scale * 1.4426950408889634);
-  HALO_CHECK_ARG(p.scale2 >= 0x1p-126f && std::isfinite(p.scale2), "scale out of range");
-  p.out = out;
-  p.o_stride_n = out_stride_n;
-  p.o_stride_h = out_stride_h;
-  p.out_f32 = out_dtype == HALO_F32;
-  p.lse = lse;
   p.part_o = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * 32 * (D / 4));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1513,11 +1716,11 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
   do {                                                                                                             \
     hipLaunchKernelGGL((KERNEL), grid, block, 0, st, p);                                                           \
     if (s.merge && s.mw == 8)                                                                                      \
-      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 8>), mgrid, dim3(512), 0, st, p);                   \
+      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 8, false>), mgrid, dim3(512), 0, st, p);                   \
     else if (s.merge)                                                                                              \
-      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 4>), mgrid, dim3(256), 0, st, p);                   \
+      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 4, false>), mgrid, dim3(256), 0, st, p);                   \
   } while (0)
-#define HALO_TREE_WIDE(DTV, DV, NWV) HALO_TREE((tree_attn_wide_kernel<DTV, DV, NWV>), DV, DTV, kTreeWideKT, NWV)
+#define HALO_TREE_WIDE(DTV, DV, NWV) HALO_TREE((tree_attn_wide_kernel<DTV, DV, NWV, false>), DV, DTV, kTreeWideKT, NWV)
 #define HALO_TREE16(DTV, DV)                                                                     \
   do {                                                                                           \
     if (s.nw == 1) HALO_TREE((tree_attn_kernel<DTV, DV>), DV, DTV, kTreeKT, 1);                \
@@ -1526,8 +1729,8 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
     else HALO_TREE_WIDE(DTV, DV, 8);                                                             \
   } while (0)
   if (dtype == HALO_F32) {
-    if (D == 128) HALO_TREE((tree_attn_f32_kernel<128>), 128, HALO_F32, kTreeKT, 1);
-    else HALO_TREE((tree_attn_f32_kernel<64>), 64, HALO_F32, kTreeKT, 1);
+    if (D == 128) HALO_TREE((tree_attn_f32_kernel<128, false>), 128, HALO_F32, kTreeKT, 1);
+    else HALO_TREE((tree_attn_f32_kernel<64, false>), 64, HALO_F32, kTreeKT, 1);
   } else if (dtype == HALO_BF16) {
     if (D == 128) HALO_TREE16(HALO_BF16, 128);
     else HALO_TREE16(HALO_BF16, 64);
@@ -1538,6 +1741,102 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
 #undef HALO_TREE16
 #undef HALO_TREE_WIDE
 #undef HALO_TREE
+  HALO_CHECK_HIP(hipGetLastError());
+  return HALO_OK;
+}
+
+namespace {
+
+// How a call of chunks is cut: rows and keys of a tile, units, items and partials at most.
+struct ChunkShape {
+  int R, KT;
+  int64_t units, items, partials, cut_units;  // units: of one head; partials: of all heads
+};
+ChunkShape chunk_shape(int dtype, int B, int N, int H, int H_kv) {
+  ChunkShape s;
+  const bool f32 = dtype == HALO_F32;
+  s.R = f32 ? kTreeRows : 256;
+  s.KT = f32 ? kTreeKT : kTreeWideKT;
+  s.units = (int64_t)N * (H / H_kv) / s.R + B;
+  s.partials = f32 ? 2048 : 512;
+  if (s.partials < 2 * H_kv) s.partials = 0;
+  s.items = s.units + s.partials / H_kv;
+  s.cut_units = s.partials / 2 / H_kv < s.units ? s.partials / 2 / H_kv : s.units;
+  return s;
+}
+size_t chunk_bytes(const ChunkShape& s, int D) {
+  return (size_t)(s.partials * (s.R / 32) * tree_part_bytes(D) + s.items * kItemInts4 * 16 + (s.cut_units * 4 + 15) / 16 * 16 + 16);
+}
+// Up to this many rows the tree kernels, without a plan.
+constexpr int kChunkTreeRows = 512;
+
+}  // namespace
+
+extern "C" size_t halo_chunk_workspace_size(int dtype, int B, int N, int H, int H_kv, int D, int64_t max_keys, int max_rows) {
+  if (max_rows <= kChunkTreeRows) return halo_tree_workspace_size(dtype, B, H, H_kv, D, max_keys, max_rows);
+  if (N <= 0 || !tree_sizes_ok(B, H, H_kv, D, max_keys, 1)) return 0;
+  return chunk_bytes(chunk_shape(dtype, B, N, H, H_kv), D);
+}
+
+extern "C" int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int N,
+                               int H, const int32_t* table, int64_t table_stride, int B, int W, const int32_t* lengths,
+                               const int32_t* cu_rows, int max_rows, float scale, void* out, int64_t out_stride_n,
+                               int64_t out_stride_h, int out_dtype, float* lse, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  if (max_rows <= kChunkTreeRows)
+    return halo_tree_attn(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_rows, max_rows, nullptr,
+                          0, scale, out, out_stride_n, out_stride_h, out_dtype, lse, workspace, workspace_bytes, stream);
+  TreeParams p;
+  const int rc = tree_params(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_rows, max_rows, 1,
+                             nullptr, 0, scale, out, out_stride_n, out_stride_h, out_dtype, lse, &p);
+  if (rc != HALO_OK || N == 0) return rc;
+  const int dtype = pool->dtype, D = pool->D;
+  HALO_CHECK_ARG(B <= kChunkMaxB && (int64_t)N * p.rep < (1ll << 30), "need B <= 4096 and rows of all heads in 30 bits");
+  HALO_CHECK_ARG((int64_t)W * pool->block_size + N < (1ll << 31) - 1024, "positions in 31 bits");
+  const ChunkShape s = chunk_shape(dtype, B, N, H, p.H_kv);
+  // the units' number in 31 bits whatever cu_rows holds
+  HALO_CHECK_ARG((s.units + s.partials) * p.H_kv < (1ll << 31) && s.units * B < (1ll << 31), "too many rows and heads");
+  HALO_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace missing or not 16-byte aligned");
+  if (workspace_bytes < chunk_bytes(s, D)) {
+    set_error("workspace too small");
+    return HALO_E_WORKSPACE;
+  }
+  const int NW = s.R / 32;
+  p.part_o = reinterpret_cast<float4*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * NW * 32 * (D / 4));
+  ChunkPlanParams c;
+  c.items = reinterpret_cast<int4*>(p.part_ml + s.partials * NW * 32);
+  c.plan = reinterpret_cast<int32_t*>(c.items + s.items * kItemInts4);
+  c.cut_units = c.plan + 4;
+  c.R = s.R;
+  c.KT = s.KT;
+  c.min_tiles = dtype == HALO_F32 ? 2 * kTreeWaves : 4;
+  c.part_cap = (int)s.partials;
+  c.unit_cap = (int)s.units;
+  p.items = c.items;
+  p.plan = c.plan;
+  p.cut_units = c.cut_units;
+  c.t = p;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, c);
+  const dim3 grid((unsigned)(s.units * p.H_kv + s.partials)), mgrid((unsigned)(s.cut_units * p.H_kv * NW), D / 32);
+#define HALO_CHUNK(KERNEL, DV, DTV, KTV, NWV, THREADS)                                                             \
+  do {                                                                                                             \
+    hipLaunchKernelGGL((KERNEL), grid, dim3(THREADS), 0, st, p);                                                   \
+    if (s.cut_units > 0)                                                                                           \
+      hipLaunchKernelGGL((tree_merge_kernel<DV, DTV, KTV, NWV, 4, true>), mgrid, dim3(256), 0, st, p);             \
+  } while (0)
+  if (dtype == HALO_F32) {
+    if (D == 128) HALO_CHUNK((tree_attn_f32_kernel<128, true>), 128, HALO_F32, kTreeKT, 1, 256);
+    else HALO_CHUNK((tree_attn_f32_kernel<64, true>), 64, HALO_F32, kTreeKT, 1, 256);
+  } else if (dtype == HALO_BF16) {
+    if (D == 128) HALO_CHUNK((tree_attn_wide_kernel<HALO_BF16, 128, 8, true>), 128, HALO_BF16, kTreeWideKT, 8, 512);
+    else HALO_CHUNK((tree_attn_wide_kernel<HALO_BF16, 64, 8, true>), 64, HALO_BF16, kTreeWideKT, 8, 512);
+  } else {
+    if (D == 128) HALO_CHUNK((tree_attn_wide_kernel<HALO_F16, 128, 8, true>), 128, HALO_F16, kTreeWideKT, 8, 512);
+    else HALO_CHUNK((tree_attn_wide_kernel<HALO_F16, 64, 8, true>), 64, HALO_F16, kTreeWideKT, 8, 512);
+  }
+#undef HALO_CHUNK
   HALO_CHECK_HIP(hipGetLastError());
   return HALO_OK;
 }

@@ -1,4 +1,4 @@
-"""Attention of drafted token trees over a paged cache.
+"""Attention of drafted token trees, and of prompts, over a paged cache.
 
 ``tree_attention`` verifies the drafted tokens of a batch in one call: every
 node attends its request's committed rows and, of the tree's own rows behind
@@ -6,8 +6,8 @@ them, itself and its ancestors.  K and V lie in the blocks of a pool
 (``halo_amd.block_pool``), so the requests' lengths and trees may differ freely
 and change from call to call without a host plan: the lengths are read on the
 device, and a captured call follows them.  With one node a request it is a
-paged decode step; without masks, a causal block of new rows (a prompt's slice
-of up to 512 rows).
+paged decode step; without masks, a causal block of new rows.
+``chunk_attention`` is the causal form for prompts, with any number of rows.
 
 The reference attends a chunk list with one row or one causal block a call
 (halo/kv_cache_chunked.py:571-964); it has no drafted trees.
@@ -46,8 +46,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     q.dtype), and with ``return_lse`` lse (N, H) fp32, both in ``out`` and ``lse``
     if given; rows of no request keep what they hold there.  The softmax and all
     sums are fp32; for 16-bit pools its weights are rounded once to the pool's
-    type (fp16 weights below 2^-21 of the largest are off by at most 2^-32 of it;
-    fp16 scores beyond 2^29 are not covered).  Equal calls give equal bits; where
+    type (fp16 weights below 2^-21 of the largest are off by at most 2^-32 of it, where
+    scores reach 2^24 2^-29; beyond 2^24 fp16 results are finite up to 2^29, but
+    their accuracy is not covered).  Equal calls give equal bits; where
     a request's rows are cut, and so its last bits, goes by all the requests of
     the call.  No gradient is kept."""
     if pool_calls.calls is not None and stream is None and out_dtype is None:
@@ -55,6 +56,37 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
                                             out, lse, return_lse)
         if r is not None:
             return pool_calls.called(r, "halo_tree_attn")
+    nat.lib()
+    if not 1 <= max_nodes <= MAX_NODES:
+        raise AssertionError(f"max_nodes must be in [1, {MAX_NODES}], got {max_nodes}")
+    return _attend(q, k_pool, v_pool, block_table, lengths, cu_nodes, "cu_nodes", max_nodes, mask, False, scale, out,
+                   out_dtype, lse, return_lse, stream)
+
+
+def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                    lengths: torch.Tensor, cu_rows: torch.Tensor, *, max_rows: int, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                    lse: Optional[torch.Tensor] = None, return_lse: bool = False, stream=None):
+    """Attention of prompts, or slices of them, over the blocks they have been
+    written to: q (N, H, D), pools, ``block_table``, ``lengths`` and the results
+    as in ``tree_attention``.
+
+    Row i of request b is row ``cu_rows[b] + i`` (``cu_rows`` (B + 1) int32) and
+    attends the rows ``[0, lengths[b] + i]``: what the request held before, the
+    new rows before it and itself, all of them in the pool already
+    (``append_rows``, ``rotate_rows``).  Requests may have any numbers of new
+    rows, none and one among them; ``max_rows`` is the largest (further rows are
+    left out).  The lengths are read on the device, so a captured call follows
+    them.  Above 512 rows at most 4096 requests; N times H / H_kv stays below
+    2^30."""
+    if max_rows < 1:
+        raise AssertionError(f"max_rows must be at least 1, got {max_rows}")
+    return _attend(q, k_pool, v_pool, block_table, lengths, cu_rows, "cu_rows", max_rows, None, True, scale, out, out_dtype,
+                   lse, return_lse, stream)
+
+
+def _attend(q, k_pool, v_pool, block_table, lengths, cu, cu_name, max_nodes, mask, chunk, scale, out, out_dtype, lse,
+            return_lse, stream):
     L = nat.lib()
     if q.dim() != 3:
         raise AssertionError(f"q must be (N, H, D), got {tuple(q.shape)}")
@@ -69,14 +101,12 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         raise AssertionError(f"head_dim must be 64 or 128, got {D}")
     if H == 0 or H % shape[1]:
         raise AssertionError(f"head count mismatch: q has {H}, kv has {shape[1]}")
-    if not 1 <= max_nodes <= MAX_NODES:
-        raise AssertionError(f"max_nodes must be in [1, {MAX_NODES}], got {max_nodes}")
     B = lengths.numel()
     if B < 1:
         raise AssertionError("no requests")
     check_table(block_table, B, dev)
     check_ints(lengths, "lengths", (B,), dev)
-    check_ints(cu_nodes, "cu_nodes", (B + 1,), dev)
+    check_ints(cu, cu_name, (B + 1,), dev)
     words = 0
     if mask is not None:
         if mask.dtype != torch.int64 or mask.device != dev or mask.dim() != 2 or mask.shape[0] != N \
@@ -120,13 +150,21 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         if return_lse and lse is None:
             lse = torch.empty((N, H), device=dev, dtype=torch.float32)
         W = block_table.shape[1]
-        nbytes = L.halo_tree_workspace_size(nat.dtype_code(q.dtype), B, H, shape[1], D, W * shape[2], max_nodes)
+        dt = nat.dtype_code(q.dtype)
+        if chunk:
+            nbytes = L.halo_chunk_workspace_size(dt, B, N, H, shape[1], D, W * shape[2], max_nodes)
+        else:
+            nbytes = L.halo_tree_workspace_size(dt, B, H, shape[1], D, W * shape[2], max_nodes)
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
         os_ = o.stride()
-        nat.check(L.halo_tree_attn(
-            pool, q.data_ptr(), qs[0], qs[1], N, H, block_table.data_ptr(), block_table.stride(0) if B > 1 else W, B, W,
-            lengths.data_ptr(), cu_nodes.data_ptr(), max_nodes, nat.ptr(mask), words, scale, o.data_ptr(), os_[0],
-            os_[1], nat.dtype_code(o.dtype), nat.ptr(lse), nat.ptr(ws), nbytes, nat.stream_ptr()), "halo_tree_attn")
+        head = (pool, q.data_ptr(), qs[0], qs[1], N, H, block_table.data_ptr(), block_table.stride(0) if B > 1 else W, B, W,
+                lengths.data_ptr(), cu.data_ptr(), max_nodes)
+        tail = (scale, o.data_ptr(), os_[0], os_[1], nat.dtype_code(o.dtype), nat.ptr(lse), nat.ptr(ws), nbytes,
+                nat.stream_ptr())
+        if chunk:
+            nat.check(L.halo_chunk_attn(*head, *tail), "halo_chunk_attn")
+        else:
+            nat.check(L.halo_tree_attn(*head, nat.ptr(mask), words, *tail), "halo_tree_attn")
         if out is None:
             out = o if o.dtype == want else o.to(want)
         elif o is not out:

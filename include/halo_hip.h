@@ -607,6 +607,111 @@ int halo_commit_path(const halo_block_pool* pool, const int32_t* table, int64_t 
                      const int32_t* lengths, const int32_t* path, int64_t path_stride, int n_path_max,
                      const int32_t* n_path, int32_t* new_lengths, void* stream);
 
+/*
+ * Attention of chunks of new rows over a paged cache: row i of request b is
+ * row cu_rows[b] + i of q, out and lse and attends the request's rows
+ * [0, lengths[b] + i]; everything else as in halo_tree_attn without masks, but
+ * a request may have any number of rows, max_rows of them at most (further
+ * ones are left out).  N * H / H_kv and W * block_size + N in 30 and 31 bits;
+ * above 512 rows B <= 4096.  workspace: at least
+ * halo_chunk_workspace_size(max_keys = W * block_size) bytes.
+ */
+size_t halo_chunk_workspace_size(int dtype, int B, int N, int H, int H_kv, int D, int64_t max_keys, int max_rows);
+int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int N, int H,
+                    const int32_t* table, int64_t table_stride, int B, int W, const int32_t* lengths,
+                    const int32_t* cu_rows, int max_rows, float scale, void* out, int64_t out_stride_n,
+                    int64_t out_stride_h, int out_dtype, float* lse, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/*
+ * Rows on their way into the pool: heads of q (N, H, D) and k (N, H_kv, D)
+ * normed (y = x w / sqrt(mean(x^2) + eps), weights q_norm and k_norm of D
+ * elements, fp32 where *_norm_f32, else of the pool's type; NULL: no norm) and
+ * rotated in their first R channels (16 <= R <= D, R % 16 == 0) by the cosines
+ * and sines of row positions[i] (int64 where pos64, else int32) of cos and sin
+ * (trig_rows, R/2 fp32, rows trig_stride apart): pairs (j, j + R/2), or
+ * (2j, 2j + 1) where interleaved.  q goes to out (N, H, D), k and v (N, H_kv, D)
+ * to slot slots[i] of the pool (one layer, D 64 or 128); rows whose slot is
+ * outside the pool are not kept.  A position outside the table makes the
+ * rotated channels NaN.  fp32 throughout, rounded once.  All rows 16-byte
+ * aligned, strides in elements.  out may be q.  Slots must differ.
+ */
+int halo_rotate_rows(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int H,
+                     const void* k, int64_t k_stride_n, int64_t k_stride_h, const void* v, int64_t v_stride_n,
+                     int64_t v_stride_h, void* out, int64_t out_stride_n, int64_t out_stride_h, int N,
+                     const void* positions, int pos64, const float* cos, const float* sin, int64_t trig_stride,
+                     int64_t trig_rows, int R, int interleaved, const void* q_norm, int q_norm_f32,
+                     const void* k_norm, int k_norm_f32, float eps, const int64_t* slots, void* stream);
+
+/*
+ * Requests that go on with other requests' blocks.  Row b of the table becomes
+ * what row a = source[b] was (a outside [0, B): b gives its blocks up), with
+ * len = min(lengths[a], n_blocks[a] * block_size):
+ *   - a's heir (a itself if source[a] = a, else the lowest b with source[b] =
+ *     a) has all n_blocks[a] blocks;
+ *   - the others share the len / block_size full ones, and where rows are left
+ *     get a block of their own with copies of these (all layers).
+ * Blocks that no row has any more are pushed on the free list in the order of
+ * their ids; then the copies' blocks are popped in the order of b.  shared[x]
+ * (one entry a block of the pool) counts the rows that have block x beyond the
+ * first; blocks handed out by halo_update_block_tables have 0.  Entries behind
+ * a row's blocks become -1 unless source[b] = b; new_lengths[b] = len, 0 for
+ * rows given up.  If the free list does not cover the copies nothing changes,
+ * ok = 0 and new_lengths = lengths.  ids pushed past n_cap are dropped; B <=
+ * 4096.  A row's blocks differ, and shared ones are full for every row that has
+ * them.  workspace: halo_fork_workspace_size bytes, 16-byte aligned.
+ */
+size_t halo_fork_workspace_size(int B, int W, int blocks);
+int halo_fork_blocks(const halo_block_pool* pool, int32_t* table, int64_t table_stride, int32_t* n_blocks, int B, int W,
+                     int32_t* free_blocks, int n_cap, int32_t* n_free, int32_t* shared, const int32_t* lengths,
+                     const int32_t* source, int32_t* new_lengths, uint8_t* ok, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * The used blocks of a pool moved to its front.  Of the blocks in the rows of
+ * the table (the first n_blocks[b] entries) and in the free list, in the order
+ * of their ids, the first n_used are used ones afterwards: the i-th used block
+ * behind them moves, all layers, into the i-th free one among them.  Table,
+ * shared and the free list (the lowest id on top) are changed to match,
+ * new_id[x] (one entry a block) is where block x went or x.  Other blocks stay
+ * as they are.  workspace: halo_compact_workspace_size bytes, 16-byte aligned.
+ */
+size_t halo_compact_workspace_size(int blocks);
+int halo_compact_blocks(const halo_block_pool* pool, int32_t* table, int64_t table_stride, const int32_t* n_blocks,
+                        int B, int W, int32_t* free_blocks, int n_cap, int32_t* n_free, int32_t* shared,
+                        int32_t* new_id, int32_t* n_used, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Drafted trees against a target's probabilities.  Nodes and parents as in
+ * halo_tree_layout; node 0 of a request is its last sampled token, tokens[i]
+ * the drafted token of node i, row i of probs (N, V, rows probs_stride apart)
+ * the target's probabilities behind node i and row i of draft_probs (or NULL)
+ * those its children were drawn from; accept (N) and sample (B) random numbers
+ * in [0, 1).  From node 0, with p and q the rows of the node reached, S = 0,
+ * Z = 1, Q = 0, its children are tried in the order of their numbers.  A child
+ * with token t and r = max(p[t] - S q[t], 0), 0 if t was rejected here, is
+ *   accepted iff accept u: u q[t] Z / (1 - Q) < r           (Q: see below),
+ *   else t is rejected here, S += Z / (1 - Q) and Z = the sum over the tokens
+ *   not rejected here of max(p - S q, 0);
+ * with replacement Q stays 0, else Q += q[t], and a child whose token was
+ * rejected here, or behind Q >= 1, is passed over.  Without draft_probs q[t] =
+ * 1, r = p[t], Z -= p[t] on rejection, and repeated tokens are passed over.
+ * Tokens outside [0, V) are passed over.  An accepted child is the next node.
+ * Where no child is accepted, or the path has max_path (<= 64) nodes, token =
+ * the first v at which the running sum of max(p - S q, 0) over the tokens not
+ * rejected here exceeds sample times its whole; of p, where that is 0.
+ * path (B, max_path): the nodes, then -1; n_path (B) how many.  A request
+ * without nodes has n_path 0 and token -1.  NaN and negative probabilities
+ * count as 0.  Products and sums in 64 bits.  V <= 2^24, max_nodes <= 512.
+ * workspace: halo_verify_workspace_size bytes, 16-byte aligned.
+ */
+size_t halo_verify_workspace_size(int B, int V);
+int halo_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* cu_nodes, int B, int N, int max_nodes,
+                     int V, int dtype, const void* probs, int64_t probs_stride, const void* draft_probs,
+                     int64_t draft_stride, int replacement, const float* accept, const float* sample, int max_path,
+                     int32_t* path, int32_t* n_path, int64_t* token, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 /* ---- tier block moves -------------------------------------------------- */
 
 /*

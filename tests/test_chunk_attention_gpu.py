@@ -1,0 +1,267 @@
+"""Chunks attended over a paged cache on the GPU, against the definition in
+float64 (tree_launch.Batch without masks).
+
+Tolerances as in test_tree_pipeline_gpu.py, with u = 2^-24, A the weighted mean
+of |v|, d the largest scale * sum |q_d k_d|, T the attended rows:
+  |out - exact| <= A (2 (D + 6) u d + (2 T + 8) u + w) + f + r |out| (1 + w)
+  |lse - exact| <= (D + 6) u d + (T + 8) u + 4 u |lse|"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import tree_launch
+from test_tree_pipeline_gpu import BF16, F16, F32, HALF, U, check
+
+pytestmark = pytest.mark.gpu
+DT = [BF16, F16, F32]
+
+
+class Batch(tree_launch.Batch):
+    def __init__(self, dev, **kw):
+        super().__init__(dev, **{**dict(H=8, Hk=2, D=64, bs=16, dtype=BF16, seed=0, blocks=200), **kw}, masks=False)
+
+    def exact(self, only=None):
+        return super().exact([b for b, n in enumerate(self.nodes) if n] if only is None else only)
+
+    def run(self, **kw):
+        import halo_amd
+        a = dict(self.args)
+        a.pop("mask")
+        a["cu_rows"] = a.pop("cu_nodes")
+        return halo_amd.chunk_attention(**{**a, **dict(max_rows=self.max_nodes, return_lse=True), **kw})
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ctx,rows", [(0, 1), (5, 1), (0, 64), (100, 511), (3, 512), (0, 513), (1, 514), (63, 577), (64, 1023),
+                                      (700, 640), (31, 1025)])
+def test_one_request(dev, ctx, rows, D, dtype):
+    b = Batch(dev, lengths=[ctx], nodes=[rows], D=D, dtype=dtype, seed=rows)
+    check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,Hk", [(1, 1), (8, 8), (28, 4), (32, 8), (6, 2), (40, 1), (24, 1)])
+def test_head_layouts(dev, dtype, H, Hk):
+    b = Batch(dev, lengths=[37, 0, 300], nodes=[600, 1, 77], H=H, Hk=Hk, D=128, dtype=dtype, seed=H)
+    check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("holes", [0.0, 0.06])
+@pytest.mark.parametrize("bs", [1, 3, 16, 24, 100, 256])
+def test_blocks_of_any_size_and_blocks_that_are_not_there(dev, bs, holes, dtype):
+    b = Batch(dev, lengths=[1500, 0, 64], nodes=[530, 700, 2], bs=bs, holes=holes, dtype=dtype, seed=bs)
+    check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_ragged_batches(dev, dtype):
+    """Empty requests, single rows behind long contexts, and prompts from nothing."""
+    lengths = [0, 4000, 17, 0, 900, 2500, 0, 1, 64, 0]
+    rows = [1200, 1, 0, 513, 64, 2, 0, 33, 640, 1]
+    for H, Hk, D in ((8, 2, 64), (28, 4, 128)):
+        b = Batch(dev, lengths=lengths, nodes=rows, H=H, Hk=Hk, D=D, dtype=dtype, seed=H)
+        check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_contexts_cut_into_many_parts(dev, dtype):
+    b = Batch(dev, lengths=[30000], nodes=[520], H=4, Hk=1, D=128, dtype=dtype, seed=3)
+    check(b, *b.run(), b.exact())
+    b = Batch(dev, lengths=[20000, 100], nodes=[513, 900], H=8, Hk=2, D=64, dtype=dtype, seed=4)
+    check(b, *b.run(), b.exact())
+
+
+def test_a_long_prompt(dev):
+    b = Batch(dev, lengths=[0], nodes=[5000], H=4, Hk=1, D=128, dtype=BF16, seed=5)
+    check(b, *b.run(), b.exact())
+    b = Batch(dev, lengths=[11], nodes=[3001], H=2, Hk=2, D=64, dtype=F32, seed=5)
+    check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("B", [65, 700, 4096])
+def test_many_requests(dev, B):
+    rows = [513 if b == 40 else (b * 7) % 4 for b in range(B)]
+    b = Batch(dev, lengths=[(b * 13) % 90 for b in range(B)], nodes=rows, H=4, Hk=2, dtype=BF16, seed=B)
+    check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_up_to_512_rows_it_is_the_causal_tree(dev, dtype):
+    b = Batch(dev, lengths=[300, 0, 1000], nodes=[40, 512, 1], dtype=dtype)
+    got, want = b.run(), tree_launch.Batch.run(b)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_rows_that_are_not_seen_have_no_part(dev, dtype, value):
+    """K and V behind a row, behind the request, and of blocks that no request has hold NaN or infinities."""
+    ctx, n, bs, Hk, D = 70, 600, 16, 2, 64
+    b = Batch(dev, lengths=[ctx], nodes=[n], dtype=dtype, seed=8)
+    a = b.args
+    a["block_table"][0] = torch.arange(b.W, device=dev)
+    exact = b.exact()
+    want = b.run()
+    at = ctx + 333
+    bounds = Batch(dev, lengths=[ctx], nodes=[n], dtype=dtype, seed=8)  # the values as they were
+    for p in (a["k_pool"], a["v_pool"]):
+        p[b.W:] = value
+        p[-(-(ctx + n) // bs):] = value
+        p[(ctx + n - 1) // bs, :, (ctx + n - 1) % bs + 1:] = value
+    got = b.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    a["v_pool"][at // bs, :, at % bs, 5] = value  # a value that the rows from 333 on see
+    out, lse = b.run()
+    assert torch.equal(lse, want[1])
+    keep = torch.ones(D, dtype=torch.bool, device=dev)
+    keep[5] = False
+    check(bounds, torch.where(torch.isfinite(out), out, want[0]), lse, exact)
+    assert torch.equal(torch.isfinite(out)[..., 5], (torch.arange(n, device=dev) < 333)[:, None].expand(n, b.H))
+    assert bool(torch.isfinite(out[..., keep]).all())
+    a["k_pool"][at // bs, :, at % bs] = value  # and a key
+    out, lse = b.run()
+    assert bool(torch.isfinite(out[:333]).all()) and bool(torch.isfinite(lse[:333]).all())
+    check(bounds, torch.where((torch.arange(n, device=dev) < 333)[:, None, None], out, want[0]),
+          torch.where((torch.arange(n, device=dev) < 333)[:, None], lse, want[1]), exact)
+
+
+def test_requests_without_any_row_there(dev):
+    b = Batch(dev, lengths=[40, 10], nodes=[600, 20])
+    b.args["block_table"][0] = -1
+    out, lse = b.run()
+    assert not bool(out[:600].any()) and bool((lse[:600] == -float("inf")).all())
+    assert bool(torch.isfinite(lse[600:]).all())
+
+
+def test_rows_behind_the_table(dev):
+    """Lengths and rows past the table's columns are not attended and nothing is read there."""
+    b = Batch(dev, lengths=[100], nodes=[600])
+    a = b.args
+    a["block_table"] = a["block_table"][:, :20].contiguous()
+    out, lse = b.run()
+    full = Batch(dev, lengths=[100], nodes=[600])
+    want = full.run()
+    assert torch.equal(out[:220], want[0][:220]) and torch.equal(lse[:220], want[1][:220])
+    a["lengths"].fill_(2 ** 30)
+    out, lse = b.run()
+    assert bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("out_dtype", DT)
+@pytest.mark.parametrize("form", ["plain", "odd start", "odd rows"])
+def test_rows_of_no_request_keep_what_they_hold(dev, dtype, out_dtype, form):
+    b = Batch(dev, lengths=[300, 20], nodes=[600, 3], dtype=dtype, seed=6)
+    want = b.run()
+    N = 607
+    q = torch.cat([b.args["q"], b.args["q"][:4]])
+    shape, cut = {"plain": ((N, 8, 64), slice(None)), "odd start": ((N, 8, 66), slice(1, 65)), "odd rows": ((N, 8, 65), slice(0, 64))}[form]
+    held = (torch.arange(N * 8 * shape[2], device=dev, dtype=torch.float32).view(shape) % 251 - 125).to(out_dtype)
+    out = held.clone()[..., cut]
+    lse = torch.full((N, 8), 7.0, device=dev)
+    got = b.run(q=q, out=out, lse=lse)
+    assert got[0] is out and got[1] is lse
+    assert torch.equal(out[603:], held[603:, :, cut]) and bool((lse[603:] == 7).all())
+    full = b.run(out_dtype=F32)[0]
+    # where a request is cut goes by the call's room for rows too, and so do its last bits
+    tol = (HALF[out_dtype] + HALF[dtype]) * 2 * full.abs() + 1e-3 * (dtype != F32) + 1e-5
+    assert bool(((out[:603].float() - full).abs() <= tol).all()) and torch.equal(full.to(dtype), want[0])
+    # rows past max_rows are left out as well
+    out = held.clone()[..., cut]
+    b.run(q=q, out=out, lse=lse, max_rows=550)
+    assert torch.equal(out[550:600], held[550:600, :, cut])
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_strides(dev, dtype):
+    b = Batch(dev, lengths=[77, 0], nodes=[520, 9], dtype=dtype, seed=7)
+    want = b.run()
+    a = b.args
+    q = a["q"]
+    for form in (q.transpose(0, 1).contiguous().transpose(0, 1), torch.cat([q, q], 2)[..., :64], torch.cat([q, q], 2)[..., 1:65].clone(),
+                 torch.nn.functional.pad(q, (1, 0))[..., 1:]):
+        if form.shape == q.shape and torch.equal(form, q):
+            got = b.run(q=form)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    pools = [p.transpose(1, 2).contiguous().transpose(1, 2) for p in (a["k_pool"], a["v_pool"])]
+    table = torch.nn.functional.pad(a["block_table"], (0, 5), value=-1)[:, :b.W]
+    got = b.run(k_pool=pools[0], v_pool=pools[1], block_table=table)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_scales(dev):
+    b = Batch(dev, lengths=[10], nodes=[520], dtype=F32, seed=9)
+    got = b.run(scale=0.5)
+    b.args["q"] = b.args["q"] * (0.5 * 8.0)  # the default is 1 / 8
+    want = b.run()
+    assert float((got[0] - want[0]).abs().max()) < 1e-5
+
+
+def test_replays_follow_the_lengths(dev):
+    """One graph, batches of other lengths and rows; eager calls between the replays."""
+    b = Batch(dev, lengths=[1000, 50, 3], nodes=[600, 40, 13], seed=10, blocks=100)
+    a = b.args
+    b.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = b.run()
+    N = sum(b.nodes)
+    for lengths, rows in (([1000, 50, 3], [600, 40, 13]), ([0, 500, 20], [1, 600, 52]), ([900, 0, 0], [0, 650, 3]),
+                          ([1, 2, 3], [217, 217, 219])):
+        b.lengths, b.nodes = lengths, rows
+        rows = [min(r, 600) for r in rows]
+        a["lengths"].copy_(torch.tensor(lengths))
+        at = [0]
+        for r in b.nodes:
+            at.append(at[-1] + r)
+        a["cu_nodes"].copy_(torch.tensor(at))
+        out.fill_(5)
+        graph.replay()
+        eager = b.run()
+        exact = b.exact()
+        live = torch.cat([torch.arange(r, device=dev) < 600 for r in b.nodes])
+        assert N == live.numel()
+        assert torch.equal(out[live], eager[0][live]) and torch.equal(lse[live], eager[1][live])
+        ref = [x[live] for x in exact]
+        check(b, out[live], lse[live], ref)
+
+
+def test_two_streams(dev):
+    b1 = Batch(dev, lengths=[2000], nodes=[600], seed=1)
+    b2 = Batch(dev, lengths=[30, 700], nodes=[700, 20], seed=2, dtype=F16)
+    want = [b1.run(), b2.run()]
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = [b.run(stream=x) for b, x in zip((b1, b2), s)]
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+def test_cu_rows_that_fall_or_pass_the_rows(dev):
+    """Whatever cu_rows holds, no other memory is read or written: rows of more than one request get either's output."""
+    b = Batch(dev, lengths=[10, 20, 30, 40], nodes=[600, 5, 600, 5])
+    for cu in ([0, 1210, 0, 1210, 5000], [0, 600, 300, 1210, 1210], [-7, 2 ** 30, -2 ** 31, 2 ** 31 - 1, 0], [1210, 5, 4, 3, 2]):
+        b.args["cu_nodes"].copy_(torch.tensor(cu))
+        for most in (600, 300):
+            out, lse = b.run(out=torch.zeros_like(b.args["q"]), max_rows=most)
+            assert bool(torch.isfinite(out).all())
+
+
+def test_huge_scores(dev):
+    """The largest scores are about 5.2 standard deviations of 8 x 2^26 x scale.  fp16 is covered up to 2^24: from exponents of
+    2^28 (steps of 32) the largest weight, rounded to a step of 2^7, may lie below 2^-14, where fp16 values lose bits."""
+    for dtype in DT:
+        b = Batch(dev, lengths=[700], nodes=[600], seed=3, dtype=dtype)
+        for t in (b.args["q"], b.args["k_pool"]):
+            t.mul_(2.0 ** 13).clamp_(-60000, 60000)
+        b.args["v_pool"].abs_()
+        out, lse = b.run(scale=2.0 ** (-8 if dtype == F16 else -3))
+        top = float(b.args["v_pool"].max()) * (1 + 2 * HALF[dtype]) * (1 + 8000 * U)
+        assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+        assert float(out.min()) >= 0 and float(out.max()) <= top
