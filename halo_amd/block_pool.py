@@ -71,9 +71,10 @@ def load_calls(path=None):
         spec = importlib.util.spec_from_file_location("_halo_poolcalls", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        mod.bind(*[ctypes.cast(getattr(nat.lib(), "halo_" + n), ctypes.c_void_p).value for n in
-                   ("update_block_tables", "append_rows", "tree_layout", "tree_workspace_size", "tree_attn",
-                    "commit_path")])
+        mod.bind([ctypes.cast(getattr(nat.lib(), "halo_" + n), ctypes.c_void_p).value for n in
+                  ("update_block_tables", "append_rows", "tree_layout", "tree_workspace_size", "tree_attn", "commit_path",
+                   "chunk_workspace_size", "chunk_attn", "verify_workspace_size", "verify_tree", "rotate_rows",
+                   "fork_workspace_size", "fork_blocks", "compact_workspace_size", "compact_blocks")])
         return mod
     except (ImportError, OSError, AttributeError):
         # built against another torch, or not a loadable module: the calls are made in Python (same results, slower)
@@ -359,6 +360,10 @@ def fork_blocks(block_table: torch.Tensor, n_blocks: torch.Tensor, free_blocks: 
     A request that shares blocks is given up here, not by a length of 0 in
     ``update_block_tables``, which knows no ``shared``: there its length may grow
     and fall, but not below the rows of its shared blocks.  B <= 4096."""
+    if calls is not None and stream is None:
+        r = calls.fork_blocks(block_table, n_blocks, free_blocks, n_free, shared, lengths, source, k_pool, v_pool)
+        if r is not None:
+            return called(r, "halo_fork_blocks")
     L = nat.lib()
     pool = pack_pool(k_pool, v_pool, written=True)
     dev = k_pool.device
@@ -393,6 +398,10 @@ def compact_blocks(block_table: torch.Tensor, n_blocks: torch.Tensor, free_block
     ``shared`` (see ``fork_blocks``; zeros where no blocks are shared) are changed
     in place.  Returns ``new_id`` (blocks) int32, where each block is now, for
     what else names blocks (slots not written yet), and ``n_used`` (1) int32."""
+    if calls is not None and stream is None:
+        r = calls.compact_blocks(block_table, n_blocks, free_blocks, n_free, shared, k_pool, v_pool)
+        if r is not None:
+            return called(r, "halo_compact_blocks")
     L = nat.lib()
     pool = pack_pool(k_pool, v_pool, written=True)
     dev = k_pool.device

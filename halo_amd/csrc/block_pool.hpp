@@ -36,6 +36,10 @@ __device__ __forceinline__ int64_t dpp_or_zero(int64_t v) {
   const uint32_t lo = (uint32_t)dpp_or_zero<CTRL, ROWS>((int)(uint32_t)v);
   return (int64_t)(((uint64_t)(uint32_t)dpp_or_zero<CTRL, ROWS>((int)(v >> 32)) << 32) | lo);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  return __builtin_bit_cast(double, dpp_or_zero<CTRL, ROWS>(__builtin_bit_cast(int64_t, v)));
+}
 template <typename T>
 __device__ __forceinline__ T wave_prefix(T v) {
   v += dpp_or_zero<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
@@ -55,6 +59,9 @@ __device__ __forceinline__ float lane_of(float v, int lane) {
 __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(int64_t, v), lane));
 }
 
 // A pool as the kernels address it.

@@ -23,8 +23,7 @@ struct RotateParams {
   const char* v;
   char* out;
   int64_t qsn, qsh, ksn, ksh, vsn, vsh, osn, osh;  // strides in bytes
-  int H, H_kv, N, parts;
-  Div per_row;  // parts
+  int H, H_kv, N;
   const void* positions;
   int pos64;
   const float* cos;
@@ -41,19 +40,20 @@ struct RotateParams {
 
 constexpr int kRotThreads = 256;
 
-template <int DT>
-__device__ __forceinline__ void load8(const char* p, float* f) {
-  if constexpr (DT == HALO_F32) {
-    unpack16<DT>(*reinterpret_cast<const uint4*>(p), f);
-    unpack16<DT>(*reinterpret_cast<const uint4*>(p + 16), f + 4);
-  } else {
-    unpack16<DT>(*reinterpret_cast<const uint4*>(p), f);
-  }
-}
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
 template <int DT>
 __device__ __forceinline__ void store8(char* p, const float* f) {
-  store_elem4(p, 0, DT, f);
-  store_elem4(p, 4, DT, f + 4);
+  if constexpr (DT == HALO_F32) {
+    store_elem4(p, 0, DT, f);
+    store_elem4(p, 4, DT, f + 4);
+  } else {
+    auto two = [](float x, float y) {
+      return DT == HALO_BF16 ? (uint32_t)f32_to_bf16_rne(x) | (uint32_t)f32_to_bf16_rne(y) << 16
+                             : (uint32_t)f32_to_f16_rne(x) | (uint32_t)f32_to_f16_rne(y) << 16;
+    };
+    *reinterpret_cast<uint4*>(p) = make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7]));
+  }
 }
 
 // Sum over the G = 4 or 8 lanes of a head.
@@ -65,24 +65,30 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-template <int DT, int D>
+// A wave takes a row: its position and slot are the same for all lanes, the
+// cosines and sines are loaded once, and the row's heads go through in batches
+// of UB for each group of lanes, whose loads are in flight together.
+template <int DT, int D, int UB>
 __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P) {
-  constexpr int G = D / 16;  // lanes of a head
-  constexpr int ES = DT == HALO_F32 ? 4 : 2;
-  const int lane = threadIdx.x & (G - 1);
-  const int unit = blockIdx.x * (kRotThreads / G) + threadIdx.x / G;
-  const int n = div_by(unit, P.per_row);
+  constexpr int G = D / 16, HEADS = 64 / G;  // lanes of a head, heads side by side
+  constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = ES / 2;
+  const int n = blockIdx.x * (kRotThreads / 64) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (n >= P.N) return;
-  const int part = unit - n * P.parts;
+  const int lane = threadIdx.x & (G - 1), group = (threadIdx.x & 63) / G;
   const int R = P.R, heads = P.H + 2 * P.H_kv;
-  const bool halves = !P.interleaved && 16 * lane < R;
+  const bool turns = 16 * lane < R, halves = turns && !P.interleaved;
   const int ca = halves ? 8 * lane : 16 * lane, cb = halves ? R / 2 + 8 * lane : 16 * lane + 8;
-
+  const int64_t slot = P.slots[n];
+  const bool kept = slot >= 0 && slot < (int64_t)P.pool.blocks * P.pool.bs.d;
+  const int blk = kept ? div_by((int)slot, P.pool.bs) : 0;
+  const int64_t place = blk * P.pool.sb + (slot - (int64_t)blk * P.pool.bs.d) * P.pool.sr;
+  int64_t pos = P.pos64 ? reinterpret_cast<const int64_t*>(P.positions)[n] : reinterpret_cast<const int32_t*>(P.positions)[n];
+  const bool there = pos >= 0 && pos < P.trig_rows;
+  pos = there ? pos : 0;
   float c[8], s[8];
-  if (16 * lane < R) {
-    int64_t pos = P.pos64 ? reinterpret_cast<const int64_t*>(P.positions)[n] : reinterpret_cast<const int32_t*>(P.positions)[n];
-    const bool there = pos >= 0 && pos < P.trig_rows;
-    pos = there ? pos : 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+  if (turns) {
     const float* cr = P.cos + pos * P.trig_stride + 8 * lane;
     const float* sr = P.sin + pos * P.trig_stride + 8 * lane;
 #pragma unroll
@@ -90,60 +96,76 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
       c[i] = there ? cr[i] : __uint_as_float(0x7fc00000u);
       s[i] = sr[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
   }
-  const int64_t slot = P.slots[n];
-  const bool kept = slot >= 0 && slot < (int64_t)P.pool.blocks * P.pool.bs.d;
-  const int blk = kept ? div_by((int)slot, P.pool.bs) : 0;
-  const int64_t place = blk * P.pool.sb + (slot - (int64_t)blk * P.pool.bs.d) * P.pool.sr;
 
-  for (int h = part; h < heads; h += P.parts) {
-    const bool is_q = h < P.H, is_v = h >= P.H + P.H_kv;
-    if (!is_q && !kept) continue;
-    const int hk = h - P.H - (is_v ? P.H_kv : 0);
-    const char* src = is_q ? P.q + n * P.qsn + h * P.qsh : is_v ? P.v + n * P.vsn + hk * P.vsh : P.k + n * P.ksn + hk * P.ksh;
-    char* dst = is_q ? P.out + n * P.osn + h * P.osh : (is_v ? P.pool.v : P.pool.k) + place + hk * P.pool.sh;
-    float a[8], b[8];
-    load8<DT>(src + ca * ES, a);
-    load8<DT>(src + cb * ES, b);
-    if (!is_v) {
-      const void* w = is_q ? P.q_norm : P.k_norm;
-      if (w != nullptr) {
-        float sum = 0.f;
+  for (int h0 = group; h0 < heads; h0 += HEADS * UB) {
+    u32x4 w[UB][2 * PIECES];
+    char* dst[UB];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a[i], a[i], __builtin_fmaf(b[i], b[i], sum));
-        const float inv = 1.f / sqrtf(head_sum<G>(sum) * (1.f / D) + P.eps);
-        const int wdt = (is_q ? P.q_norm_f32 : P.k_norm_f32) ? HALO_F32 : DT;
+    for (int u = 0; u < UB; ++u) {
+      const int h = h0 + u * HEADS;
+      const bool is_q = h < P.H, is_v = h >= P.H + P.H_kv;
+      const int hk = h - P.H - (is_v ? P.H_kv : 0);
+      dst[u] = h >= heads || !(is_q || kept) ? nullptr
+               : is_q                        ? P.out + n * P.osn + h * P.osh
+                                             : (is_v ? P.pool.v : P.pool.k) + place + hk * P.pool.sh;
+      if (dst[u] != nullptr) {
+        const char* src = is_q ? P.q + n * P.qsn + h * P.qsh : is_v ? P.v + n * P.vsn + hk * P.vsh : P.k + n * P.ksn + hk * P.ksh;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] = a[i] * inv * load_elem(w, ca + i, wdt);
-          b[i] = b[i] * inv * load_elem(w, cb + i, wdt);
-        }
-      }
-      if (16 * lane < R) {
-        if (P.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
-            a[i] = a0 * c[i / 2] - a1 * s[i / 2];
-            a[i + 1] = a1 * c[i / 2] + a0 * s[i / 2];
-            b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
-            b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = a[i], y = b[i];
-            a[i] = x * c[i] - y * s[i];
-            b[i] = y * c[i] + x * s[i];
-          }
+        for (int i = 0; i < PIECES; ++i) {
+          w[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + ca * ES) + i);
+          w[u][PIECES + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + cb * ES) + i);
         }
       }
     }
-    store8<DT>(dst + ca * ES, a);
-    store8<DT>(dst + cb * ES, b);
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int h = h0 + u * HEADS;
+      if (dst[u] == nullptr) continue;
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        unpack16<DT>(__builtin_bit_cast(uint4, w[u][i]), a + i * (8 / PIECES));
+        unpack16<DT>(__builtin_bit_cast(uint4, w[u][PIECES + i]), b + i * (8 / PIECES));
+      }
+      if (h < P.H + P.H_kv) {
+        const bool is_q = h < P.H;
+        const void* wt = is_q ? P.q_norm : P.k_norm;
+        if (wt != nullptr) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a[i], a[i], __builtin_fmaf(b[i], b[i], sum));
+          const float inv = 1.f / sqrtf(head_sum<G>(sum) * (1.f / D) + P.eps);
+          const int wdt = (is_q ? P.q_norm_f32 : P.k_norm_f32) ? HALO_F32 : DT;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            a[i] = a[i] * inv * load_elem(wt, ca + i, wdt);
+            b[i] = b[i] * inv * load_elem(wt, cb + i, wdt);
+          }
+        }
+        if (turns) {
+          if (P.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
+              a[i] = a0 * c[i / 2] - a1 * s[i / 2];
+              a[i + 1] = a1 * c[i / 2] + a0 * s[i / 2];
+              b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
+              b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float x = a[i], y = b[i];
+              a[i] = x * c[i] - y * s[i];
+              b[i] = y * c[i] + x * s[i];
+            }
+          }
+        }
+      }
+      store8<DT>(dst[u] + ca * ES, a);
+      store8<DT>(dst[u] + cb * ES, b);
+    }
   }
 }
 
@@ -189,8 +211,6 @@ extern "C" int halo_rotate_rows(const halo_block_pool* pool, const void* q, int6
   p.H = H;
   p.H_kv = pool->H_kv;
   p.N = N;
-  p.parts = (int)heads;
-  p.per_row = make_div(p.parts);
   p.positions = positions;
   p.pos64 = pos64;
   p.cos = cos;
@@ -205,17 +225,17 @@ extern "C" int halo_rotate_rows(const halo_block_pool* pool, const void* q, int6
   p.k_norm_f32 = k_norm_f32;
   p.eps = eps;
   p.slots = slots;
-  const int per = kRotThreads / (pool->D / 16);
-  const dim3 grid((unsigned)(((int64_t)p.parts * N + per - 1) / per)), block(kRotThreads);
+  const int per = kRotThreads / 64;
+  const dim3 grid((unsigned)((N + per - 1) / per)), block(kRotThreads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-#define HALO_ROTATE(DTV)                                                                            \
-  do {                                                                                              \
-    if (pool->D == 128) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128>), grid, block, 0, st, p);  \
-    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64>), grid, block, 0, st, p);                  \
+#define HALO_ROTATE(DTV, UB)                                                                            \
+  do {                                                                                                  \
+    if (pool->D == 128) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128, UB>), grid, block, 0, st, p);  \
+    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64, UB>), grid, block, 0, st, p);                  \
   } while (0)
-  if (pool->dtype == HALO_F32) HALO_ROTATE(HALO_F32);
-  else if (pool->dtype == HALO_BF16) HALO_ROTATE(HALO_BF16);
-  else HALO_ROTATE(HALO_F16);
+  if (pool->dtype == HALO_F32) HALO_ROTATE(HALO_F32, 2);
+  else if (pool->dtype == HALO_BF16) HALO_ROTATE(HALO_BF16, 3);
+  else HALO_ROTATE(HALO_F16, 3);
 #undef HALO_ROTATE
   HALO_CHECK_HIP(hipGetLastError());
   return HALO_OK;

@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kVerMaxNodes = 512, kVerMaxPath = 64;
 constexpr int kWalkThreads = 1024, kSumThreads = 256;
-constexpr int kMaxSlab = 16384;  // tokens of a workgroup of the sums
+constexpr int kEach = 8;                     // tokens of a thread
+constexpr int kSlab = kSumThreads * kEach;   // of a workgroup of the sums
 
 // Where a request's walk ended: its last node's row, what is left of that row's
 // probabilities, and the tokens rejected there.
@@ -54,24 +55,41 @@ struct VerifyParams {
   int32_t* n_path;
   int64_t* token;
   VerifyEnd* ends;
-  double* parts;  // (B, slabs, 2): sums of R and of p
-  int slabs, slab;
+  double2* parts;  // (B, slabs): sums of R and of p
+  int slabs;
 };
 
 // A probability; NaN and what is below 0 count as 0.
 template <int DT>
-__device__ __forceinline__ double prob(const void* base, int64_t at) {
-  return fmax((double)load_elem(base, at, DT), 0.0);
+__device__ __forceinline__ float prob(const void* base, int64_t at) {
+  return fmaxf(load_elem(base, at, DT), 0.f);
+}
+// Those of kEach tokens from v on, 0 from V on.  Rows begin at any element: the
+// wide loads need no alignment.
+template <int DT>
+__device__ __forceinline__ void probs_at(const void* base, int64_t row, int v, int V, float (&f)[kEach]) {
+  constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = kEach * ES / 16;
+  if (v + kEach <= V) {
+    uint4 w[PIECES];
+    __builtin_memcpy(w, static_cast<const char*>(base) + (row + v) * ES, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) unpack16<DT>(w[i], f + i * (kEach / PIECES));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) f[i] = v + i < V ? load_elem(base, row + v + i, DT) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) f[i] = fmaxf(f[i], 0.f);
 }
 // What is left at one token.
-__device__ __forceinline__ double rest_of(double p, double q, double S) { return fmax(p - S * q, 0.0); }
+__device__ __forceinline__ double rest_of(float p, float q, double S) { return fmax((double)p - S * (double)q, 0.0); }
 
+// Sum over the workgroup, the same in every thread.
 template <int THREADS>
 __device__ __forceinline__ double block_sum(double x, double* s_wave) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
+  x = wave_prefix(x);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = x;
+  if ((threadIdx.x & 63) == 63) s_wave[threadIdx.x >> 6] = x;
   __syncthreads();
   double t = 0.0;
 #pragma unroll
@@ -83,8 +101,8 @@ __device__ __forceinline__ double block_sum(double x, double* s_wave) {
 // probabilities are gathered first, all at once.
 template <int DT>
 __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyParams P) {
-  __shared__ double s_p[kVerMaxNodes], s_q[kVerMaxNodes], s_wave[kWalkThreads / 64];
-  __shared__ float s_u[kVerMaxNodes];
+  __shared__ double s_wave[kWalkThreads / 64];
+  __shared__ float s_p[kVerMaxNodes], s_q[kVerMaxNodes], s_u[kVerMaxNodes];
   __shared__ int s_tok[kVerMaxNodes], s_gone[kVerMaxNodes];
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const int lo = max(P.cu[b], 0);
@@ -116,8 +134,8 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyParams 
     const bool there = x >= 0 && x < i && t >= 0 && t < P.V;
     s_tok[i] = there ? (int)t : -1;
     s_u[i] = P.accept[lo + i];
-    s_p[i] = there ? prob<DT>(P.p, (lo + x) * P.p_stride + t) : 0.0;
-    s_q[i] = there && P.q ? prob<DT>(P.q, (lo + x) * P.q_stride + t) : 1.0;
+    s_p[i] = there ? prob<DT>(P.p, (lo + x) * P.p_stride + t) : 0.f;
+    s_q[i] = there && P.q ? prob<DT>(P.q, (lo + x) * P.q_stride + t) : 1.f;
   }
   __syncthreads();
 
@@ -145,9 +163,9 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyParams 
       if (P.q == nullptr || !P.replacement) tried = !was && 1.0 - Q > 0.0;
     }
     const double d = P.q != nullptr && !P.replacement ? 1.0 / (1.0 - Q) : 1.0;
-    const double r = was ? 0.0 : P.q != nullptr ? rest_of(s_p[c], s_q[c], S) : s_p[c];
+    const double r = was ? 0.0 : P.q != nullptr ? rest_of(s_p[c], s_q[c], S) : (double)s_p[c];
     const int after = next_child(node, c);
-    if (tried && (double)s_u[c] * s_q[c] * d * Z < r) {
+    if (tried && (double)s_u[c] * (double)s_q[c] * d * Z < r) {
       if (threadIdx.x == 0) path[len] = c;
       node = c;
       ++len;
@@ -162,14 +180,21 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyParams 
       n_gone += !was;
       __syncthreads();
       if (P.q == nullptr) {
-        Z -= s_p[c];
+        Z -= (double)s_p[c];
       } else {
         S += Z * d;
-        Q += was ? 0.0 : s_q[c];
+        Q += was ? 0.0 : (double)s_q[c];
         if (after < n) {  // what is left counts for the next child
           double sum = 0.0;
           const int64_t pr = (lo + node) * P.p_stride, qr = (lo + node) * P.q_stride;
-          for (int v = threadIdx.x; v < P.V; v += kWalkThreads) sum += rest_of(prob<DT>(P.p, pr + v), prob<DT>(P.q, qr + v), S);
+#pragma unroll 2
+          for (int v = threadIdx.x * kEach; v < P.V; v += kWalkThreads * kEach) {
+            float p[kEach], q[kEach];
+            probs_at<DT>(P.p, pr, v, P.V, p);
+            probs_at<DT>(P.q, qr, v, P.V, q);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum += rest_of(p[i], q[i], S);
+          }
           for (int i = threadIdx.x; i < n_gone; i += kWalkThreads)
             sum -= rest_of(prob<DT>(P.p, pr + s_gone[i]), prob<DT>(P.q, qr + s_gone[i]), S);
           Z = block_sum<kWalkThreads>(sum, s_wave);
@@ -188,58 +213,64 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyParams 
   }
 }
 
-// Marks the rejected tokens of [v0, v0 + kMaxSlab) in LDS.
-__device__ __forceinline__ void mark_gone(const VerifyEnd* end, int n_gone, int v0, uint32_t* s_gone) {
-  for (int i = threadIdx.x; i < kMaxSlab / 32; i += kSumThreads) s_gone[i] = 0;
+// Which of this thread's tokens v0 + kEach t .. were rejected.
+__device__ __forceinline__ uint32_t gone_of(const VerifyEnd* end, int n_gone, int v0, uint32_t* s_gone) {
+  if (n_gone == 0) return 0;
+  if (threadIdx.x < kSlab / 32) s_gone[threadIdx.x] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n_gone; i += kSumThreads) {
     const int x = end->gone[i] - v0;
-    if (x >= 0 && x < kMaxSlab) atomicOr(&s_gone[x >> 5], 1u << (x & 31));
+    if (x >= 0 && x < kSlab) atomicOr(&s_gone[x >> 5], 1u << (x & 31));
   }
   __syncthreads();
+  return s_gone[threadIdx.x / 4] >> (threadIdx.x % 4 * kEach) & 0xff;
+}
+
+// What is left of this thread's tokens.
+template <int DT>
+__device__ __forceinline__ void rests(const VerifyParams& P, int row, int v, double S, uint32_t gone, float (&p)[kEach],
+                                      double (&r)[kEach]) {
+  probs_at<DT>(P.p, row * P.p_stride, v, P.V, p);
+  if (S != 0.0) {
+    float q[kEach];
+    probs_at<DT>(P.q, row * P.q_stride, v, P.V, q);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) r[i] = gone >> i & 1 ? 0.0 : rest_of(p[i], q[i], S);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) r[i] = gone >> i & 1 ? 0.0 : (double)p[i];
+  }
 }
 
 // Sums of what is left, a slab of tokens a workgroup.
 template <int DT>
 __global__ void __launch_bounds__(kSumThreads) verify_sum_kernel(VerifyParams P) {
-  __shared__ uint32_t s_gone[kMaxSlab / 32];
+  __shared__ uint32_t s_gone[kSlab / 32];
   __shared__ double s_wave[kSumThreads / 64];
-  const int b = blockIdx.y, v0 = blockIdx.x * P.slab, v1 = min(v0 + P.slab, P.V);
+  const int b = blockIdx.y, v0 = blockIdx.x * kSlab;
   const VerifyEnd* end = P.ends + b;
   const int row = end->row, n_gone = end->n_gone;
   if (row < 0) return;
-  const double S = end->S;
-  mark_gone(end, n_gone, v0, s_gone);
-  const int64_t pr = row * P.p_stride, qr = row * P.q_stride;
-  double rest = 0.0, all = 0.0;
-  for (int v = v0 + threadIdx.x; v < v1; v += kSumThreads) {
-    const double p = prob<DT>(P.p, pr + v), q = S != 0.0 ? prob<DT>(P.q, qr + v) : 0.0;
-    const bool gone = s_gone[(v - v0) >> 5] >> ((v - v0) & 31) & 1;
-    rest += gone ? 0.0 : rest_of(p, q, S);
-    all += p;
-  }
+  const uint32_t gone = gone_of(end, n_gone, v0, s_gone);
+  float p[kEach];
+  double r[kEach], rest = 0.0, all = 0.0;
+  rests<DT>(P, row, v0 + threadIdx.x * kEach, end->S, gone, p, r);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) rest += r[i], all += (double)p[i];
   rest = block_sum<kSumThreads>(rest, s_wave);
   all = block_sum<kSumThreads>(all, s_wave);
-  if (threadIdx.x == 0) {
-    P.parts[2 * ((int64_t)b * P.slabs + blockIdx.x)] = rest;
-    P.parts[2 * ((int64_t)b * P.slabs + blockIdx.x) + 1] = all;
-  }
+  if (threadIdx.x == 0) P.parts[(int64_t)b * P.slabs + blockIdx.x] = make_double2(rest, all);
 }
 
-// Exclusive sums over the workgroup's threads in order.
+// Sum over the workgroup's threads before this one.
 __device__ __forceinline__ double block_before(double x, double* s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double in = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double y = __shfl_up(in, off, 64);
-    if (lane >= off) in += y;
-  }
+  const int wave = threadIdx.x >> 6;
+  const double in = wave_prefix(x);
   __syncthreads();
-  if (lane == 63) s_wave[wave] = in;
+  if ((threadIdx.x & 63) == 63) s_wave[wave] = in;
   __syncthreads();
   double before = __shfl_up(in, 1, 64);
-  if (lane == 0) before = 0.0;
+  if ((threadIdx.x & 63) == 0) before = 0.0;
   for (int w = 0; w < wave; ++w) before += s_wave[w];
   return before;
 }
@@ -247,7 +278,7 @@ __device__ __forceinline__ double block_before(double x, double* s_wave) {
 // The token: the slab that passes u times the whole sum, then the token in it.
 template <int DT>
 __global__ void __launch_bounds__(kSumThreads) verify_pick_kernel(VerifyParams P) {
-  __shared__ uint32_t s_gone[kMaxSlab / 32];
+  __shared__ uint32_t s_gone[kSlab / 32];
   __shared__ double s_wave[kSumThreads / 64], s_from;
   __shared__ int s_slab, s_last, s_tok;
   const int b = blockIdx.x, tid = threadIdx.x;
@@ -257,82 +288,59 @@ __global__ void __launch_bounds__(kSumThreads) verify_pick_kernel(VerifyParams P
     if (tid == 0) P.token[b] = -1;
     return;
   }
-  const double* parts = P.parts + 2 * (int64_t)b * P.slabs;
-  if (tid == 0) s_slab = 0x7fffffff, s_last = -1, s_tok = 0x7fffffff;
-  double rest = 0.0, all = 0.0;
-  for (int g = tid; g < P.slabs; g += kSumThreads) rest += parts[2 * g], all += parts[2 * g + 1];
-  rest = block_sum<kSumThreads>(rest, s_wave);
-  all = block_sum<kSumThreads>(all, s_wave);
-  // where nothing is left (by rounding) the token comes from the target's probabilities
-  const bool whole = !(rest > 0.0);
-  const int n_gone = whole ? 0 : end->n_gone;
-  const double S = whole ? 0.0 : end->S;
-  const double T = (double)P.sample[b] * (whole ? all : rest);
   // slabs in order, as many a thread as there have to be
+  const double2* parts = P.parts + (int64_t)b * P.slabs;
   const int per = (P.slabs + kSumThreads - 1) / kSumThreads;
   const int g0 = min(tid * per, P.slabs), g1 = min(g0 + per, P.slabs);
-  double mine = 0.0;
-  for (int g = g0; g < g1; ++g) mine += parts[2 * g + whole];
-  double before = block_before(mine, s_wave);
+  if (tid == 0) s_slab = 0x7fffffff, s_last = -1, s_tok = 0x7fffffff;
+  double rest = 0.0, all = 0.0;
+  for (int g = g0; g < g1; ++g) rest += parts[g].x, all += parts[g].y;
+  const double rest_all = block_sum<kSumThreads>(rest, s_wave);
+  // where nothing is left (by rounding) the token comes from the target's probabilities
+  const bool whole = !(rest_all > 0.0);
+  const double T = (double)P.sample[b] * (whole ? block_sum<kSumThreads>(all, s_wave) : rest_all);
+  const double start = block_before(whole ? all : rest, s_wave);
+  double upto = start;
   for (int g = g0; g < g1; ++g) {
-    const double x = parts[2 * g + whole];
+    const double x = whole ? parts[g].y : parts[g].x;
     if (x > 0.0) atomicMax(&s_last, g);
-    if (before + x > T) atomicMin(&s_slab, g);
-    before += x;
+    upto += x;
+    if (upto > T) atomicMin(&s_slab, g);
   }
   __syncthreads();
   const int slab = s_slab != 0x7fffffff ? s_slab : max(s_last, 0);
-  // sum before the slab
-  mine = 0.0;
-  for (int g = tid; g < slab; g += kSumThreads) mine += parts[2 * g + whole];
-  const double from = block_sum<kSumThreads>(mine, s_wave);
-  const int v0 = slab * P.slab, v1 = min(v0 + P.slab, P.V);
-  mark_gone(end, n_gone, v0, s_gone);
-  if (tid == 0) s_last = -1;
-  __syncthreads();
-  const int64_t pr = row * P.p_stride, qr = row * P.q_stride;
-  const int each = (v1 - v0 + kSumThreads - 1) / kSumThreads;
-  const int a = min(v0 + tid * each, v1), z = min(a + each, v1);
-  auto left = [&](int v) {
-    const double p = prob<DT>(P.p, pr + v), q = S != 0.0 ? prob<DT>(P.q, qr + v) : 0.0;
-    return s_gone[(v - v0) >> 5] >> ((v - v0) & 31) & 1 ? 0.0 : rest_of(p, q, S);
-  };
-  mine = 0.0;
+  if (slab >= g0 && slab < g1) {  // one thread: what lies before the slab
+    upto = start;
+    for (int g = g0; g < slab; ++g) upto += whole ? parts[g].y : parts[g].x;
+    s_from = upto;
+  }
+  const int v0 = slab * kSlab, v = v0 + tid * kEach;
+  const uint32_t gone = gone_of(end, whole ? 0 : end->n_gone, v0, s_gone);
+  float p[kEach];
+  double r[kEach], mine = 0.0;
+  rests<DT>(P, row, v, whole ? 0.0 : end->S, gone, p, r);
   int last = -1;
-  for (int v = a; v < z; ++v) {
-    const double x = left(v);
-    mine += x;
-    if (x > 0.0) last = v;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    mine += r[i];
+    if (r[i] > 0.0) last = v + i;
   }
-  double upto = from + block_before(mine, s_wave);
+  __syncthreads();  // s_from is there, s_last has been read
+  if (tid == 0) s_last = -1;
+  upto = s_from + block_before(mine, s_wave);
   if (last >= 0) atomicMax(&s_last, last);
-  if (upto + mine > T) {
-    for (int v = a; v < z; ++v) {
-      upto += left(v);
-      if (upto > T) {
-        atomicMin(&s_tok, v);
-        break;
-      }
-    }
+  int tok = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    upto += r[i];
+    if (upto > T && r[i] > 0.0) tok = min(tok, v + i);
   }
+  if (tok != 0x7fffffff) atomicMin(&s_tok, tok);
   __syncthreads();
   if (tid == 0) P.token[b] = s_tok != 0x7fffffff ? s_tok : max(s_last, 0);
 }
 
-// Slabs: enough workgroups for the GPU, at least 2048 tokens each.
-struct VerifyShape {
-  int slabs, slab;
-};
-VerifyShape verify_shape(int B, int V) {
-  int64_t want = 512 / B < 1 ? 1 : 512 / B;
-  const int64_t most = (V + 2047) / 2048, least = (V + kMaxSlab - 1) / kMaxSlab;
-  want = want > most ? most : want < least ? least : want;
-  VerifyShape s;
-  s.slab = (int)((V + want - 1) / want + 7) / 8 * 8;
-  if (s.slab > kMaxSlab) s.slab = kMaxSlab;
-  s.slabs = (V + s.slab - 1) / s.slab;
-  return s;
-}
+int verify_slabs(int V) { return (V + kSlab - 1) / kSlab; }
 
 }  // namespace
 }  // namespace halo
@@ -341,7 +349,7 @@ using namespace halo;
 
 extern "C" size_t halo_verify_workspace_size(int B, int V) {
   if (B <= 0 || V <= 0) return 0;
-  return (size_t)B * sizeof(VerifyEnd) + (size_t)B * verify_shape(B, V).slabs * 16;
+  return (size_t)B * sizeof(VerifyEnd) + (size_t)B * verify_slabs(V) * sizeof(double2);
 }
 
 extern "C" int halo_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* cu_nodes, int B, int N,
@@ -361,15 +369,15 @@ extern "C" int halo_verify_tree(const int64_t* tokens, const int32_t* parents, c
     set_error("workspace too small");
     return HALO_E_WORKSPACE;
   }
-  const VerifyShape s = verify_shape(B, V);
+  const int slabs = verify_slabs(V);
   VerifyParams p = {tokens, parents, cu_nodes, B, N, max_nodes, V, probs, probs_stride, draft_probs, draft_stride, replacement,
                     accept, sample, max_path, path, n_path, token, reinterpret_cast<VerifyEnd*>(workspace),
-                    reinterpret_cast<double*>(reinterpret_cast<VerifyEnd*>(workspace) + B), s.slabs, s.slab};
+                    reinterpret_cast<double2*>(reinterpret_cast<VerifyEnd*>(workspace) + B), slabs};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
 #define HALO_VERIFY(DTV)                                                                                              \
   do {                                                                                                                \
     hipLaunchKernelGGL((verify_walk_kernel<DTV>), dim3((unsigned)B), dim3(kWalkThreads), 0, st, p);                   \
-    hipLaunchKernelGGL((verify_sum_kernel<DTV>), dim3((unsigned)s.slabs, (unsigned)B), dim3(kSumThreads), 0, st, p);  \
+    hipLaunchKernelGGL((verify_sum_kernel<DTV>), dim3((unsigned)slabs, (unsigned)B), dim3(kSumThreads), 0, st, p);  \
     hipLaunchKernelGGL((verify_pick_kernel<DTV>), dim3((unsigned)B), dim3(kSumThreads), 0, st, p);                    \
   } while (0)
   if (dtype == HALO_F32) HALO_VERIFY(HALO_F32);

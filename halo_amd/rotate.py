@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from . import _native as nat
+from . import block_pool as pool_calls
 from .block_pool import check_ints, on_stream, overlap, pack_pool
 
 
@@ -36,6 +37,10 @@ def rotate_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     is fp32, rounded once at the end.  A position outside the table makes the
     rotated channels NaN.  Slots must differ, as in ``append_rows``.  No gradient
     is kept."""
+    if pool_calls.calls is not None and stream is None and out is None:
+        r = pool_calls.calls.rotate_rows(q, k, v, positions, cos, sin, slots, k_pool, v_pool, q_norm, k_norm, eps, interleaved)
+        if r is not None:
+            return pool_calls.called(r, "halo_rotate_rows")
     L = nat.lib()
     pool = pack_pool(k_pool, v_pool, written=True)
     dev, dtype = k_pool.device, k_pool.dtype

@@ -79,6 +79,12 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     left out).  The lengths are read on the device, so a captured call follows
     them.  Above 512 rows at most 4096 requests; N times H / H_kv stays below
     2^30."""
+    if pool_calls.calls is not None and stream is None and out_dtype is None:
+        r = pool_calls.calls.chunk_attention(q, k_pool, v_pool, block_table, lengths, cu_rows, max_rows, scale, out, lse,
+                                             return_lse)
+        if r is not None:
+            return pool_calls.called(r, "halo_chunk_attn")
+    nat.lib()
     if max_rows < 1:
         raise AssertionError(f"max_rows must be at least 1, got {max_rows}")
     return _attend(q, k_pool, v_pool, block_table, lengths, cu_rows, "cu_rows", max_rows, None, True, scale, out, out_dtype,

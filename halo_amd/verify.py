@@ -13,6 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as nat
+from . import block_pool as pool_calls
 from .block_pool import _DTYPES, MAX_NODES, MAX_PATH, check_ints, on_stream
 
 
@@ -53,6 +54,11 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, cu_nodes: torch.Ten
     ``max_nodes`` (<= 512) is the largest tree, further nodes are left out; V <=
     2^24.  Tokens outside [0, V) are not accepted; NaN and negative probabilities
     count as 0.  Sums are held in 64 bits, and equal calls give equal results."""
+    if pool_calls.calls is not None and stream is None:
+        r = pool_calls.calls.verify_tree(tokens, parents, cu_nodes, probs, accept, sample, max_nodes, draft_probs, replacement,
+                                         min(max_nodes, MAX_PATH) if max_path is None else max_path)
+        if r is not None:
+            return Verified(*pool_calls.called(r, "halo_verify_tree"))
     L = nat.lib()
     dev = probs.device
     N, B = tokens.numel(), cu_nodes.numel() - 1
