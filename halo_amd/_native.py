@@ -204,12 +204,11 @@ _SIGNATURES = {
         _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # free, cap, n_free, shared, new_id, n_used
         _c_void_p, _size_t, _c_void_p,                           # workspace, bytes, stream
     ]),
-    "halo_verify_workspace_size": (_size_t, [_i32, _i32]),
     "halo_verify_tree": (_i32, [
         _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32,  # tokens, parents, cu_nodes, B, N, max_nodes, V, dtype
         _c_void_p, _i64, _c_void_p, _i64, _i32,          # probs, stride, draft_probs, stride, replacement
         _c_void_p, _c_void_p, _i32,                      # accept, sample, max_path
-        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size_t, _c_void_p,  # path, n_path, token, workspace, bytes, stream
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,      # path, n_path, token, stream
     ]),
     "halo_copy_blocks": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32, _i64,
                                 _c_void_p, _i32, _c_void_p]),

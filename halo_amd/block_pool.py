@@ -73,7 +73,7 @@ def load_calls(path=None):
         spec.loader.exec_module(mod)
         mod.bind([ctypes.cast(getattr(nat.lib(), "halo_" + n), ctypes.c_void_p).value for n in
                   ("update_block_tables", "append_rows", "tree_layout", "tree_workspace_size", "tree_attn", "commit_path",
-                   "chunk_workspace_size", "chunk_attn", "verify_workspace_size", "verify_tree", "rotate_rows",
+                   "chunk_workspace_size", "chunk_attn", "verify_tree", "rotate_rows",
                    "fork_workspace_size", "fork_blocks", "compact_workspace_size", "compact_blocks")])
         return mod
     except (ImportError, OSError, AttributeError):

@@ -34,7 +34,6 @@ struct Entries {
   decltype(&halo_commit_path) commit;
   decltype(&halo_chunk_workspace_size) chunk_workspace;
   decltype(&halo_chunk_attn) chunk;
-  decltype(&halo_verify_workspace_size) verify_workspace;
   decltype(&halo_verify_tree) verify;
   decltype(&halo_rotate_rows) rotate;
   decltype(&halo_fork_workspace_size) fork_workspace;
@@ -55,7 +54,6 @@ void bind(const std::vector<uintptr_t>& at) {
   next(lib.commit);
   next(lib.chunk_workspace);
   next(lib.chunk);
-  next(lib.verify_workspace);
   next(lib.verify);
   next(lib.rotate);
   next(lib.fork_workspace);
@@ -310,13 +308,11 @@ py::object verify_tree(const Tensor& tokens, const Tensor& parents, const Tensor
                 (V > 1 && draft->stride(1) != 1)))
     return py::none();
   Tensor path = empty({B, max_path}, at::kInt, d), n_path = empty({B}, at::kInt, d), token = empty({B}, at::kLong, d);
-  const size_t bytes = lib.verify_workspace((int)B, (int)V);
-  Tensor ws = empty({(int64_t)bytes}, at::kByte, d);
   const int rc = lib.verify(tokens.data_ptr<int64_t>(), parents.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), (int)B, (int)N,
                             (int)max_nodes, (int)V, dt, probs.data_ptr(), probs.stride(0), draft ? draft->data_ptr() : nullptr,
                             draft ? draft->stride(0) : 0, replacement, accept.data_ptr<float>(), sample.data_ptr<float>(),
                             (int)max_path, path.data_ptr<int32_t>(), n_path.data_ptr<int32_t>(), token.data_ptr<int64_t>(),
-                            ws.data_ptr(), bytes, stream_of(dev));
+                            stream_of(dev));
   if (rc != HALO_OK) return py::int_(rc);
   return py::make_tuple(path, n_path, token);
 }

@@ -11,6 +11,8 @@
 // A head's D channels are D / 16 lanes of two 8-channel pieces.  For the pairs
 // (i, i + R/2) the pieces of a lane are R/2 channels apart, so both of a pair
 // are in one lane, and its cosines and sines are 8 floats in a row either way.
+#include <type_traits>
+
 #include "block_pool.hpp"
 
 namespace halo {
@@ -23,7 +25,8 @@ struct RotateParams {
   const char* v;
   char* out;
   int64_t qsn, qsh, ksn, ksh, vsn, vsh, osn, osh;  // strides in bytes
-  int H, H_kv, N;
+  int H, H_kv, N, parts;
+  Div per_row;  // parts
   const void* positions;
   int pos64;
   const float* cos;
@@ -48,10 +51,9 @@ __device__ __forceinline__ void store8(char* p, const float* f) {
     store_elem4(p, 0, DT, f);
     store_elem4(p, 4, DT, f + 4);
   } else {
-    auto two = [](float x, float y) {
-      return DT == HALO_BF16 ? (uint32_t)f32_to_bf16_rne(x) | (uint32_t)f32_to_bf16_rne(y) << 16
-                             : (uint32_t)f32_to_f16_rne(x) | (uint32_t)f32_to_f16_rne(y) << 16;
-    };
+    typedef std::conditional_t<DT == HALO_BF16, __bf16, _Float16> T;
+    typedef __attribute__((ext_vector_type(2))) T T2;
+    auto two = [](float x, float y) { return __builtin_bit_cast(uint32_t, T2{(T)x, (T)y}); };  // to nearest even
     *reinterpret_cast<uint4*>(p) = make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7]));
   }
 }
@@ -65,19 +67,52 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-// A wave takes a row: its position and slot are the same for all lanes, the
-// cosines and sines are loaded once, and the row's heads go through in batches
-// of UB for each group of lanes, whose loads are in flight together.
+// Eight elements of a weight, which may begin anywhere.
+template <int DT>
+__device__ __forceinline__ void weights8(const void* at, bool f32, int i, float* w) {
+  if (f32) {
+    __builtin_memcpy(w, reinterpret_cast<const float*>(at) + i, 32);
+  } else if constexpr (DT != HALO_F32) {
+    uint4 x;
+    __builtin_memcpy(&x, reinterpret_cast<const uint16_t*>(at) + i, 16);
+    unpack16<DT>(x, w);
+  }
+}
+
+// A group of lanes takes UB heads of a row, `parts` apart, whose loads are in
+// flight together; position, cosines and sines are loaded once for them.  Bound
+// by memory: 32768 rows of 32 + 8 + 8 heads of 128 in bf16, normed, 822 MB: 170
+// to 176 us by the card (4.7 to 4.8 TB/s; a plain copy reaches 5.1).  One head a
+// group 263, two 198, four 179; a wave for a whole row 261 to 291, for its
+// reads and writes lie far apart.  Few heads are bound by the chain position ->
+// cosines -> store, which one head a group has shortest: 768 heads 5.0 us with one
+// and 6.3 with three, 12288 heads 6.2 and 6.8, 49152 heads 11.6 and 9.2.
+constexpr int64_t kRotFew = 16384;
 template <int DT, int D, int UB>
 __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P) {
-  constexpr int G = D / 16, HEADS = 64 / G;  // lanes of a head, heads side by side
+  constexpr int G = D / 16;  // lanes of a head
   constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = ES / 2;
-  const int n = blockIdx.x * (kRotThreads / 64) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int unit = blockIdx.x * (kRotThreads / G) + threadIdx.x / G;
+  const int n = div_by(unit, P.per_row);
   if (n >= P.N) return;
-  const int lane = threadIdx.x & (G - 1), group = (threadIdx.x & 63) / G;
+  const int part = unit - n * P.parts, lane = threadIdx.x & (G - 1);
   const int R = P.R, heads = P.H + 2 * P.H_kv;
   const bool turns = 16 * lane < R, halves = turns && !P.interleaved;
   const int ca = halves ? 8 * lane : 16 * lane, cb = halves ? R / 2 + 8 * lane : 16 * lane + 8;
+  u32x4 w[UB][2 * PIECES];
+#pragma unroll
+  for (int u = 0; u < UB; ++u) {
+    const int h = part + u * P.parts;
+    if (h >= heads) break;
+    const bool is_q = h < P.H, is_v = h >= P.H + P.H_kv;
+    const int hk = h - P.H - (is_v ? P.H_kv : 0);
+    const char* src = is_q ? P.q + n * P.qsn + h * P.qsh : is_v ? P.v + n * P.vsn + hk * P.vsh : P.k + n * P.ksn + hk * P.ksh;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      w[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + ca * ES) + i);
+      w[u][PIECES + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + cb * ES) + i);
+    }
+  }
   const int64_t slot = P.slots[n];
   const bool kept = slot >= 0 && slot < (int64_t)P.pool.blocks * P.pool.bs.d;
   const int blk = kept ? div_by((int)slot, P.pool.bs) : 0;
@@ -87,7 +122,7 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
   pos = there ? pos : 0;
   float c[8], s[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;  // channels that do not rotate
   if (turns) {
     const float* cr = P.cos + pos * P.trig_stride + 8 * lane;
     const float* sr = P.sin + pos * P.trig_stride + 8 * lane;
@@ -97,75 +132,58 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
       s[i] = sr[i];
     }
   }
-
-  for (int h0 = group; h0 < heads; h0 += HEADS * UB) {
-    u32x4 w[UB][2 * PIECES];
-    char* dst[UB];
 #pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int h = h0 + u * HEADS;
-      const bool is_q = h < P.H, is_v = h >= P.H + P.H_kv;
-      const int hk = h - P.H - (is_v ? P.H_kv : 0);
-      dst[u] = h >= heads || !(is_q || kept) ? nullptr
-               : is_q                        ? P.out + n * P.osn + h * P.osh
-                                             : (is_v ? P.pool.v : P.pool.k) + place + hk * P.pool.sh;
-      if (dst[u] != nullptr) {
-        const char* src = is_q ? P.q + n * P.qsn + h * P.qsh : is_v ? P.v + n * P.vsn + hk * P.vsh : P.k + n * P.ksn + hk * P.ksh;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          w[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + ca * ES) + i);
-          w[u][PIECES + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + cb * ES) + i);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int h = h0 + u * HEADS;
-      if (dst[u] == nullptr) continue;
-      float a[8], b[8];
+  for (int u = 0; u < UB; ++u) {
+    const int h = part + u * P.parts;
+    const bool is_q = h < P.H, is_v = h >= P.H + P.H_kv;
+    const int hk = h - P.H - (is_v ? P.H_kv : 0);
+    if (h >= heads || !(is_q || kept)) break;
+    char* dst = is_q ? P.out + n * P.osn + h * P.osh : (is_v ? P.pool.v : P.pool.k) + place + hk * P.pool.sh;
+    if (is_v) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        unpack16<DT>(__builtin_bit_cast(uint4, w[u][i]), a + i * (8 / PIECES));
-        unpack16<DT>(__builtin_bit_cast(uint4, w[u][PIECES + i]), b + i * (8 / PIECES));
+        *(reinterpret_cast<u32x4*>(dst + ca * ES) + i) = w[u][i];
+        *(reinterpret_cast<u32x4*>(dst + cb * ES) + i) = w[u][PIECES + i];
       }
-      if (h < P.H + P.H_kv) {
-        const bool is_q = h < P.H;
-        const void* wt = is_q ? P.q_norm : P.k_norm;
-        if (wt != nullptr) {
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a[i], a[i], __builtin_fmaf(b[i], b[i], sum));
-          const float inv = 1.f / sqrtf(head_sum<G>(sum) * (1.f / D) + P.eps);
-          const int wdt = (is_q ? P.q_norm_f32 : P.k_norm_f32) ? HALO_F32 : DT;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            a[i] = a[i] * inv * load_elem(wt, ca + i, wdt);
-            b[i] = b[i] * inv * load_elem(wt, cb + i, wdt);
-          }
-        }
-        if (turns) {
-          if (P.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-              const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
-              a[i] = a0 * c[i / 2] - a1 * s[i / 2];
-              a[i + 1] = a1 * c[i / 2] + a0 * s[i / 2];
-              b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
-              b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float x = a[i], y = b[i];
-              a[i] = x * c[i] - y * s[i];
-              b[i] = y * c[i] + x * s[i];
-            }
-          }
-        }
-      }
-      store8<DT>(dst[u] + ca * ES, a);
-      store8<DT>(dst[u] + cb * ES, b);
+      continue;
     }
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      unpack16<DT>(__builtin_bit_cast(uint4, w[u][i]), a + i * (8 / PIECES));
+      unpack16<DT>(__builtin_bit_cast(uint4, w[u][PIECES + i]), b + i * (8 / PIECES));
+    }
+    const void* norm = is_q ? P.q_norm : P.k_norm;
+    if (norm != nullptr) {
+      const bool f32 = DT == HALO_F32 || (is_q ? P.q_norm_f32 : P.k_norm_f32);
+      float wa[8], wb[8], sum = 0.f;
+      weights8<DT>(norm, f32, ca, wa);
+      weights8<DT>(norm, f32, cb, wb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a[i], a[i], __builtin_fmaf(b[i], b[i], sum));
+      const float inv = 1.f / sqrtf(head_sum<G>(sum) * (1.f / D) + P.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = a[i] * inv * wa[i], b[i] = b[i] * inv * wb[i];
+    }
+    if (P.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
+        a[i] = a0 * c[i / 2] - a1 * s[i / 2];
+        a[i + 1] = a1 * c[i / 2] + a0 * s[i / 2];
+        b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
+        b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = a[i], y = b[i];
+        a[i] = x * c[i] - y * s[i];
+        b[i] = y * c[i] + x * s[i];
+      }
+    }
+    store8<DT>(dst + ca * ES, a);
+    store8<DT>(dst + cb * ES, b);
   }
 }
 
@@ -225,17 +243,22 @@ extern "C" int halo_rotate_rows(const halo_block_pool* pool, const void* q, int6
   p.k_norm_f32 = k_norm_f32;
   p.eps = eps;
   p.slots = slots;
-  const int per = kRotThreads / 64;
-  const dim3 grid((unsigned)((N + per - 1) / per)), block(kRotThreads);
+  const int ub = heads * N < kRotFew ? 1 : 3;
+  p.parts = (int)((heads + ub - 1) / ub);
+  p.per_row = make_div(p.parts);
+  const int per = kRotThreads / (pool->D / 16);
+  const dim3 grid((unsigned)(((int64_t)p.parts * N + per - 1) / per)), block(kRotThreads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-#define HALO_ROTATE(DTV, UB)                                                                            \
-  do {                                                                                                  \
-    if (pool->D == 128) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128, UB>), grid, block, 0, st, p);  \
-    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64, UB>), grid, block, 0, st, p);                  \
+#define HALO_ROTATE(DTV)                                                                                               \
+  do {                                                                                                                 \
+    if (pool->D == 128 && ub == 3) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128, 3>), grid, block, 0, st, p);       \
+    else if (pool->D == 128) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128, 1>), grid, block, 0, st, p);             \
+    else if (ub == 3) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64, 3>), grid, block, 0, st, p);                     \
+    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64, 1>), grid, block, 0, st, p);                                  \
   } while (0)
-  if (pool->dtype == HALO_F32) HALO_ROTATE(HALO_F32, 2);
-  else if (pool->dtype == HALO_BF16) HALO_ROTATE(HALO_BF16, 3);
-  else HALO_ROTATE(HALO_F16, 3);
+  if (pool->dtype == HALO_F32) HALO_ROTATE(HALO_F32);
+  else if (pool->dtype == HALO_BF16) HALO_ROTATE(HALO_BF16);
+  else HALO_ROTATE(HALO_F16);
 #undef HALO_ROTATE
   HALO_CHECK_HIP(hipGetLastError());
   return HALO_OK;

@@ -26,17 +26,11 @@ namespace halo {
 namespace {
 
 constexpr int kVerMaxNodes = 512, kVerMaxPath = 64;
-constexpr int kWalkThreads = 1024, kSumThreads = 256;
-constexpr int kEach = 8;                     // tokens of a thread
-constexpr int kSlab = kSumThreads * kEach;   // of a workgroup of the sums
-
-// Where a request's walk ended: its last node's row, what is left of that row's
-// probabilities, and the tokens rejected there.
-struct VerifyEnd {
-  double S;
-  int32_t row, n_gone;  // row -1: a request without nodes
-  int32_t gone[kVerMaxNodes];
-};
+constexpr int kVerThreads = 1024, kVerWaves = kVerThreads / 64;
+constexpr int kEach = 8;                      // tokens of a thread at a time
+constexpr int kStep = 64 * kEach;             // of a wave
+constexpr int kTurn = kVerThreads * kEach;    // of the workgroup
+constexpr int kMarks = 16384;                 // bits that mark groups of kEach tokens, one of which may be rejected
 
 struct VerifyParams {
   const int64_t* tokens;
@@ -54,309 +48,332 @@ struct VerifyParams {
   int32_t* path;
   int32_t* n_path;
   int64_t* token;
-  VerifyEnd* ends;
-  double2* parts;  // (B, slabs): sums of R and of p
-  int slabs;
 };
 
 // A probability; NaN and what is below 0 count as 0.
+__device__ __forceinline__ float clean(float x) { return x > 0.f ? x : 0.f; }
+// What is left at one token.
+__device__ __forceinline__ double rest_of(float p, float q, double S) { return fmax(__builtin_fma(-S, (double)q, (double)p), 0.0); }
+
+// kEach tokens of a row.  Rows begin at any element: the wide loads need no alignment.
 template <int DT>
-__device__ __forceinline__ float prob(const void* base, int64_t at) {
-  return fmaxf(load_elem(base, at, DT), 0.f);
-}
-// Those of kEach tokens from v on, 0 from V on.  Rows begin at any element: the
-// wide loads need no alignment.
-template <int DT>
-__device__ __forceinline__ void probs_at(const void* base, int64_t row, int v, int V, float (&f)[kEach]) {
-  constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = kEach * ES / 16;
-  if (v + kEach <= V) {
-    uint4 w[PIECES];
-    __builtin_memcpy(w, static_cast<const char*>(base) + (row + v) * ES, sizeof(w));
+struct Probs {
+  static constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = kEach * ES / 16;
+  uint4 w[PIECES];
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    __builtin_memcpy(w, static_cast<const char*>(base) + at * ES, sizeof(w));
+  }
+  __device__ __forceinline__ void get(float (&f)[kEach]) const {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) unpack16<DT>(w[i], f + i * (kEach / PIECES));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) f[i] = v + i < V ? load_elem(base, row + v + i, DT) : 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) f[i] = fmaxf(f[i], 0.f);
-}
-// What is left at one token.
-__device__ __forceinline__ double rest_of(float p, float q, double S) { return fmax((double)p - S * (double)q, 0.0); }
+};
 
-// Sum over the workgroup, the same in every thread.
-template <int THREADS>
-__device__ __forceinline__ double block_sum(double x, double* s_wave) {
-  x = wave_prefix(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) s_wave[threadIdx.x >> 6] = x;
-  __syncthreads();
-  double t = 0.0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) t += s_wave[w];
-  return t;
-}
-
-// One workgroup a request walks its tree: all waves find the same.  Nodes'
-// probabilities are gathered first, all at once.
+// A workgroup's view of the row that its request's walk has reached: what is
+// left of it goes by S and the rejected tokens (list and marks in LDS).
+// The kernel's code is short on purpose: each line of it runs a few times, and
+// with every loop unrolled for itself (70 KB) half of the time was instruction fetch.
 template <int DT>
-__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyParams P) {
-  __shared__ double s_wave[kWalkThreads / 64];
-  __shared__ float s_p[kVerMaxNodes], s_q[kVerMaxNodes], s_u[kVerMaxNodes];
-  __shared__ int s_tok[kVerMaxNodes], s_gone[kVerMaxNodes];
-  const int b = blockIdx.x, lane = threadIdx.x & 63;
+struct VerifyRow {
+  const void* p;
+  const void* q;  // null where S is 0 for good
+  int64_t pr, qr;  // first elements
+  int V, n_gone;
+  double S;
+  const int* gone;
+  const uint32_t* marks;
+
+  // What is left of the tokens v .. v + kEach - 1 (v a multiple of kEach).
+  __device__ __forceinline__ void rests(int v, const float (&x)[kEach], const float (&y)[kEach], double (&r)[kEach]) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) r[i] = rest_of(x[i], clean(y[i]), S);
+    if (n_gone == 0) return;
+    const int g = v / kEach % kMarks;
+    if (marks[g >> 5] >> (g & 31) & 1)
+#pragma unroll 1
+      for (int k = 0; k < n_gone; ++k) {
+        const int x0 = gone[k] - v;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) r[i] = x0 == i ? 0.0 : r[i];
+      }
+  }
+  // The same one by one, 0 from V on.
+  __device__ __forceinline__ void rests_at(int v, double (&r)[kEach]) const {
+    float x[kEach], y[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      x[i] = v + i < V ? load_elem(p, pr + v + i, DT) : 0.f;
+      y[i] = S != 0.0 && v + i < V ? load_elem(q, qr + v + i, DT) : 0.f;
+    }
+    rests(v, x, y, r);
+  }
+  __device__ static __forceinline__ double sum8(const double (&r)[kEach]) {
+    return ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+  }
+  // This lane's part of the sum over [v0, v1), a wave's range (v0 a multiple of
+  // kEach): the loads of BATCH steps are in flight together.
+  __device__ __forceinline__ double part(int v0, int v1) const {
+    constexpr int BATCH = 4;
+    double sum = 0.0, r[kEach];
+    const int full = min(v1, V) - kEach;  // the last place of a wide load
+    const bool two = S != 0.0;
+#pragma unroll 1
+    for (int v = v0 + (threadIdx.x & 63) * kEach; v <= full; v += BATCH * kStep) {
+      Probs<DT> x[BATCH], y[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int at = min(v + k * kStep, full);  // (what is read twice is left out below)
+        x[k].load(p, pr + at);
+        if (two) y[k].load(q, qr + at);
+        else y[k] = {};
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        float f[kEach], g[kEach];
+        x[k].get(f);
+        y[k].get(g);
+        rests(v + k * kStep, f, g, r);
+        sum += v + k * kStep <= full ? sum8(r) : 0.0;
+      }
+    }
+    return sum;
+  }
+};
+
+// Tokens of each wave's range where the workgroup shares n of them: whole steps.
+__device__ __forceinline__ int range_of(int n) { return ((n + kVerWaves - 1) / kVerWaves + kStep - 1) / kStep * kStep; }
+
+struct VerifyNode {
+  float p, q, u;
+  int tok;  // -1: not tried
+};
+
+// One workgroup a request.  All its waves walk the tree alike: the nodes'
+// probabilities are gathered first, all at once, and a pass over the vocabulary
+// is made only where a rejected child has a sibling behind it (Z), and once for
+// the last token.  A pass gives each wave a range of tokens, so the range that
+// holds the token is found from 16 sums, and the token in it by one scan.
+template <int DT>
+__global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P) {
+  __shared__ double s_sum[kVerWaves];
+  __shared__ VerifyNode s_node[kVerMaxNodes];
+  __shared__ int s_gone[kVerMaxNodes], s_last, s_found;
+  __shared__ uint32_t s_marks[kMarks / 32];
+  constexpr int WORDS = kVerMaxNodes / 64;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lo = max(P.cu[b], 0);
   const int n = max(min(min(max(P.cu[b + 1], 0), P.N) - lo, P.max_nodes), 0);
-  VerifyEnd* end = P.ends + b;
   int32_t* path = P.path + (int64_t)b * P.max_path;
-  if (n == 0) {
-    for (int i = threadIdx.x; i < P.max_path; i += kWalkThreads) path[i] = -1;
-    if (threadIdx.x == 0) {
-      P.n_path[b] = 0;
-      end->row = -1;
-      end->n_gone = 0;
-    }
-    return;
-  }
-  int par[kVerMaxNodes / 64];  // of nodes lane, lane + 64, ..; -1: none
+  const float u_last = P.sample[b];
+  int par[WORDS], tok[WORDS];  // of nodes lane, lane + 64, ..; -1: none
 #pragma unroll
-  for (int w = 0; w < kVerMaxNodes / 64; ++w) {
+  for (int w = 0; w < WORDS; ++w) {
     const int i = w * 64 + lane;
-    par[w] = -1;
-    if (i < n) {
+    par[w] = tok[w] = -1;
+    if (w * 64 < n && i < n) {
+      const int64_t t = P.tokens[lo + i];
       const int x = P.parents[lo + i];
       par[w] = x >= 0 && x < i ? x : -1;
+      tok[w] = t >= 0 && t < P.V ? (int)t : -1;
+      if ((w & (kVerWaves - 1)) == wave) {  // one wave looks the node's probabilities up
+        VerifyNode y = {0.f, 1.f, P.accept[lo + i], tok[w]};
+        if (par[w] >= 0 && t >= 0 && t < P.V) {
+          y.p = clean(load_elem(P.p, (lo + x) * P.p_stride + t, DT));
+          if (P.q != nullptr) y.q = clean(load_elem(P.q, (lo + x) * P.q_stride + t, DT));
+        }
+        s_node[i] = y;
+      }
     }
-  }
-  for (int i = threadIdx.x; i < n; i += kWalkThreads) {
-    const int64_t t = P.tokens[lo + i];
-    const int x = P.parents[lo + i];
-    const bool there = x >= 0 && x < i && t >= 0 && t < P.V;
-    s_tok[i] = there ? (int)t : -1;
-    s_u[i] = P.accept[lo + i];
-    s_p[i] = there ? prob<DT>(P.p, (lo + x) * P.p_stride + t) : 0.f;
-    s_q[i] = there && P.q ? prob<DT>(P.q, (lo + x) * P.q_stride + t) : 1.f;
   }
   __syncthreads();
 
   // The first child of `node` behind `last`, or n.
   auto next_child = [&](int node, int last) {
+    int c = n;
 #pragma unroll
-    for (int w = 0; w < kVerMaxNodes / 64; ++w) {
+    for (int w = WORDS - 1; w >= 0; --w) {
+      if (w * 64 >= n) continue;
       uint64_t m = __ballot(par[w] == node);
       const int past = last + 1 - w * 64;  // bits from here on
       m &= past >= 64 ? 0 : past > 0 ? ~0ull << past : ~0ull;
-      if (m != 0) return w * 64 + (int)__builtin_ctzll(m);
+      if (m != 0) c = w * 64 + (int)__builtin_ctzll(m);
     }
-    return n;
+    return c;
   };
-
-  int node = 0, len = 1, n_gone = 0;
-  double S = 0.0, Z = 1.0, Q = 0.0;
-  if (threadIdx.x == 0) path[0] = 0;
-  int c = P.max_path > 1 ? next_child(0, 0) : n;
-  while (c < n) {
-    const int t = s_tok[c];
-    bool tried = t >= 0, was = false;
-    if (tried) {
-      for (int i0 = 0; i0 < n_gone; i0 += 64) was |= __ballot(i0 + lane < n_gone && s_gone[i0 + lane] == t) != 0;
-      if (P.q == nullptr || !P.replacement) tried = !was && 1.0 - Q > 0.0;
-    }
-    const double d = P.q != nullptr && !P.replacement ? 1.0 / (1.0 - Q) : 1.0;
-    const double r = was ? 0.0 : P.q != nullptr ? rest_of(s_p[c], s_q[c], S) : (double)s_p[c];
-    const int after = next_child(node, c);
-    if (tried && (double)s_u[c] * (double)s_q[c] * d * Z < r) {
-      if (threadIdx.x == 0) path[len] = c;
-      node = c;
-      ++len;
-      n_gone = 0;
-      S = 0.0, Z = 1.0, Q = 0.0;
-      c = len < P.max_path ? next_child(c, c) : n;
-      continue;
-    }
-    if (tried) {
-      __syncthreads();  // the list has been read
-      if (!was && threadIdx.x == 0) s_gone[n_gone] = t;
-      n_gone += !was;
-      __syncthreads();
-      if (P.q == nullptr) {
-        Z -= (double)s_p[c];
-      } else {
-        S += Z * d;
-        Q += was ? 0.0 : (double)s_q[c];
-        if (after < n) {  // what is left counts for the next child
-          double sum = 0.0;
-          const int64_t pr = (lo + node) * P.p_stride, qr = (lo + node) * P.q_stride;
-#pragma unroll 2
-          for (int v = threadIdx.x * kEach; v < P.V; v += kWalkThreads * kEach) {
-            float p[kEach], q[kEach];
-            probs_at<DT>(P.p, pr, v, P.V, p);
-            probs_at<DT>(P.q, qr, v, P.V, q);
+  VerifyRow<DT> R = {P.p, P.q, 0, 0, P.V, 0, 0.0, s_gone, s_marks};
+  uint32_t gone = 0;  // bit w: node w * 64 + lane was rejected at the node reached
+  int node = 0, len = 1, v0 = 0, v1 = P.V;
+  double Z = 1.0, Q = 0.0, T = 0.0, from = 0.0;
+  if (tid == 0 && n > 0) path[0] = 0;
+  int c = n > 0 && P.max_path > 1 ? next_child(0, 0) : n;
+  enum { kWalk, kLast, kWhole, kNarrow } mode = kWalk;
+  for (;;) {
+    if (mode == kWalk) {
+      bool left = false;  // whether what is left has to be summed for the next child
+#pragma unroll 1
+      while (c < n && !left) {
+        const VerifyNode y = s_node[c];
+        uint64_t same = 0;
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) sum += rest_of(p[i], q[i], S);
-          }
-          for (int i = threadIdx.x; i < n_gone; i += kWalkThreads)
-            sum -= rest_of(prob<DT>(P.p, pr + s_gone[i]), prob<DT>(P.q, qr + s_gone[i]), S);
-          Z = block_sum<kWalkThreads>(sum, s_wave);
+        for (int w = 0; w < WORDS; ++w)
+          if (w * 64 < n) same |= __ballot((gone >> w & 1) && tok[w] == y.tok);
+        const bool was = same != 0;
+        const double rest = 1.0 - Q;  // 1 with replacement
+        const bool tried = y.tok >= 0 && ((P.q != nullptr && P.replacement) || (!was && rest > 0.0));
+        const double r = was ? 0.0 : rest_of(y.p, y.q, P.q != nullptr ? R.S : 0.0);
+        // u q Z / rest < r, multiplied by rest: one division less on the way
+        if (tried && (double)y.u * (double)y.q * Z < r * rest) {
+          if (tid == 0) path[len] = c;
+          node = c;
+          ++len;
+          gone = 0;
+          R.S = 0.0, Z = 1.0, Q = 0.0;
+          c = len < P.max_path ? next_child(c, c) : n;
+          continue;
         }
+        const int after = next_child(node, c);
+        if (tried) {
+          if ((c & 63) == lane) gone |= 1u << (c >> 6);
+          if (P.q == nullptr) {
+            Z -= (double)y.p;
+          } else {
+            R.S += Z / rest;
+            if (!P.replacement) Q += (double)y.q;
+            left = after < n;
+          }
+        }
+        c = after;
+      }
+      if (!left) mode = kLast;
+      R.pr = (lo + node) * P.p_stride;
+      R.qr = (lo + node) * P.q_stride;
+      if (n == 0) break;
+    }
+    if (mode <= kLast) {  // the rejected tokens, listed and marked
+      R.n_gone = 0;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        if (w * 64 >= n) continue;
+        const uint64_t m = __ballot(gone >> w & 1);
+        if (wave == 0 && (gone >> w & 1)) s_gone[R.n_gone + __popcll(m & ((1ull << lane) - 1))] = tok[w];
+        R.n_gone += __popcll(m);
+      }
+      if (R.n_gone > 0) {
+        if (tid < kMarks / 32) s_marks[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < R.n_gone; i += kVerThreads) {
+          const int g = s_gone[i] / kEach % kMarks;
+          atomicOr(&s_marks[g >> 5], 1u << (g & 31));
+        }
+        __syncthreads();
       }
     }
-    c = after;
-  }
-  for (int i = len + threadIdx.x; i < P.max_path; i += kWalkThreads) path[i] = -1;
-  for (int i = threadIdx.x; i < n_gone; i += kWalkThreads) end->gone[i] = s_gone[i];
-  if (threadIdx.x == 0) {
-    P.n_path[b] = len;
-    end->S = S;
-    end->row = lo + node;
-    end->n_gone = n_gone;
-  }
-}
-
-// Which of this thread's tokens v0 + kEach t .. were rejected.
-__device__ __forceinline__ uint32_t gone_of(const VerifyEnd* end, int n_gone, int v0, uint32_t* s_gone) {
-  if (n_gone == 0) return 0;
-  if (threadIdx.x < kSlab / 32) s_gone[threadIdx.x] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_gone; i += kSumThreads) {
-    const int x = end->gone[i] - v0;
-    if (x >= 0 && x < kSlab) atomicOr(&s_gone[x >> 5], 1u << (x & 31));
-  }
-  __syncthreads();
-  return s_gone[threadIdx.x / 4] >> (threadIdx.x % 4 * kEach) & 0xff;
-}
-
-// What is left of this thread's tokens.
-template <int DT>
-__device__ __forceinline__ void rests(const VerifyParams& P, int row, int v, double S, uint32_t gone, float (&p)[kEach],
-                                      double (&r)[kEach]) {
-  probs_at<DT>(P.p, row * P.p_stride, v, P.V, p);
-  if (S != 0.0) {
-    float q[kEach];
-    probs_at<DT>(P.q, row * P.q_stride, v, P.V, q);
+    const int each = range_of(v1 - v0);
+    {
+      const int a = v0 + wave * each, z = min(a + each, v1);
+      double x = R.part(a, z);
+      // the one group of tokens that the row's end cuts
+      const int cut = P.V / kEach * kEach;
+      if (cut < P.V && cut >= a && cut < z && lane == 0) {
+        double r[kEach];
+        R.rests_at(cut, r);
+        x += R.sum8(r);
+      }
+      x = wave_prefix(x);
+      __syncthreads();  // sums of an earlier pass have been read
+      if (lane == 63) s_sum[wave] = x;
+      __syncthreads();
+    }
+    double sums[kVerWaves], total = 0.0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) r[i] = gone >> i & 1 ? 0.0 : rest_of(p[i], q[i], S);
-  } else {
+    for (int w = 0; w < kVerWaves; ++w) sums[w] = s_sum[w];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) r[i] = gone >> i & 1 ? 0.0 : (double)p[i];
+    for (int w = 0; w < kVerWaves; ++w) total += sums[w];
+    if (mode == kWalk) {
+      Z = total;
+      continue;
+    }
+    if (mode == kLast && !(total > 0.0)) {  // nothing is left (by rounding): the token comes from the target's probabilities
+      R.S = 0.0;
+      R.n_gone = 0;
+      mode = kWhole;
+      continue;
+    }
+    if (mode != kNarrow) T = (double)u_last * total;
+    mode = kNarrow;
+    // to the range that passes T; the last one with anything if rounding lets none pass
+    double upto = from, before = from;
+    int w = 0;
+    bool passed = false;
+#pragma unroll
+    for (int i = 0; i < kVerWaves; ++i) {
+      if (!passed && sums[i] > 0.0) w = i, before = upto;
+      upto += sums[i];
+      passed |= upto > T && sums[i] > 0.0;
+    }
+    if (!passed) T = INFINITY;
+    from = before;
+    v0 += w * each;
+    v1 = min(v0 + each, v1);
+    if (each <= kTurn) break;
   }
-}
-
-// Sums of what is left, a slab of tokens a workgroup.
-template <int DT>
-__global__ void __launch_bounds__(kSumThreads) verify_sum_kernel(VerifyParams P) {
-  __shared__ uint32_t s_gone[kSlab / 32];
-  __shared__ double s_wave[kSumThreads / 64];
-  const int b = blockIdx.y, v0 = blockIdx.x * kSlab;
-  const VerifyEnd* end = P.ends + b;
-  const int row = end->row, n_gone = end->n_gone;
-  if (row < 0) return;
-  const uint32_t gone = gone_of(end, n_gone, v0, s_gone);
-  float p[kEach];
-  double r[kEach], rest = 0.0, all = 0.0;
-  rests<DT>(P, row, v0 + threadIdx.x * kEach, end->S, gone, p, r);
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) rest += r[i], all += (double)p[i];
-  rest = block_sum<kSumThreads>(rest, s_wave);
-  all = block_sum<kSumThreads>(all, s_wave);
-  if (threadIdx.x == 0) P.parts[(int64_t)b * P.slabs + blockIdx.x] = make_double2(rest, all);
-}
-
-// Sum over the workgroup's threads before this one.
-__device__ __forceinline__ double block_before(double x, double* s_wave) {
-  const int wave = threadIdx.x >> 6;
-  const double in = wave_prefix(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) s_wave[wave] = in;
-  __syncthreads();
-  double before = __shfl_up(in, 1, 64);
-  if ((threadIdx.x & 63) == 0) before = 0.0;
-  for (int w = 0; w < wave; ++w) before += s_wave[w];
-  return before;
-}
-
-// The token: the slab that passes u times the whole sum, then the token in it.
-template <int DT>
-__global__ void __launch_bounds__(kSumThreads) verify_pick_kernel(VerifyParams P) {
-  __shared__ uint32_t s_gone[kSlab / 32];
-  __shared__ double s_wave[kSumThreads / 64], s_from;
-  __shared__ int s_slab, s_last, s_tok;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const VerifyEnd* end = P.ends + b;
-  const int row = end->row;
-  if (row < 0) {
-    if (tid == 0) P.token[b] = -1;
+  for (int i = (n > 0 ? len : 0) + tid; i < P.max_path; i += kVerThreads) path[i] = -1;
+  if (n == 0) {
+    if (tid == 0) {
+      P.n_path[b] = 0;
+      P.token[b] = -1;
+    }
     return;
   }
-  // slabs in order, as many a thread as there have to be
-  const double2* parts = P.parts + (int64_t)b * P.slabs;
-  const int per = (P.slabs + kSumThreads - 1) / kSumThreads;
-  const int g0 = min(tid * per, P.slabs), g1 = min(g0 + per, P.slabs);
-  if (tid == 0) s_slab = 0x7fffffff, s_last = -1, s_tok = 0x7fffffff;
-  double rest = 0.0, all = 0.0;
-  for (int g = g0; g < g1; ++g) rest += parts[g].x, all += parts[g].y;
-  const double rest_all = block_sum<kSumThreads>(rest, s_wave);
-  // where nothing is left (by rounding) the token comes from the target's probabilities
-  const bool whole = !(rest_all > 0.0);
-  const double T = (double)P.sample[b] * (whole ? block_sum<kSumThreads>(all, s_wave) : rest_all);
-  const double start = block_before(whole ? all : rest, s_wave);
-  double upto = start;
-  for (int g = g0; g < g1; ++g) {
-    const double x = whole ? parts[g].y : parts[g].x;
-    if (x > 0.0) atomicMax(&s_last, g);
-    upto += x;
-    if (upto > T) atomicMin(&s_slab, g);
-  }
-  __syncthreads();
-  const int slab = s_slab != 0x7fffffff ? s_slab : max(s_last, 0);
-  if (slab >= g0 && slab < g1) {  // one thread: what lies before the slab
-    upto = start;
-    for (int g = g0; g < slab; ++g) upto += whole ? parts[g].y : parts[g].x;
-    s_from = upto;
-  }
-  const int v0 = slab * kSlab, v = v0 + tid * kEach;
-  const uint32_t gone = gone_of(end, whole ? 0 : end->n_gone, v0, s_gone);
-  float p[kEach];
-  double r[kEach], mine = 0.0;
-  rests<DT>(P, row, v, whole ? 0.0 : end->S, gone, p, r);
+
+  // the range's tokens, kEach a thread, in order
+  const int v = v0 + tid * kEach;
+  double r[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) r[i] = 0.0;
+  if (v < v1) R.rests_at(v, r);
+  const double mine = R.sum8(r), in = wave_prefix(mine);
   int last = -1;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    mine += r[i];
+  for (int i = 0; i < kEach; ++i)
     if (r[i] > 0.0) last = v + i;
-  }
-  __syncthreads();  // s_from is there, s_last has been read
-  if (tid == 0) s_last = -1;
-  upto = s_from + block_before(mine, s_wave);
-  if (last >= 0) atomicMax(&s_last, last);
-  int tok = 0x7fffffff;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    upto += r[i];
-    if (upto > T && r[i] > 0.0) tok = min(tok, v + i);
-  }
-  if (tok != 0x7fffffff) atomicMin(&s_tok, tok);
+  const uint64_t some = __ballot(last >= 0);
   __syncthreads();
-  if (tid == 0) P.token[b] = s_tok != 0x7fffffff ? s_tok : max(s_last, 0);
+  if (lane == 63) s_sum[wave] = in;
+  if (tid == 0) s_last = 0, s_found = 0x7fffffff;
+  __syncthreads();
+  double upto = from;
+#pragma unroll
+  for (int w = 0; w < kVerWaves; ++w) upto += w < wave ? s_sum[w] : 0.0;
+  upto += in - mine;
+  if (some != 0 && lane == 63 - (int)__builtin_clzll(some)) atomicMax(&s_last, last);
+  int found = 0x7fffffff;
+#pragma unroll
+  for (int i = kEach - 1; i >= 0; --i) {
+    double at = upto;
+#pragma unroll
+    for (int k = 0; k <= i; ++k) at += r[k];
+    if (at > T && r[i] > 0.0) found = v + i;
+  }
+  const uint64_t passes = __ballot(found != 0x7fffffff);
+  if (passes != 0 && lane == (int)__builtin_ctzll(passes)) atomicMin(&s_found, found);
+  __syncthreads();
+  if (tid == 0) {
+    P.n_path[b] = len;
+    P.token[b] = s_found != 0x7fffffff ? s_found : s_last;
+  }
 }
-
-int verify_slabs(int V) { return (V + kSlab - 1) / kSlab; }
 
 }  // namespace
 }  // namespace halo
 
 using namespace halo;
 
-extern "C" size_t halo_verify_workspace_size(int B, int V) {
-  if (B <= 0 || V <= 0) return 0;
-  return (size_t)B * sizeof(VerifyEnd) + (size_t)B * verify_slabs(V) * sizeof(double2);
-}
-
 extern "C" int halo_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* cu_nodes, int B, int N,
                                 int max_nodes, int V, int dtype, const void* probs, int64_t probs_stride,
                                 const void* draft_probs, int64_t draft_stride, int replacement, const float* accept,
                                 const float* sample, int max_path, int32_t* path, int32_t* n_path, int64_t* token,
-                                void* workspace, size_t workspace_bytes, void* stream) {
+                                void* stream) {
   HALO_CHECK_ARG(cu_nodes && sample && path && n_path && token, "null pointer argument");
   HALO_CHECK_ARG(N >= 0 && (N == 0 || (tokens && parents && probs && accept)), "null pointer argument");
   HALO_CHECK_ARG(dtype == HALO_F32 || dtype == HALO_BF16 || dtype == HALO_F16, "dtype must be bf16, f16 or f32");
@@ -364,22 +381,11 @@ extern "C" int halo_verify_tree(const int64_t* tokens, const int32_t* parents, c
                  "need 1 <= B <= 65535, 1 <= V <= 2^24 and 1 <= max_nodes <= 512");
   HALO_CHECK_ARG(max_path > 0 && max_path <= kVerMaxPath, "need 1 <= max_path <= 64");
   HALO_CHECK_ARG(probs_stride >= 0 && draft_stride >= 0, "negative strides");
-  HALO_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace missing or not 16-byte aligned");
-  if (workspace_bytes < halo_verify_workspace_size(B, V)) {
-    set_error("workspace too small");
-    return HALO_E_WORKSPACE;
-  }
-  const int slabs = verify_slabs(V);
-  VerifyParams p = {tokens, parents, cu_nodes, B, N, max_nodes, V, probs, probs_stride, draft_probs, draft_stride, replacement,
-                    accept, sample, max_path, path, n_path, token, reinterpret_cast<VerifyEnd*>(workspace),
-                    reinterpret_cast<double2*>(reinterpret_cast<VerifyEnd*>(workspace) + B), slabs};
+  const VerifyParams p = {tokens, parents, cu_nodes, B, N, max_nodes, V, probs, probs_stride, draft_probs, draft_stride,
+                          replacement, accept, sample, max_path, path, n_path, token};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-#define HALO_VERIFY(DTV)                                                                                              \
-  do {                                                                                                                \
-    hipLaunchKernelGGL((verify_walk_kernel<DTV>), dim3((unsigned)B), dim3(kWalkThreads), 0, st, p);                   \
-    hipLaunchKernelGGL((verify_sum_kernel<DTV>), dim3((unsigned)slabs, (unsigned)B), dim3(kSumThreads), 0, st, p);  \
-    hipLaunchKernelGGL((verify_pick_kernel<DTV>), dim3((unsigned)B), dim3(kSumThreads), 0, st, p);                    \
-  } while (0)
+  const dim3 grid((unsigned)B), block(kVerThreads);
+#define HALO_VERIFY(DTV) hipLaunchKernelGGL((verify_tree_kernel<DTV>), grid, block, 0, st, p)
   if (dtype == HALO_F32) HALO_VERIFY(HALO_F32);
   else if (dtype == HALO_BF16) HALO_VERIFY(HALO_BF16);
   else HALO_VERIFY(HALO_F16);

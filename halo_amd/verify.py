@@ -87,11 +87,9 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, cu_nodes: torch.Ten
         path = torch.empty((B, max_path), device=dev, dtype=torch.int32)
         n_path = torch.empty(B, device=dev, dtype=torch.int32)
         token = torch.empty(B, device=dev, dtype=torch.int64)
-        nbytes = L.halo_verify_workspace_size(B, V)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         nat.check(L.halo_verify_tree(
             tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(), B, N, max_nodes, V, nat.dtype_code(probs.dtype),
             probs.data_ptr(), probs.stride(0), nat.ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
             replacement, accept.data_ptr(), sample.data_ptr(), max_path, path.data_ptr(), n_path.data_ptr(),
-            token.data_ptr(), ws.data_ptr(), nbytes, nat.stream_ptr()), "halo_verify_tree")
+            token.data_ptr(), nat.stream_ptr()), "halo_verify_tree")
     return Verified(path, n_path, token)

@@ -703,14 +703,11 @@ int halo_compact_blocks(const halo_block_pool* pool, int32_t* table, int64_t tab
  * path (B, max_path): the nodes, then -1; n_path (B) how many.  A request
  * without nodes has n_path 0 and token -1.  NaN and negative probabilities
  * count as 0.  Products and sums in 64 bits.  V <= 2^24, max_nodes <= 512.
- * workspace: halo_verify_workspace_size bytes, 16-byte aligned.
  */
-size_t halo_verify_workspace_size(int B, int V);
 int halo_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* cu_nodes, int B, int N, int max_nodes,
                      int V, int dtype, const void* probs, int64_t probs_stride, const void* draft_probs,
                      int64_t draft_stride, int replacement, const float* accept, const float* sample, int max_path,
-                     int32_t* path, int32_t* n_path, int64_t* token, void* workspace, size_t workspace_bytes,
-                     void* stream);
+                     int32_t* path, int32_t* n_path, int64_t* token, void* stream);
 
 /* ---- tier block moves -------------------------------------------------- */
 

@@ -227,13 +227,11 @@ def _call(fn, d, kw):
 
 def test_verify_entry_refuses(entries):  # noqa: F811
     d = dict(t=P, p=P, cu=P, B=2, N=5, mn=5, V=100, dt=0, pr=P, ps=100, q=P, qs=100, re=1, ac=P, sa=P, mp=4, pa=P, np=P, to=P,
-             ws=P, nb=entries.halo_verify_workspace_size(2, 100), st=None)
+             st=None)
     for kw in (dict(t=None), dict(cu=None), dict(pr=None), dict(sa=None), dict(to=None), dict(B=0), dict(B=70000), dict(N=-1),
                dict(mn=0), dict(mn=513), dict(V=0), dict(V=2 ** 24 + 1), dict(dt=5), dict(ps=-1), dict(qs=-1), dict(mp=0),
-               dict(mp=65), dict(ws=None), dict(ws=P + 8)):
+               dict(mp=65)):
         assert _call(entries.halo_verify_tree, d, kw) == -1, kw
-    assert _call(entries.halo_verify_tree, d, dict(nb=d["nb"] - 1)) == -4
-    assert entries.halo_verify_workspace_size(0, 5) == 0
 
 
 def test_rotate_entry_refuses(entries):  # noqa: F811
