@@ -27,10 +27,10 @@ namespace {
 
 constexpr int kVerMaxNodes = 512, kVerMaxPath = 64;
 constexpr int kVerThreads = 1024, kVerWaves = kVerThreads / 64;
-constexpr int kEach = 8;                      // tokens of a thread at a time
-constexpr int kStep = 64 * kEach;             // of a wave
-constexpr int kTurn = kVerThreads * kEach;    // of the workgroup
-constexpr int kMarks = 16384;                 // bits that mark groups of kEach tokens, one of which may be rejected
+constexpr int kEach = 8;                    // tokens of a thread in the last scan
+constexpr int kStep = 64 * kEach;           // waves' ranges are multiples of this
+constexpr int kTurn = kVerThreads * kEach;  // tokens that the last scan takes
+constexpr int kMarks = 16384;               // bits that mark groups of kEach tokens, one of which may be rejected
 
 struct VerifyParams {
   const int64_t* tokens;
@@ -55,18 +55,15 @@ __device__ __forceinline__ float clean(float x) { return x > 0.f ? x : 0.f; }
 // What is left at one token.
 __device__ __forceinline__ double rest_of(float p, float q, double S) { return fmax(__builtin_fma(-S, (double)q, (double)p), 0.0); }
 
-// kEach tokens of a row.  Rows begin at any element: the wide loads need no alignment.
+// The tokens of a 16-byte piece.  Rows begin at any element: the loads need no alignment.
 template <int DT>
-struct Probs {
-  static constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = kEach * ES / 16;
-  uint4 w[PIECES];
+struct Piece16 {
+  static constexpr int ES = DT == HALO_F32 ? 4 : 2, N = 16 / ES;
+  uint4 w;
   __device__ __forceinline__ void load(const void* base, int64_t at) {
-    __builtin_memcpy(w, static_cast<const char*>(base) + at * ES, sizeof(w));
+    __builtin_memcpy(&w, static_cast<const char*>(base) + at * ES, 16);
   }
-  __device__ __forceinline__ void get(float (&f)[kEach]) const {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) unpack16<DT>(w[i], f + i * (kEach / PIECES));
-  }
+  __device__ __forceinline__ void get(float* f) const { unpack16<DT>(w, f); }
 };
 
 // A workgroup's view of the row that its request's walk has reached: what is
@@ -80,60 +77,105 @@ struct VerifyRow {
   int64_t pr, qr;  // first elements
   int V, n_gone;
   double S;
+  bool masked;  // without a draft: rejected tokens are left out one by one, found by their marks
   const int* gone;
   const uint32_t* marks;
 
-  // What is left of the tokens v .. v + kEach - 1 (v a multiple of kEach).
-  __device__ __forceinline__ void rests(int v, const float (&x)[kEach], const float (&y)[kEach], double (&r)[kEach]) const {
+  static constexpr int EP = Piece16<DT>::N;
+
+  // What is left of the tokens v .. v + N - 1, the rejected ones included.
+  template <int N>
+  __device__ __forceinline__ void rests(const float (&x)[N], const float (&y)[N], double (&r)[N]) const {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) r[i] = rest_of(x[i], clean(y[i]), S);
-    if (n_gone == 0) return;
-    const int g = v / kEach % kMarks;
-    if (marks[g >> 5] >> (g & 31) & 1)
-#pragma unroll 1
-      for (int k = 0; k < n_gone; ++k) {
-        const int x0 = gone[k] - v;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) r[i] = x0 == i ? 0.0 : r[i];
-      }
+    for (int i = 0; i < N; ++i) r[i] = rest_of(x[i], clean(y[i]), S);
   }
-  // The same one by one, 0 from V on.
+  // Without those of the tokens v .. that were rejected.
+  template <int N>
+  __device__ __forceinline__ void leave_out(int v, double (&r)[N]) const {
+#pragma unroll 1
+    for (int k = 0; k < n_gone; ++k) {
+      const int x0 = gone[k] - v;
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = x0 == i ? 0.0 : r[i];
+    }
+  }
+  __device__ __forceinline__ bool marked(int v) const {
+    const int g = v / kEach % kMarks;
+    return marks[g >> 5] >> (g & 31) & 1;
+  }
+  template <int N>
+  __device__ static __forceinline__ double sum_of(const double (&r)[N]) {
+    const double t = (r[0] + r[1]) + (r[2] + r[3]);
+    if constexpr (N == 8) return t + ((r[4] + r[5]) + (r[6] + r[7]));
+    else return t;
+  }
+  // The same for kEach tokens from v on, 0 from V on.
   __device__ __forceinline__ void rests_at(int v, double (&r)[kEach]) const {
     float x[kEach], y[kEach];
+    if (v + kEach <= V) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      x[i] = v + i < V ? load_elem(p, pr + v + i, DT) : 0.f;
-      y[i] = S != 0.0 && v + i < V ? load_elem(q, qr + v + i, DT) : 0.f;
+      for (int i = 0; i < kEach; i += EP) {
+        Piece16<DT> a, b = {};
+        a.load(p, pr + v + i);
+        if (S != 0.0) b.load(q, qr + v + i);
+        a.get(x + i);
+        b.get(y + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        x[i] = v + i < V ? load_elem(p, pr + v + i, DT) : 0.f;
+        y[i] = S != 0.0 && v + i < V ? load_elem(q, qr + v + i, DT) : 0.f;
+      }
     }
-    rests(v, x, y, r);
-  }
-  __device__ static __forceinline__ double sum8(const double (&r)[kEach]) {
-    return ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+    rests(x, y, r);
+    leave_out(v, r);
   }
   // This lane's part of the sum over [v0, v1), a wave's range (v0 a multiple of
-  // kEach): the loads of BATCH steps are in flight together.
+  // kStep).  A load of the wave is 1 KiB side by side, and those of BATCH pieces
+  // of p and of q are in flight together.
   __device__ __forceinline__ double part(int v0, int v1) const {
-    constexpr int BATCH = 4;
-    double sum = 0.0, r[kEach];
-    const int full = min(v1, V) - kEach;  // the last place of a wide load
+    constexpr int BATCH = 32 / EP, STEP = 64 * EP;
+    double sum = 0.0, r[EP];
+    const int full = min(v1, V) - EP;  // the last place of a whole piece
     const bool two = S != 0.0;
 #pragma unroll 1
-    for (int v = v0 + (threadIdx.x & 63) * kEach; v <= full; v += BATCH * kStep) {
-      Probs<DT> x[BATCH], y[BATCH];
+    for (int v = v0 + (threadIdx.x & 63) * EP; v <= full; v += BATCH * STEP) {
+      Piece16<DT> x[BATCH], y[BATCH];
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
-        const int at = min(v + k * kStep, full);  // (what is read twice is left out below)
+        const int at = min(v + k * STEP, full);  // (what is read twice is left out below)
         x[k].load(p, pr + at);
         if (two) y[k].load(q, qr + at);
         else y[k] = {};
       }
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
-        float f[kEach], g[kEach];
+        float f[EP], g[EP];
         x[k].get(f);
         y[k].get(g);
-        rests(v + k * kStep, f, g, r);
-        sum += v + k * kStep <= full ? sum8(r) : 0.0;
+        rests(f, g, r);
+        if (masked && marked(v + k * STEP)) leave_out(v + k * STEP, r);
+        sum += v + k * STEP <= full ? sum_of(r) : 0.0;
+      }
+    }
+    // the one piece that the row's end cuts
+    const int cut = V / EP * EP;
+    if (cut < V && cut >= v0 && cut < v1 && (threadIdx.x & 63) == 0) {
+#pragma unroll 1
+      for (int v = cut; v < V; ++v) {
+        double one = rest_of(load_elem(p, pr + v, DT), two ? clean(load_elem(q, qr + v, DT)) : 0.f, S);
+#pragma unroll 1
+        for (int k = 0; masked && k < n_gone; ++k) one = gone[k] == v ? 0.0 : one;
+        sum += one;
+      }
+    }
+    // Against a draft a rejected token has p - S q < 0 but for rounding: what is above 0 of it is taken back.
+    if (!masked && n_gone > 0) {
+#pragma unroll 1
+      for (int k = threadIdx.x & 63; k < n_gone; k += 64) {
+        const int v = gone[k];
+        if (v >= v0 && v < v1) sum -= rest_of(load_elem(p, pr + v, DT), two ? clean(load_elem(q, qr + v, DT)) : 0.f, S);
       }
     }
     return sum;
@@ -200,7 +242,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P
     }
     return c;
   };
-  VerifyRow<DT> R = {P.p, P.q, 0, 0, P.V, 0, 0.0, s_gone, s_marks};
+  VerifyRow<DT> R = {P.p, P.q, 0, 0, P.V, 0, 0.0, false, s_gone, s_marks};
   uint32_t gone = 0;  // bit w: node w * 64 + lane was rejected at the node reached
   int node = 0, len = 1, v0 = 0, v1 = P.V;
   double Z = 1.0, Q = 0.0, T = 0.0, from = 0.0;
@@ -233,7 +275,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P
         }
         const int after = next_child(node, c);
         if (tried) {
-          if ((c & 63) == lane) gone |= 1u << (c >> 6);
+          if (!was && (c & 63) == lane) gone |= 1u << (c >> 6);
           if (P.q == nullptr) {
             Z -= (double)y.p;
           } else {
@@ -258,7 +300,10 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P
         if (wave == 0 && (gone >> w & 1)) s_gone[R.n_gone + __popcll(m & ((1ull << lane) - 1))] = tok[w];
         R.n_gone += __popcll(m);
       }
-      if (R.n_gone > 0) {
+      R.masked = R.n_gone > 0 && P.q == nullptr;
+      if (!R.masked) {
+        if (R.n_gone > 0) __syncthreads();
+      } else {
         if (tid < kMarks / 32) s_marks[tid] = 0;
         __syncthreads();
         for (int i = tid; i < R.n_gone; i += kVerThreads) {
@@ -272,23 +317,12 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P
     {
       const int a = v0 + wave * each, z = min(a + each, v1);
       double x = R.part(a, z);
-      // the one group of tokens that the row's end cuts
-      const int cut = P.V / kEach * kEach;
-      if (cut < P.V && cut >= a && cut < z && lane == 0) {
-        double r[kEach];
-        R.rests_at(cut, r);
-        x += R.sum8(r);
-      }
       x = wave_prefix(x);
       __syncthreads();  // sums of an earlier pass have been read
       if (lane == 63) s_sum[wave] = x;
       __syncthreads();
     }
-    double sums[kVerWaves], total = 0.0;
-#pragma unroll
-    for (int w = 0; w < kVerWaves; ++w) sums[w] = s_sum[w];
-#pragma unroll
-    for (int w = 0; w < kVerWaves; ++w) total += sums[w];
+    const double mine = lane < kVerWaves ? s_sum[lane] : 0.0, upto = wave_prefix(mine), total = lane_of(upto, 63);
     if (mode == kWalk) {
       Z = total;
       continue;
@@ -296,23 +330,17 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P
     if (mode == kLast && !(total > 0.0)) {  // nothing is left (by rounding): the token comes from the target's probabilities
       R.S = 0.0;
       R.n_gone = 0;
+      R.masked = false;
       mode = kWhole;
       continue;
     }
     if (mode != kNarrow) T = (double)u_last * total;
     mode = kNarrow;
     // to the range that passes T; the last one with anything if rounding lets none pass
-    double upto = from, before = from;
-    int w = 0;
-    bool passed = false;
-#pragma unroll
-    for (int i = 0; i < kVerWaves; ++i) {
-      if (!passed && sums[i] > 0.0) w = i, before = upto;
-      upto += sums[i];
-      passed |= upto > T && sums[i] > 0.0;
-    }
-    if (!passed) T = INFINITY;
-    from = before;
+    const uint64_t passed = __ballot(mine > 0.0 && from + upto > T), some = __ballot(mine > 0.0);
+    if (passed == 0) T = INFINITY;
+    const int w = passed != 0 ? (int)__builtin_ctzll(passed) : some != 0 ? 63 - (int)__builtin_clzll(some) : 0;
+    if (w > 0) from += lane_of(upto, w - 1);
     v0 += w * each;
     v1 = min(v0 + each, v1);
     if (each <= kTurn) break;
@@ -332,7 +360,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P
 #pragma unroll
   for (int i = 0; i < kEach; ++i) r[i] = 0.0;
   if (v < v1) R.rests_at(v, r);
-  const double mine = R.sum8(r), in = wave_prefix(mine);
+  const double mine = R.sum_of(r), in = wave_prefix(mine);
   int last = -1;
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
