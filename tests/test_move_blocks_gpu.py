@@ -283,3 +283,32 @@ def test_pools_past_32_bit_offsets(dev):
     new_id, used = halo_amd.compact_blocks(table, n, free, n_free, shared, kp, vp)
     assert used.tolist() == [2] and table.tolist() == [[P - 2, -1], [5, -1]] and new_id[P - 1].item() == 5
     assert bool((kp[5, 0, :40] == 3).all()) and bool((vp[5, 0, :40] == 4).all()) and free[:1].tolist() == [P - 1]
+
+
+@pytest.mark.parametrize("B,W,P", [(10, 1700, 900), (3, 5, 9000), (600, 4, 2000)])
+def test_tables_and_pools_that_one_workgroup_does_not_hold(dev, B, W, P):
+    """More entries, blocks or requests than the single launch takes."""
+    s = Store(dev, B=B, W=W, P=P, bs=4, L=2, H=1, D=8, dtype=F32, seed=B)
+    for b in range(0, B, 2):
+        s.give(b, s.rng.randint(0, 4 * min(W, P // B) - 4))
+    s.send()
+    s.compact()
+    for step in range(4):
+        s.fork([s.rng.choice([-1, b, b, s.rng.randrange(B), s.rng.randrange(B)]) for b in range(B)])
+        for b in range(B):
+            if s.rng.random() < 0.5 and s.n_free > 3 and s.lengths[b] < 4 * W - 4:
+                s.give(b, s.lengths[b] + s.rng.randint(0, 4))
+        s.send()
+    s.compact()
+
+
+@pytest.mark.parametrize("B,W,P", [(4, 7, 33000), (33, 2000, 3000)])
+def test_compaction_beyond_one_workgroup(dev, B, W, P):
+    s = Store(dev, B=B, W=W, P=P, bs=1, L=1, H=1, D=4, dtype=F32, seed=W)
+    for b in range(B):
+        s.give(b, s.rng.randint(0, min(W, P // B // 2)))
+    s.n_free -= 11  # blocks of somebody else
+    s.send()
+    s.compact()
+    assert s.fork([b if b % 3 else -1 for b in range(B)])
+    s.compact()
