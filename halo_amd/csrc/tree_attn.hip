@@ -104,6 +104,7 @@ __device__ __forceinline__ TreeReq tree_req(const TreeParams& P, int b) {
 struct TreeItem {
   int b, lo, ctx, n, rbs, tiles;
   int h, rb, cut, cuts;  // the cut-th of `cuts` cuts of the unit (h, rb)
+  int t0, t1;            // its tiles
   int part;              // partial of the unit's first cut
   int seen;              // rows from the first on that all rows of the unit see
 };
@@ -198,6 +199,8 @@ __device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeIte
       it.h = z;
       it.part = part + (it.rb * P.H_kv + it.h) * it.cuts;
       it.seen = it.ctx;
+      it.t0 = (int)((int64_t)it.tiles * it.cut / it.cuts);
+      it.t1 = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
       return true;
     }
     base += lane_of(at, 63);
@@ -216,32 +219,49 @@ __device__ __forceinline__ bool tree_find(const TreeParams& P, int x, TreeItem& 
   return P.B <= 64 ? tree_find_of<KT, R, ITEMS, 1>(P, x, it) : tree_find_of<KT, R, ITEMS, 4>(P, x, it);
 }
 
-// The same from the plan of a call of chunks; the heads of an item side by side.
+// Item i of the plan of a call of chunks, for head h.
 constexpr int kItemInts4 = 3;
-template <int R, bool ITEMS>
-__device__ __forceinline__ bool chunk_find(const TreeParams& P, int x, TreeItem& it) {
-  const int i = x / P.H_kv;
-  if (i >= P.plan[ITEMS ? 0 : 1]) return false;
-  const int4* at = P.items + (int64_t)(ITEMS ? i : P.cut_units[i]) * kItemInts4;
+template <int R>
+__device__ __forceinline__ void chunk_item(const TreeParams& P, int i, int h, TreeItem& it) {
+  const int4* at = P.items + (int64_t)i * kItemInts4;
   const int4 a = at[0], b = at[1], c = at[2];
-  it.h = x - i * P.H_kv;
+  it.h = h;
   it.b = uni(a.x);
   it.rb = uni(a.y);
   it.cut = uni(a.z);
   it.cuts = uni(a.w);
-  it.tiles = uni(b.x);
-  it.part = uni(b.y) + it.h * it.cuts;
-  it.lo = uni(b.z);
-  it.ctx = uni(b.w);
-  it.n = uni(c.x);
-  it.rbs = 0;
+  it.t0 = uni(b.x);
+  it.t1 = uni(b.y);
+  it.part = uni(b.z) + h * it.cuts;
+  it.lo = uni(b.w);
+  it.ctx = uni(c.x);
+  it.n = uni(c.y);
+  it.rbs = it.tiles = 0;
   it.seen = it.ctx + it.rb * R / P.rep + 1;
-  return true;
 }
-template <int KT, int R, bool ITEMS, bool CHUNK>
-__device__ __forceinline__ bool find_item(const TreeParams& P, int x, TreeItem& it) {
-  if constexpr (CHUNK) return chunk_find<R, ITEMS>(P, x, it);
-  else return tree_find<KT, R, ITEMS>(P, x, it);
+// The unit that block x of a merge launch has part in.
+template <int KT, int R, bool CHUNK>
+__device__ __forceinline__ bool find_cut_unit(const TreeParams& P, int x, TreeItem& it) {
+  if constexpr (!CHUNK) {
+    return tree_find<KT, R, false>(P, x, it);
+  } else {
+    const int i = x / P.H_kv;
+    if (i >= P.plan[1]) return false;
+    chunk_item<R>(P, P.cut_units[i], x - i * P.H_kv, it);
+    return true;
+  }
+}
+// Finds this workgroup's item; false past the last one.
+template <int KT, int R, bool CHUNK>
+__device__ __forceinline__ bool find_item(const TreeParams& P, TreeItem& it) {
+  if constexpr (!CHUNK) {
+    return tree_find<KT, R, true>(P, blockIdx.x, it);
+  } else {
+    const int i = blockIdx.x / P.H_kv;
+    if (i >= P.plan[0]) return false;
+    chunk_item<R>(P, i, blockIdx.x - i * P.H_kv, it);  // the heads of an item side by side
+    return true;
+  }
 }
 
 // Staging.  An LDS-DMA instruction fills 1 KiB, lane l its piece l, so RPI rows
@@ -796,12 +816,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __attribute__((aligned(16))) char sK[kTreeWaves][TB], sV[kTreeWaves][TB];
   __shared__ float2 s_ml[kTreeWaves][32];
   TreeItem it;
-  if (!find_item<kTreeKT, kTreeRows, true, CHUNK>(P, blockIdx.x, it)) return;
+  if (!find_item<kTreeKT, kTreeRows, CHUNK>(P, it)) return;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
-  const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
-  int t = (int)((int64_t)it.tiles * it.cut / it.cuts) + wave;
+  const int t_end = it.t1;
+  int t = it.t0 + wave;
   const int tree0 = it.seen / kTreeKT;
   char* const stK = sK[wave];
   char* const stV = sV[wave];
@@ -1016,12 +1036,11 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
   static_assert(L::KEYS * NW == KT, "the waves stage the tile");
   __shared__ __attribute__((aligned(16))) char sK0[TB], sK1[TB], sV0[TB], sV1[TB];
   TreeItem it;
-  if (!find_item<KT, R, true, CHUNK>(P, blockIdx.x, it)) return;
+  if (!find_item<KT, R, CHUNK>(P, it)) return;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)(threadIdx.x >> 6));
   const int qc = lane & 31, hh = lane >> 5;
-  const int t_end = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
-  const int t0 = (int)((int64_t)it.tiles * it.cut / it.cuts);
+  const int t_end = it.t1, t0 = it.t0;
   const int tree0 = it.seen / KT;  // first tile with rows that not all see
   const char* kh = P.k + (int64_t)it.h * P.sh * 16;
   const char* vh = P.v + (int64_t)it.h * P.sh * 16;
@@ -1317,7 +1336,7 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
   __shared__ float2 s_ml[MW][32];
   TreeItem it;
   const int rows32 = NW == 1 ? 0 : blockIdx.x % NW;  // which 32 of the unit's rows
-  if (!find_item<KT, 32 * NW, false, CHUNK>(P, blockIdx.x / NW, it)) return;
+  if (!find_cut_unit<KT, 32 * NW, CHUNK>(P, blockIdx.x / NW, it)) return;
   const int row0 = (it.rb * NW + rows32) * 32;
   if (row0 >= it.n * P.rep) return;
   const int lane = threadIdx.x & 63;
@@ -1405,36 +1424,38 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
 // ---------------------------------------------------------------------------
 // Chunks: any number of new rows a request, row i sees the rows up to length + i.
 // A unit (request, block of R rows) walks the tiles up to its last row, so units
-// differ, and one workgroup plans the call: with tiles_u the tiles of unit u and
-// H_kv workgroups for each, it weighs cutting the longest unit into c = 1 .. 32
-// and all others into pieces no longer than those,
-//   rounds of 256 workgroups x (mean item + kItemCost) + kPartCost x partials,
-// against the longest item alone, takes the cheapest c whose partials fit the
-// workspace, and lists the items, last rows (most tiles) first.
+// differ, and one workgroup plans the call, for each head the same.  It weighs
+// cutting the longest unit into c = 1 .. 32 pieces and all others into pieces no
+// longer than those,
+//   rounds of the workgroups that fit the GPU x (mean item + kItemCost),
+//   the longest item at least, and what the partials cost,
+// and lists the items, the last rows first (they have most tiles).  The pieces of
+// a request's units lie at nearly the same keys, so the workgroups that walk them
+// at one time share K and V in L2.  One stream of all tiles in even shares, one
+// for each workgroup, has no idle ones, but each reads other keys: 9 requests of
+// 1 to 2048 rows took 244 us where this takes XX.
 // ---------------------------------------------------------------------------
-constexpr int kChunkMaxB = 4096, kPlanThreads = 1024, kCandidates = 32;
-// In tiles: what an item costs besides its tiles (staging its first tiles, its
-// output), and a partial (written and read by all workgroups together).
-constexpr float kItemCost = 3.0f, kPartCost = 0.025f;
+constexpr int kChunkMaxB = 4096, kPlanThreads = 1024, kCandidates = 32, kPlanUnits = 8192;
+// In tiles: what an item costs besides its tiles (its first tiles are waited for,
+// its output stored), a partial (written, read and folded by all workgroups
+// together), and the launch that folds them.
+constexpr float kItemCost = 3.0f, kPartCost = 0.025f, kMergeCost = 2.0f;
 
 struct ChunkPlanParams {
   TreeParams t;
   int32_t* plan;
   int4* items;
   int32_t* cut_units;
-  int R, KT, min_tiles, unit_cap, part_cap;  // room for units, and for partials (of R rows, all heads)
+  int R, KT, slots, min_tiles, unit_cap, part_cap;  // slots: workgroups that fit the GPU; caps: room
 };
 
+// (Short code in 32 bits: it runs once, and fetching it is a good part of its time.)
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(ChunkPlanParams C) {
   const TreeParams& P = C.t;
-  __shared__ int s_at[kChunkMaxB + 1], s_sum[kPlanThreads / 64], s_max, s_best;
+  __shared__ int s_at[kChunkMaxB], s_n[kChunkMaxB], s_ctx[kChunkMaxB], s_tiles[kPlanUnits];
+  __shared__ int s_sum[kPlanThreads / 64], s_longest;
   __shared__ float s_cost[kCandidates];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-  auto rows_of = [&](int b, int& lo, int& ctx) {
-    lo = max(P.cu[b], 0);
-    ctx = (int)min((int64_t)max(P.lengths[b], 0), (int64_t)P.W * P.bs.d);
-    return max(min(min(max(P.cu[b + 1], 0), P.N) - lo, P.max_nodes), 0);  // (a difference of values below 0 could wrap)
-  };
   // Sum over the threads before this one, and of all.
   auto scan = [&](int x, int& all) {
     const int in = wave_prefix(x);
@@ -1443,104 +1464,106 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(ChunkPlanParam
     __syncthreads();
     const int t = lane < kPlanThreads / 64 ? s_sum[lane] : 0;
     const int ws = wave_prefix(t);
-    all = lane_of(ws, kPlanThreads / 64 - 1);
+    all = lane_of(ws, 63);
     return lane_of(ws - t, wave) + in - x;
   };
-  auto tiles_at = [&](int ctx, int n, int rb) {
-    const int last = min((int)min((int64_t)(rb + 1) * C.R, (int64_t)n * P.rep) - 1, n * P.rep - 1) / P.rep;
-    return (ctx + last + C.KT) / C.KT;
-  };
-  if (tid == 0) s_max = 0;
-  __syncthreads();
   const int per = (P.B + kPlanThreads - 1) / kPlanThreads;
   const int b0 = min(tid * per, P.B), b1 = min(b0 + per, P.B);
-  int mine = 0, pairs, longest = 0;
+  int mine = 0;
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
-    int lo, ctx;
-    const int n = rows_of(b, lo, ctx), rbs = (int)(((int64_t)n * P.rep + C.R - 1) / C.R);
-    mine += rbs;
-    if (n > 0) longest = max(longest, tiles_at(ctx, n, rbs - 1));
+    const int lo = max(P.cu[b], 0);
+    const int n = max(min(min(max(P.cu[b + 1], 0), P.N) - lo, P.max_nodes), 0);  // (a difference of values below 0 could wrap)
+    s_at[b] = mine;
+    s_n[b] = n;
+    s_ctx[b] = min(max(P.lengths[b], 0), P.W * P.bs.d);
+    mine += (n * P.rep + C.R - 1) / C.R;
   }
-  int at = scan(mine, pairs);
-  for (int b = b0; b < b1; ++b) {
-    int lo, ctx;
-    s_at[b] = at;
-    at += (int)(((int64_t)rows_of(b, lo, ctx) * P.rep + C.R - 1) / C.R);
-  }
-  if (tid == 0) s_at[P.B] = pairs;
-  atomicMax(&s_max, longest);
+  if (tid == 0) s_longest = 0;
+  int all;
+  const int before = scan(mine, all);
+  const int units = min(all, C.unit_cap);  // more only if the requests' rows overlap
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) s_at[b] += before;
   __syncthreads();
-  longest = s_max;
-  pairs = min(pairs, C.unit_cap);  // more only if the requests' rows overlap
-  if (pairs == 0) {
-    if (tid == 0) C.plan[0] = C.plan[1] = 0;
-    return;
-  }
-  auto find = [&](int u) {  // the request of unit u
-    int b = 0;
+  // Unit x from the last: its request, block of rows and tiles.
+  auto unit = [&](int x, int& b, int& rb) {
+    const int u = units - 1 - x;
+    b = 0;
+#pragma unroll 1
     for (int s = 1 << (31 - __clz(P.B)); s > 0; s >>= 1)
-      if (b + s < P.B && s_at[b + s] <= u) b += s;
-    return b;  // the last that starts at or before u, which has rows
+      if (b + s < P.B && s_at[b + s] <= u) b += s;  // the last that starts at or before u, which has rows
+    rb = u - s_at[b];
+    const int rows = min((rb + 1) * C.R, s_n[b] * P.rep);
+    return (s_ctx[b] + (rows - 1) / P.rep + C.KT) / C.KT;
   };
-  auto tiles_of = [&](int u, int& b, int& n, int& lo, int& ctx) {
-    b = find(u);
-    n = rows_of(b, lo, ctx);
-    return tiles_at(ctx, n, u - s_at[b]);
-  };
+  int longest = 0;
+#pragma unroll 1
+  for (int x = tid; x < units; x += kPlanThreads) {
+    int b, rb;
+    const int t = unit(x, b, rb);
+    if (x < kPlanUnits) s_tiles[x] = t;
+    longest = max(longest, t);
+  }
+  if (longest > 0) atomicMax(&s_longest, longest);
+  __syncthreads();
+  longest = s_longest;
+  auto piece = [&](int c) { return max((longest + c) / (c + 1), C.min_tiles); };
+#pragma unroll 1
   for (int c = wave; c < kCandidates; c += kPlanThreads / 64) {
-    const int L = max((longest + c) / (c + 1), C.min_tiles);
-    int64_t items = 0, parts = 0;
-    float total = 0.f;
-    for (int u = lane; u < pairs; u += 64) {
-      int b, n, lo, ctx;
-      const int t = tiles_of(u, b, n, lo, ctx), cuts = (t + L - 1) / L;
-      items += cuts;
-      parts += cuts > 1 ? cuts : 0;
+    const uint32_t L = piece(c);
+    float n = 0.f, parts = 0.f, total = 0.f;  // whole numbers, exact where they are small enough to matter
+#pragma unroll 1
+    for (int x = lane; x < units; x += 64) {
+      int b, rb;
+      const uint32_t t = x < kPlanUnits ? s_tiles[x] : unit(x, b, rb), cuts = (t + L - 1) / L;
+      n += (float)cuts;
+      parts += cuts > 1 ? (float)cuts : 0.f;
       total += (float)t;
     }
-    items = lane_of(wave_prefix(items), 63) * P.H_kv;
-    parts = lane_of(wave_prefix(parts), 63) * P.H_kv;
-    total = lane_of(wave_prefix(total), 63) * (float)P.H_kv;
-    const float mean = total / (float)items;
-    const float rounds = (float)((items + 255) / 256) * (mean + kItemCost);
-    const float cost = fmaxf(rounds, (float)min(L, longest) + kItemCost) + kPartCost * (float)parts;
-    if (lane == 0) s_cost[c] = parts <= C.part_cap ? cost : INFINITY;
+    n = lane_of(wave_prefix(n), 63);
+    parts = lane_of(wave_prefix(parts), 63) * (float)P.H_kv;
+    total = lane_of(wave_prefix(total), 63);
+    const float rounds = ceilf(n * (float)P.H_kv / (float)C.slots) * (total / n + kItemCost);
+    const float cost =
+        fmaxf(rounds, (float)min((int)L, longest) + kItemCost) + kPartCost * parts + (parts > 0.f ? kMergeCost : 0.f);
+    if (lane == 0) s_cost[c] = parts <= (float)C.part_cap ? cost : INFINITY;
   }
   __syncthreads();
-  if (tid == 0) {
-    int best = 0;
-    for (int c = 1; c < kCandidates; ++c)
-      if (s_cost[c] < s_cost[best]) best = c;
-    s_best = best;
-  }
-  __syncthreads();
-  const int L = max((longest + s_best) / (s_best + 1), C.min_tiles);
-  int base = 0, part = 0, cut_base = 0;
-  for (int u0 = 0; u0 < pairs; u0 += kPlanThreads) {
-    const int u = pairs - 1 - (u0 + tid);
-    int b = 0, n = 0, lo = 0, ctx = 0, t = 0, cuts = 0;
-    if (u >= 0) {
-      t = tiles_of(u, b, n, lo, ctx);
-      cuts = (t + L - 1) / L;
-    }
-    int all, all_parts, all_cut;
-    const int i0 = base + scan(cuts, all);
-    const int p0 = part + scan(cuts > 1 ? cuts * P.H_kv : 0, all_parts);
-    const int c0 = cut_base + scan(cuts > 1, all_cut);
-    for (int k = 0; k < cuts; ++k) {
+  // the cheapest, the first of equals; without cuts in any case where nothing else fits
+  const float cost = lane < kCandidates ? s_cost[lane] : INFINITY;
+  float least = cost;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) least = fminf(least, __shfl_xor(least, o, 64));
+  const uint64_t at_least = __ballot(cost == least);
+  const int best = at_least != 0 ? (int)__builtin_ctzll(at_least) : 0;
+  const uint32_t L = best == 0 ? 0x3fffffff : piece(best);
+  int items = 0, parts = 0, cut = 0;
+#pragma unroll 1
+  for (int x0 = 0; x0 < units; x0 += kPlanThreads) {
+    int b = 0, rb = 0;
+    const uint32_t t = x0 + tid < units ? unit(x0 + tid, b, rb) : 0;
+    const int cuts = (int)((t + L - 1) / L);
+    int items_all, parts_all, cut_all;
+    const int i0 = items + scan(cuts, items_all);
+    const int p0 = parts + scan(cuts > 1 ? cuts * P.H_kv : 0, parts_all);
+    const int c0 = cut + scan(cuts > 1, cut_all);
+    const int lo = cuts > 0 ? max(P.cu[b], 0) : 0;
+#pragma unroll 1
+    for (int k = 0; k < cuts; ++k) {  // t < 2^25, k <= 32
       int4* it = C.items + (int64_t)(i0 + k) * kItemInts4;
-      it[0] = make_int4(b, u - s_at[b], k, cuts);
-      it[1] = make_int4(t, p0, lo, ctx);
-      it[2] = make_int4(n, 0, 0, 0);
+      it[0] = make_int4(b, rb, k, cuts);
+      it[1] = make_int4(t * k / cuts, t * (k + 1) / cuts, p0, lo);
+      it[2] = make_int4(s_ctx[b], s_n[b], 0, 0);
     }
     if (cuts > 1) C.cut_units[c0] = i0;
-    base += all;
-    part += all_parts;
-    cut_base += all_cut;
+    items += items_all;
+    parts += parts_all;
+    cut += cut_all;
   }
   if (tid == 0) {
-    C.plan[0] = base;
-    C.plan[1] = cut_base;
+    C.plan[0] = items;
+    C.plan[1] = cut;
   }
 }
 
@@ -1747,25 +1770,27 @@ extern "C" int halo_tree_attn(const halo_block_pool* pool, const void* q, int64_
 
 namespace {
 
-// How a call of chunks is cut: rows and keys of a tile, units, items and partials at most.
+// How a call of chunks is cut: rows and keys of a tile, workgroups that the GPU
+// holds, units, cut units and items at most (of one head), partials (of all heads).
 struct ChunkShape {
-  int R, KT;
-  int64_t units, items, partials, cut_units;  // units: of one head; partials: of all heads
+  int R, KT, slots;
+  int64_t units, cut_units, items, partials;
 };
-ChunkShape chunk_shape(int dtype, int B, int N, int H, int H_kv) {
+ChunkShape chunk_shape(int dtype, int B, int N, int H, int H_kv, int D) {
   ChunkShape s;
   const bool f32 = dtype == HALO_F32;
   s.R = f32 ? kTreeRows : 256;
   s.KT = f32 ? kTreeKT : kTreeWideKT;
   s.units = (int64_t)N * (H / H_kv) / s.R + B;
-  s.partials = f32 ? 2048 : 512;
-  if (s.partials < 2 * H_kv) s.partials = 0;
+  // by registers one workgroup of 8 waves a CU, by LDS one or two of the fp32 kernel
+  s.slots = 256 * (f32 && D == 64 ? 2 : 1);
+  s.partials = 3 * s.slots;
   s.items = s.units + s.partials / H_kv;
   s.cut_units = s.partials / 2 / H_kv < s.units ? s.partials / 2 / H_kv : s.units;
   return s;
 }
 size_t chunk_bytes(const ChunkShape& s, int D) {
-  return (size_t)(s.partials * (s.R / 32) * tree_part_bytes(D) + s.items * kItemInts4 * 16 + (s.cut_units * 4 + 15) / 16 * 16 + 16);
+  return (size_t)(s.partials * (s.R / 32) * tree_part_bytes(D) + s.items * kItemInts4 * 16 + (s.cut_units + 8) * 4);
 }
 // Up to this many rows the tree kernels, without a plan.
 constexpr int kChunkTreeRows = 512;
@@ -1775,7 +1800,7 @@ constexpr int kChunkTreeRows = 512;
 extern "C" size_t halo_chunk_workspace_size(int dtype, int B, int N, int H, int H_kv, int D, int64_t max_keys, int max_rows) {
   if (max_rows <= kChunkTreeRows) return halo_tree_workspace_size(dtype, B, H, H_kv, D, max_keys, max_rows);
   if (N <= 0 || !tree_sizes_ok(B, H, H_kv, D, max_keys, 1)) return 0;
-  return chunk_bytes(chunk_shape(dtype, B, N, H, H_kv), D);
+  return chunk_bytes(chunk_shape(dtype, B, N, H, H_kv, D), D);
 }
 
 extern "C" int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64_t q_stride_n, int64_t q_stride_h, int N,
@@ -1793,9 +1818,9 @@ extern "C" int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64
   const int dtype = pool->dtype, D = pool->D;
   HALO_CHECK_ARG(B <= kChunkMaxB && (int64_t)N * p.rep < (1ll << 30), "need B <= 4096 and rows of all heads in 30 bits");
   HALO_CHECK_ARG((int64_t)W * pool->block_size + N < (1ll << 31) - 1024, "positions in 31 bits");
-  const ChunkShape s = chunk_shape(dtype, B, N, H, p.H_kv);
+  const ChunkShape s = chunk_shape(dtype, B, N, H, p.H_kv, D);
   // the units' number in 31 bits whatever cu_rows holds
-  HALO_CHECK_ARG((s.units + s.partials) * p.H_kv < (1ll << 31) && s.units * B < (1ll << 31), "too many rows and heads");
+  HALO_CHECK_ARG((s.units * p.H_kv + s.partials) < (1ll << 31) && s.units * B < (1ll << 31), "too many rows and heads");
   HALO_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace missing or not 16-byte aligned");
   if (workspace_bytes < chunk_bytes(s, D)) {
     set_error("workspace too small");
@@ -1810,16 +1835,17 @@ extern "C" int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64
   c.cut_units = c.plan + 4;
   c.R = s.R;
   c.KT = s.KT;
+  c.slots = s.slots;
   c.min_tiles = dtype == HALO_F32 ? 2 * kTreeWaves : 4;
-  c.part_cap = (int)s.partials;
   c.unit_cap = (int)s.units;
+  c.part_cap = (int)s.partials;
   p.items = c.items;
   p.plan = c.plan;
   p.cut_units = c.cut_units;
   c.t = p;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, c);
-  const dim3 grid((unsigned)(s.units * p.H_kv + s.partials)), mgrid((unsigned)(s.cut_units * p.H_kv * NW), D / 32);
+  const dim3 grid((unsigned)(s.items * p.H_kv)), mgrid((unsigned)(s.cut_units * p.H_kv * NW), D / 32);
 #define HALO_CHUNK(KERNEL, DV, DTV, KTV, NWV, THREADS)                                                             \
   do {                                                                                                             \
     hipLaunchKernelGGL((KERNEL), grid, dim3(THREADS), 0, st, p);                                                   \
