@@ -1792,14 +1792,21 @@ ChunkShape chunk_shape(int dtype, int B, int N, int H, int H_kv, int D) {
 size_t chunk_bytes(const ChunkShape& s, int D) {
   return (size_t)(s.partials * (s.R / 32) * tree_part_bytes(D) + s.items * kItemInts4 * 16 + (s.cut_units + 8) * 4);
 }
-// Up to this many rows the tree kernels, without a plan.
-constexpr int kChunkTreeRows = 512;
+// Up to this many rows in all the tree kernels, without a plan: each request's row
+// blocks walk all its tiles there, but nothing runs in front of them.  bf16, 32/8
+// heads of 128, one request behind 2000 rows, tree and chunk kernels: 96 rows 32
+// and 40 us, 192 rows 40 and 46, 256 rows 48 and 48, 512 rows 81 and 58; 8
+// requests: 48 rows each 46 and 48, 96 rows 85 and 77, 256 rows 129 and 116 (from
+// nothing 14 and 23, 27 and 25, 44 and 37).
+constexpr int kChunkTreeRows = 256;
+int tree_rows_of(int N, int max_rows) { return max_rows < N ? max_rows : N; }
 
 }  // namespace
 
 extern "C" size_t halo_chunk_workspace_size(int dtype, int B, int N, int H, int H_kv, int D, int64_t max_keys, int max_rows) {
-  if (max_rows <= kChunkTreeRows) return halo_tree_workspace_size(dtype, B, H, H_kv, D, max_keys, max_rows);
-  if (N <= 0 || !tree_sizes_ok(B, H, H_kv, D, max_keys, 1)) return 0;
+  if (N <= 0 || max_rows <= 0) return 0;
+  if (N <= kChunkTreeRows) return halo_tree_workspace_size(dtype, B, H, H_kv, D, max_keys, tree_rows_of(N, max_rows));
+  if (!tree_sizes_ok(B, H, H_kv, D, max_keys, 1)) return 0;
   return chunk_bytes(chunk_shape(dtype, B, N, H, H_kv, D), D);
 }
 
@@ -1808,9 +1815,11 @@ extern "C" int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64
                                const int32_t* cu_rows, int max_rows, float scale, void* out, int64_t out_stride_n,
                                int64_t out_stride_h, int out_dtype, float* lse, void* workspace, size_t workspace_bytes,
                                void* stream) {
-  if (max_rows <= kChunkTreeRows)
-    return halo_tree_attn(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_rows, max_rows, nullptr,
-                          0, scale, out, out_stride_n, out_stride_h, out_dtype, lse, workspace, workspace_bytes, stream);
+  HALO_CHECK_ARG(max_rows > 0, "need max_rows >= 1");
+  if (N <= kChunkTreeRows)
+    return halo_tree_attn(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_rows,
+                          N > 0 ? tree_rows_of(N, max_rows) : 1, nullptr, 0, scale, out, out_stride_n, out_stride_h, out_dtype,
+                          lse, workspace, workspace_bytes, stream);
   TreeParams p;
   const int rc = tree_params(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_rows, max_rows, 1,
                              nullptr, 0, scale, out, out_stride_n, out_stride_h, out_dtype, lse, &p);

@@ -613,7 +613,7 @@ int halo_commit_path(const halo_block_pool* pool, const int32_t* table, int64_t 
  * [0, lengths[b] + i]; everything else as in halo_tree_attn without masks, but
  * a request may have any number of rows, max_rows of them at most (further
  * ones are left out).  N * H / H_kv and W * block_size + N in 30 and 31 bits;
- * above 512 rows B <= 4096.  workspace: at least
+ * with N above 256 B <= 4096.  workspace: at least
  * halo_chunk_workspace_size(max_keys = W * block_size) bytes.
  */
 size_t halo_chunk_workspace_size(int dtype, int B, int N, int H, int H_kv, int D, int64_t max_keys, int max_rows);

@@ -34,8 +34,8 @@ class Batch(tree_launch.Batch):
 
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("ctx,rows", [(0, 1), (5, 1), (0, 64), (100, 511), (3, 512), (0, 513), (1, 514), (63, 577), (64, 1023),
-                                      (700, 640), (31, 1025)])
+@pytest.mark.parametrize("ctx,rows", [(0, 1), (5, 1), (0, 64), (100, 256), (3, 257), (0, 512), (1, 514), (63, 577), (64, 1023),
+                                      (700, 640), (31, 1025), (5000, 300)])
 def test_one_request(dev, ctx, rows, D, dtype):
     b = Batch(dev, lengths=[ctx], nodes=[rows], D=D, dtype=dtype, seed=rows)
     check(b, *b.run(), b.exact())
@@ -89,10 +89,16 @@ def test_many_requests(dev, B):
 
 
 @pytest.mark.parametrize("dtype", DT)
-def test_up_to_512_rows_it_is_the_causal_tree(dev, dtype):
-    b = Batch(dev, lengths=[300, 0, 1000], nodes=[40, 512, 1], dtype=dtype)
+def test_few_rows_are_the_causal_tree(dev, dtype):
+    """Up to 256 rows in all, by the same kernels; more rows, and so other kernels, give the same up to rounding."""
+    b = Batch(dev, lengths=[300, 0, 1000], nodes=[40, 215, 1], dtype=dtype)
     got, want = b.run(), tree_launch.Batch.run(b)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    got = b.run(max_rows=100000)
+    check(b, *got, b.exact())
+    b = Batch(dev, lengths=[300, 0, 1000], nodes=[40, 216, 1], dtype=dtype)
+    check(b, *b.run(), b.exact())
+    check(b, *tree_launch.Batch.run(b), b.exact())
 
 
 @pytest.mark.parametrize("dtype", DT)

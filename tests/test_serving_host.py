@@ -260,16 +260,16 @@ def test_fork_and_compact_entries_refuse(entries):  # noqa: F811
     assert _call(entries.halo_compact_blocks, d, dict(nb=d["nb"] - 1)) == -4
 
 
-@pytest.mark.parametrize("rows", [5, 600])
-def test_chunk_entry_refuses(entries, rows):  # noqa: F811
-    need = entries.halo_chunk_workspace_size(1, 1, 700, 4, 2, 64, 3 * 16, rows)
-    d = dict(pool=_pool(), q=P, qn=256, qh=64, N=700, H=4, table=P, ts=3, B=1, W=3, ln=P, cu=P, mr=rows, scale=0.125, out=P, on=256,
+@pytest.mark.parametrize("N,rows", [(200, 5), (200, 600), (700, 5), (700, 600)])
+def test_chunk_entry_refuses(entries, N, rows):  # noqa: F811
+    need = entries.halo_chunk_workspace_size(1, 1, N, 4, 2, 64, 3 * 16, rows)
+    d = dict(pool=_pool(), q=P, qn=256, qh=64, N=N, H=4, table=P, ts=3, B=1, W=3, ln=P, cu=P, mr=rows, scale=0.125, out=P, on=256,
              oh=64, odt=1, lse=None, ws=P, nb=max(need, 1 << 20), st=None)
     for kw in (dict(pool=_pool(dt=3)), dict(pool=_pool(D=96)), dict(pool=_pool(layers=2)), dict(pool=_pool(k=4104)), dict(H=5),
                dict(H=0), dict(B=0), dict(W=0), dict(mr=0), dict(q=4100), dict(q=None), dict(qn=257), dict(table=None), dict(ts=2),
                dict(scale=0.0), dict(out=None), dict(odt=7), dict(out=4100), dict(N=-1)):
         assert _call(entries.halo_chunk_attn, d, kw) == -1, kw
-    if rows > 512:
+    if N > 256:
         for kw in (dict(B=4097), dict(N=2 ** 30), dict(W=2 ** 27 - 128, ts=2 ** 27, N=2000), dict(ws=None), dict(ws=P + 4)):
             assert _call(entries.halo_chunk_attn, d, kw) == -1, kw
         assert need > 0 and _call(entries.halo_chunk_attn, d, dict(nb=need - 1)) == -4
