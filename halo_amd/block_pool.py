@@ -1,5 +1,6 @@
 """Requests over a pool of K/V blocks: block tables and slots, rows written to
-their slots, drafted trees and their accepted paths.
+their slots, drafted trees and their accepted paths, blocks shared, given up and
+moved.
 
 A pool is one layer (or all layers) of a ``TieredStorage`` tier,
 ``(blocks, H_kv, block_size, D)`` or ``(L, blocks, H_kv, block_size, D)``.  Row
@@ -13,10 +14,16 @@ One speculative step of a batch, all of it on the device::
     mask, depth = tree_layout(parents, up.cu_rows, max_nodes=n)    # row positions: lengths + depth
     for layer: append_rows(k, v, up.slots, k_pool[layer], v_pool[layer])
                tree_attention(q, k_pool[layer], v_pool[layer], block_table, lengths, up.cu_rows, mask=mask, ...)
-    lengths = commit_path(k_pool, v_pool, block_table, lengths, path, n_path)   # all layers
+    got = verify_tree(tokens, parents, up.cu_rows, probs, accept, sample, max_nodes=n)
+    lengths = commit_path(k_pool, v_pool, block_table, lengths, got.path, got.n_path)   # all layers
+
+Requests that share blocks, or end, go through ``fork_blocks``; ``compact_blocks``
+moves the used blocks to the pool's front.
 
 The calls know blocks, not tiers: where a store moves blocks between tiers,
-``TieredStorage.write_rows`` is ``append_rows`` with the tier directory kept.
+``TieredStorage.write_rows`` is ``append_rows`` with the tier directory kept
+(``TieredStorage.rotate_rows`` likewise); ``fork_blocks`` and ``compact_blocks``
+are for pools whose blocks all lie in the GPU tier.
 
 No call waits for the device, so a step can be captured in a HIP graph; the
 tensors a call changes are the caller's.  The calls run on ``stream`` (default:

@@ -37,6 +37,11 @@ __device__ __forceinline__ int plan_scan(int x, int* s_wave, int* all) {
 // that hold a block are whole numbers, so their order does not matter.  Blocks
 // whose holders come to none are pushed in the order of their ids, and the rows
 // that need a block for a copy pop theirs in the rows' order.
+//
+// Four launches, each a few dependent reads: begin 2.8 us, count 4.0 to 4.9, plan
+// 6.5, apply 6.8 for 32 beams of 256 to 4096 rows, 28 layers (19 MB of copies would
+// take 3.8).  All but the copies in one workgroup took 12.9 us where three
+// launches take 13.5, and 17 for 64 rows of 1026 entries.
 // ---------------------------------------------------------------------------
 // What a row becomes: whose blocks, how many of them, a block for a copy or -1;
 // and what that holds: the block to copy and how many of its rows.
@@ -237,6 +242,11 @@ __global__ void __launch_bounds__(kMoveThreads) fork_apply_kernel(ForkParams P, 
 // number of such blocks before x, the free blocks of rank below U are gaps and
 // the used ones of rank U and above move, the i-th of these into the i-th gap.
 // The number of gaps before x is rank(x) - used(x), so one scan places all.
+//
+// The moves are bound by memory: 480 blocks of 8 layers of 32 KiB, K and V, 0.5 GB
+// read and written in 92 to 102 us (a plain copy of as much 99); the three
+// launches in front of them take 16 (five blocks of a small pool: 1.4, 1.6, 5.4
+// and 5.1 us).
 // ---------------------------------------------------------------------------
 struct CompactParams {
   PoolView pool;

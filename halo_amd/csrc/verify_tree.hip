@@ -195,6 +195,13 @@ struct VerifyNode {
 // is made only where a rejected child has a sibling behind it (Z), and once for
 // the last token.  A pass gives each wave a range of tokens, so the range that
 // holds the token is found from 16 sums, and the token in it by one scan.
+//
+// Bound by chains: gather 0.8 us, walk 2 to 3, a pass, 2 to 3 for the last token;
+// and a pass by what one CU reads, 85 to 150 GB/s.  One request of 32768 bf16
+// tokens without draft probabilities 9.8 us; 48 chains over 131072 fp32 tokens,
+// 38 MB, 22 us (a pass of 1 MB 12, when 4.9 TB/s come from memory in all); 13 trees
+// over 50001 with up to 4 siblings 34 us (up to 5 passes of 4.5).  Spreading the
+// last sums over the GPU, with two more launches, took 16.4, 32 and 37 us.
 template <int DT>
 __global__ void __launch_bounds__(kVerThreads) verify_tree_kernel(VerifyParams P) {
   __shared__ double s_sum[kVerWaves];

@@ -350,12 +350,31 @@ class TieredStorage:
         tier holds: a block whose rows were written in another tier is moved here
         first.  Moves of the same blocks on other streams are waited for before
         (``HALORefetcher.wait``, ``HALODemoter.wait``)."""
-        from .block_pool import append_rows, on_stream
+        from .block_pool import append_rows
+        self._directory_for_capture()
+        append_rows(keys, values, slots, *self.pool("gpu", layer), stream=stream)
+        self._mark_written(slots, layer, stream)
+
+    def rotate_rows(self, *, q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, positions: torch.Tensor,
+                    cos: torch.Tensor, sin: torch.Tensor, slots: torch.Tensor, layer: int,
+                    stream: Optional[torch.cuda.Stream] = None, **kw) -> torch.Tensor:
+        """``halo_amd.rotate_rows`` to the GPU tier's pool of one layer (the norms'
+        weights and other options as there), after which the directory names the
+        GPU tier for the blocks written, as ``write_rows`` has it.  Returns q."""
+        from .rotate import rotate_rows
+        self._directory_for_capture()
+        out = rotate_rows(q, keys, values, positions, cos, sin, slots, *self.pool("gpu", layer), stream=stream, **kw)
+        self._mark_written(slots, layer, stream)
+        return out
+
+    def _directory_for_capture(self) -> None:
         if self._dir is None and self.on_device and torch.cuda.is_current_stream_capturing():
             raise AssertionError("the directory must exist before a graph is captured, whose replays would clear it")
-        k_pool, v_pool = self.pool("gpu", layer)
-        append_rows(keys, values, slots, k_pool, v_pool, stream=stream)
-        with on_stream(k_pool.device, stream):
+
+    def _mark_written(self, slots: torch.Tensor, layer: Optional[int], stream) -> None:
+        """The directory names the GPU tier for the blocks that these slots lie in."""
+        from .block_pool import on_stream
+        with on_stream(self.pool("gpu", layer)[0].device, stream):
             rows = self.directory() if layer is None else self.directory()[layer][None]
             blocks = torch.div(slots, self.block_size, rounding_mode="floor")
             blocks = torch.where((blocks >= 0) & (blocks < self.max_blocks), blocks, -1).to(torch.int32)
