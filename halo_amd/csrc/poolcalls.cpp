@@ -197,10 +197,11 @@ py::object attend(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, c
   const at::Device d = q.device();
   const int64_t N = q.size(0), H = q.size(1), D = q.size(2), B = lengths.dim() == 1 ? lengths.size(0) : 0;
   if (!on(k_pool, d) || k_pool.scalar_type() != q.scalar_type() || pool.D != D || (D != 64 && D != 128) || H < 1 ||
-      H > 0x7fffffff || H % pool.H_kv != 0 || N < 1 || N > 0x7fffffff || max_nodes < 1 || max_nodes > (chunk ? 0x7fffffff : kMaxNodes) || B < 1 ||
+      H > 0x7fffffff || H % pool.H_kv != 0 || N < 1 || N > 0x7fffffff || max_nodes < 1 || (!chunk && max_nodes > kMaxNodes) || B < 1 ||
       B > 0x7ffffff || !table_ok(table, B, d) || table.size(1) > 0x7fffffff || !ints(lengths, B, d) ||
       !ints(cu, B + 1, d))
     return py::none();
+  if (max_nodes > N) max_nodes = chunk ? N : max_nodes;  // no request has more rows than there are
   const int64_t per = 16 / q.element_size();
   if (q.stride(2) != 1 || q.stride(0) % per || q.stride(1) % per || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16)
     return py::none();

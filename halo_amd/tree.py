@@ -87,8 +87,9 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     nat.lib()
     if max_rows < 1:
         raise AssertionError(f"max_rows must be at least 1, got {max_rows}")
-    return _attend(q, k_pool, v_pool, block_table, lengths, cu_rows, "cu_rows", max_rows, None, True, scale, out, out_dtype,
-                   lse, return_lse, stream)
+    # (no request has more rows than there are)
+    return _attend(q, k_pool, v_pool, block_table, lengths, cu_rows, "cu_rows", min(max_rows, max(q.shape[0], 1)) if q.dim() else 1,
+                   None, True, scale, out, out_dtype, lse, return_lse, stream)
 
 
 def _attend(q, k_pool, v_pool, block_table, lengths, cu, cu_name, max_nodes, mask, chunk, scale, out, out_dtype, lse,

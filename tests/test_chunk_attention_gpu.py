@@ -94,8 +94,10 @@ def test_few_rows_are_the_causal_tree(dev, dtype):
     b = Batch(dev, lengths=[300, 0, 1000], nodes=[40, 215, 1], dtype=dtype)
     got, want = b.run(), tree_launch.Batch.run(b)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
-    got = b.run(max_rows=100000)
-    check(b, *got, b.exact())
+    for most in (100000, 2 ** 31 + 5, 2 ** 40):
+        got = b.run(max_rows=most)
+        check(b, *got, b.exact())
+        assert torch.equal(got[0], b.run(max_rows=most, stream=torch.cuda.current_stream())[0])
     b = Batch(dev, lengths=[300, 0, 1000], nodes=[40, 216, 1], dtype=dtype)
     check(b, *b.run(), b.exact())
     check(b, *tree_launch.Batch.run(b), b.exact())

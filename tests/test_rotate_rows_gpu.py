@@ -214,3 +214,49 @@ def test_slots_past_32_bit_offsets(dev):
         for i, s in enumerate(c.slots.tolist()):
             assert torch.equal(t[s // 64, :, s % 64], new[i])
     assert math.isclose(float((c.vp != 0).sum()), float((c.v != 0).sum()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("norm32", [False, True])
+def test_weights_that_begin_anywhere(dev, dtype, norm32):
+    c = Case(dev, N=23, D=128, dtype=dtype, norm32=norm32, pairs=True, R=48)
+    wide = torch.zeros(300, dtype=c.qn.dtype, device=dev)
+    wide[1:129], wide[133:261] = c.qn, c.kn
+    c.qn, c.kn = wide[1:129], wide[133:261]
+    c.check()
+
+
+def test_tables_of_cosines_that_begin_anywhere(dev):
+    c = Case(dev, N=9, R=32)
+    wide = [torch.zeros(c.cos.numel() + 3, device=dev) for _ in range(2)]
+    for w, t in zip(wide, (c.cos, c.sin)):
+        w[3:] = t.reshape(-1)
+    c.cos, c.sin = (w[3:].view(500, 16) for w in wide)
+    c.check()
+
+
+def test_a_stores_rows_stay_where_blocks_move(dev):
+    """TieredStorage.rotate_rows: the blocks written are the GPU tier's again, at once and after a move back."""
+    from halo_amd import TieredStorage
+    c = Case(dev, N=5, H=4, Hk=2, D=64, bs=4)
+    st = TieredStorage(tiers=["gpu", "dram"], num_layers=2, num_kv_heads=2, head_dim=64, block_size=4, dtype=BF16, device=dev,
+                       max_blocks=8)
+    for layer in range(2):
+        for b in range(8):
+            st.write_new_block(layer=layer, block=b, keys=torch.full((2, 4, 64), float(b), device=dev),
+                               values=torch.full((2, 4, 64), 100.0 + b, device=dev))
+        st.move_blocks(layer=layer, blocks=torch.arange(1, 8, dtype=torch.int32, device=dev), src="gpu", dst="dram")
+    slots = torch.tensor([9, -1, 10, 20, 2 ** 34], device=dev)
+    want = c.run()  # the same rows in another pool
+    rows = [c.kp[s // 4, :, s % 4].clone() for s in c.slots.tolist()]
+    q = st.rotate_rows(q=c.q, keys=c.k, values=c.v, positions=c.pos, cos=c.cos, sin=c.sin, slots=slots, layer=1, q_norm=c.qn,
+                       k_norm=c.kn)
+    assert torch.equal(q, want)
+    assert st.directory().tolist() == [[0] + [1] * 7, [0, 1, 0, 1, 1, 0, 1, 1]]
+    for again in (False, True):
+        for b, r, n in ((2, 1, 0), (2, 2, 2), (5, 0, 3)):
+            kb, vb = st.read_block(layer=1, block=b)
+            assert torch.equal(kb[:, r], rows[n]) and torch.equal(vb[:, r], c.v[n])
+        kb, _ = st.read_block(layer=1, block=2)
+        assert bool((kb[:, [0, 3]] == 2).all())
+        st.move_blocks(layer=1, blocks=torch.arange(8, dtype=torch.int32, device=dev), src="dram", dst="gpu")
