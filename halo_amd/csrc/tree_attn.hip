@@ -1200,11 +1200,13 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
     char* const knxt = stage ? sK0 : sK1;  // K(t+1)
     char* const vcur = stage ? sV1 : sV0;  // V(t)
     char* const vnxt = stage ? sV0 : sV1;  // receives V(t+1)
-    stage_next(kcur, vnxt);
-    if (active) {
+    if (!active) {
+      stage_next(kcur, vnxt);
+    } else {
       // Both blocks are issued in source order (a scheduling barrier after
       // each MFMA step): every MFMA's operand was read RING steps earlier, and
-      // the VALU work is spread evenly between the MFMAs.
+      // the VALU work is spread evenly between the MFMAs.  The next tiles are
+      // staged among them too (a prompt of 8192 rows: 565 us, and 578 with it in front).
       int kx = kx0, vx = vx0;
       asm volatile("" : "+v"(kx), "+v"(vx));
       uint4 kr[RING], vr[RING];
@@ -1217,6 +1219,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       for (int i = 0; i < NKS; ++i) {
         Sn[i & 1] = PMfma<DT>::run(kr[i % RING], qb[i >> 1], i < 2 ? pf32x16{} : Sn[i & 1]);
         if (i + RING < NKS) kr[i % RING] = kread(knxt, i + RING, kx);
+        else vr[i + RING - NKS] = vread(vcur, i + RING - NKS, vx);
+        if (i == NKS / 2) stage_next(kcur, vnxt);
 #pragma unroll
         for (int x = 0; x < EPM; x += 2) {
           const int w = (i * EPM + x) / 2, e = 2 * (w & 7);
@@ -1237,8 +1241,6 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 
       constexpr int MPM = 32 / NPV;  // score elements folded into the max per output MFMA
       float bm = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < RING; ++i) vr[i] = vread(vcur, i, vx);
 #pragma unroll
       for (int i = 0; i < NPV; ++i) {
         const uint32_t* pb = pw + 4 * (i / DB);
@@ -1436,9 +1438,11 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
 // for each workgroup, has no idle ones, but each reads other keys: 9 requests of
 // 1 to 2048 rows took 244 us where this takes 169.
 //
-// Measured, 32/8 heads of 128, bf16: 8192 rows from nothing 571 us (plan 8, walk
-// 560, an idle merge 5): 963 TFLOP/s of the causal half, where a large matrix product
-// reaches 1197; 601 rows behind 32768 in 352 (merge 12): 925.  The walk is the wide
+// Measured, 32/8 heads of 128, bf16, on the fastest card: 8192 rows from nothing 562
+// us (plan 8, walk 548, an idle merge 5): 978 TFLOP/s of the causal half, where a large
+// matrix product reaches 1197; 601 rows behind 32768 in 346 (merge 12): 941.  On the
+// slowest one 661 and 405.  Four stages with a barrier every second tile, and half of
+// the exponentials moved among the output products, took as long.  The walk is the wide
 // tree kernel's: per tile and SIMD the matrix cores are busy 45 % of the cycles, the
 // VALU nearly as long (exponentials), LDS reads half, and a barrier ends each tile.
 // Four waves of a workgroup and two workgroups a CU took 602 and 395 us.
