@@ -1078,19 +1078,36 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
     row.load(P, it, (t + 1) * KT + lane);
     return x;
   };
+  // Where a lane stages one or two rows (8 waves, or 4 with 64 channels) there are registers to keep
+  // the pieces that it stages and the operands' addresses: the VALU has as much to do as the matrix cores, and each
+  // instruction less in a tile counts (a prompt of 8192 rows: 541 us, 556 with the pieces alone, 565
+  // with neither).  The others work them out anew in each tile, from values that pass through a
+  // register of unknown value.
+  constexpr bool KEEP = NJ <= 2;
+  auto piece_of = [&](const char* base, bool is_v, int j) {
+    const int k = my_key + j * L::STEP, slot = lane % L::SL;
+    return base + ((slot ^ (is_v ? tree_vswz<RB>(k) : tree_kswz<RB>(k))) << 4);
+  };
+  const char* kept[2][KEEP ? NJ : 1];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      kept[0][j] = piece_of(kh, false, j);
+      kept[1][j] = piece_of(vh, true, j);
+      asm volatile("" : "+v"(kept[0][j]), "+v"(kept[1][j]));
+    }
+  }
   auto issue = [&](const Tile& x, const char* base, char* st, bool is_v) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int k = my_key + j * L::STEP, slot = lane % L::SL;
-      const int piece = slot ^ (is_v ? tree_vswz<RB>(k) : tree_kswz<RB>(k));
-      const char* from = base + (int64_t)x.pl[j] * 16 + (piece << 4);
+      const char* from = (KEEP ? kept[is_v][j % (KEEP ? NJ : 1)] : piece_of(base, is_v, j)) + (int64_t)x.pl[j] * 16;
       tree_dma(x.pl[j] == kNoRow ? reinterpret_cast<const char*>(tree_zeros) : from, st + (wave * NJ + j) * 1024);
     }
   };
   // Operand addresses: the key's LDS row and, xored, the piece.  lds_row takes
   // the bits of a key apart, so the rows of key step u are those of the first
-  // by a constant.  kx and vx pass through a register of unknown value in each
-  // tile: the xors are cheaper than keeping all their results.
+  // by a constant.  Where kx and vx pass through a register of unknown value in each
+  // tile, the xors are cheaper than keeping all their results (see KEEP).
   auto lds_row = [](int k) { return k / L::KEYS * L::KEYS + L::lds_row(k % L::KEYS); };
   const int kx0 = L::lds_row(qc % L::KEYS) * RB + qc / L::KEYS * L::KEYS * RB + ((hh ^ tree_kswz<RB>(qc)) << 4);
   auto kread = [&](const char* sk, int i, int kx) {  // step i: d-step i / 2, key block i % 2
@@ -1181,7 +1198,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 
   // Stages K(t+2) over K(t) and V(t+1), and moves on the places.
   auto stage_next = [&](char* kcur, char* vnxt) {
-    asm volatile("" : "+v"(my_key));  // the pieces are worked out anew in each tile
+    if (!KEEP) asm volatile("" : "+v"(my_key));
     if (t + 2 < t_end) issue(c2, kh, kcur, false);
     if (t + 1 < t_end) issue(c1, vh, vnxt, true);
     there = c1.there;
@@ -1208,7 +1225,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       // the VALU work is spread evenly between the MFMAs.  The next tiles are
       // staged among them too (a prompt of 8192 rows: 565 us, and 578 with it in front).
       int kx = kx0, vx = vx0;
-      asm volatile("" : "+v"(kx), "+v"(vx));
+      if (!KEEP) asm volatile("" : "+v"(kx), "+v"(vx));
       uint4 kr[RING], vr[RING];
 #pragma unroll
       for (int i = 0; i < RING; ++i) kr[i] = kread(knxt, i, kx);
@@ -1438,11 +1455,11 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
 // for each workgroup, has no idle ones, but each reads other keys: 9 requests of
 // 1 to 2048 rows took 244 us where this takes 169.
 //
-// Measured, 32/8 heads of 128, bf16, on the fastest card: 8192 rows from nothing 562
-// us (plan 8, walk 548, an idle merge 5): 978 TFLOP/s of the causal half, where a large
-// matrix product reaches 1197; 601 rows behind 32768 in 346 (merge 12): 941.  On the
-// slowest one 661 and 405.  Four stages with a barrier every second tile, and half of
-// the exponentials moved among the output products, took as long.  The walk is the wide
+// Measured, 32/8 heads of 128, bf16, on the fastest card: 8192 rows from nothing 541
+// us (plan 8, walk 527, an idle merge 5): 1016 TFLOP/s of the causal half, where a large
+// matrix product reaches 1197; 601 rows behind 32768 in 333 (merge 12): 978.  Cards
+// differ by a sixth.  Four stages with a barrier every second tile, and half of the
+// exponentials moved among the output products, took as long.  The walk is the wide
 // tree kernel's: per tile and SIMD the matrix cores are busy 45 % of the cycles, the
 // VALU nearly as long (exponentials), LDS reads half, and a barrier ends each tile.
 // Four waves of a workgroup and two workgroups a CU took 602 and 395 us.
