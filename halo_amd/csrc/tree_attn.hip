@@ -1453,16 +1453,17 @@ __global__ void __launch_bounds__(64 * MW) tree_merge_kernel(TreeParams P) {
 // a request's units lie at nearly the same keys, so the workgroups that walk them
 // at one time share K and V in L2.  One stream of all tiles in even shares, one
 // for each workgroup, has no idle ones, but each reads other keys: 9 requests of
-// 1 to 2048 rows took 244 us where this takes 169.
+// 1 to 2048 rows took 244 us where this took 169 (162 now).
 //
 // Measured, 32/8 heads of 128, bf16, on the fastest card: 8192 rows from nothing 541
 // us (plan 8, walk 527, an idle merge 5): 1016 TFLOP/s of the causal half, where a large
 // matrix product reaches 1197; 601 rows behind 32768 in 333 (merge 12): 978.  Cards
 // differ by a sixth.  Four stages with a barrier every second tile, and half of the
 // exponentials moved among the output products, took as long.  The walk is the wide
-// tree kernel's: per tile and SIMD the matrix cores are busy 45 % of the cycles, the
-// VALU nearly as long (exponentials), LDS reads half, and a barrier ends each tile.
-// Four waves of a workgroup and two workgroups a CU took 602 and 395 us.
+// tree kernel's: per tile and SIMD the matrix cores are busy 51 % of the cycles, the
+// VALU about as long (exponentials), LDS reads half, and a barrier ends each tile.
+// Four waves of a workgroup and two workgroups a CU took 602 and 395 us, when eight
+// waves took 571 and 352.
 // ---------------------------------------------------------------------------
 constexpr int kChunkMaxB = 4096, kPlanThreads = 1024, kCandidates = 32, kPlanUnits = 8192;
 // In tiles: what an item costs besides its tiles (its first tiles are waited for,
