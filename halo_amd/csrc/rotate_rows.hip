@@ -120,9 +120,7 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
   int64_t pos = P.pos64 ? reinterpret_cast<const int64_t*>(P.positions)[n] : reinterpret_cast<const int32_t*>(P.positions)[n];
   const bool there = pos >= 0 && pos < P.trig_rows;
   pos = there ? pos : 0;
-  float c[8], s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;  // channels that do not rotate
+  float c[8] = {}, s[8] = {};
   if (turns) {
     const float* cr = P.cos + pos * P.trig_stride + 8 * lane;
     const float* sr = P.sin + pos * P.trig_stride + 8 * lane;
@@ -165,7 +163,8 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] = a[i] * inv * wa[i], b[i] = b[i] * inv * wb[i];
     }
-    if (P.interleaved) {
+    // Channels behind R stay as they are: with c = 1 and s = 0 an infinity among them would make a neighbour NaN.
+    if (turns && P.interleaved) {
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
@@ -174,7 +173,7 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
         b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
         b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
       }
-    } else {
+    } else if (turns) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = a[i], y = b[i];

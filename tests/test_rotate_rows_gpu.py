@@ -260,3 +260,26 @@ def test_a_stores_rows_stay_where_blocks_move(dev):
         kb, _ = st.read_block(layer=1, block=2)
         assert bool((kb[:, [0, 3]] == 2).all())
         st.move_blocks(layer=1, blocks=torch.arange(8, dtype=torch.int32, device=dev), src="dram", dst="gpu")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("D,R", [(64, 32), (128, 16), (128, 112)])
+def test_channels_that_do_not_rotate_meet_no_others(dev, D, R, pairs, dtype):
+    """An infinity or NaN behind the first R channels stays where it is; the others, zeros of either sign too, are the input's."""
+    c = Case(dev, N=70 if D == 64 else 1400, D=D, R=R, dtype=dtype, pairs=pairs, norm=False, seed=R)  # few heads and many
+    want, rows = c.run(), lambda t: t[c.slots // 16, :, c.slots % 16]
+    k_want = rows(c.kp)
+    for t in (c.q, c.k):
+        t[..., R + 1], t[..., R + 4] = -0.0, 0.0
+        t[0:60:3, :, R + 3] = float("inf")
+        t[1:60:3, :, D - 1] = float("nan")
+        t[2:60:3, :, R + 9] = -float("inf")
+    out = c.run()
+    for got, x, ref in ((out, c.q, want), (rows(c.kp), c.k, k_want)):
+        tail = x[..., R:]
+        assert torch.equal(got[..., R:].nan_to_num(nan=7.0), tail.nan_to_num(nan=7.0))
+        assert torch.equal(torch.isnan(got[..., R:]), torch.isnan(tail))
+        there = ~torch.isnan(tail)
+        assert torch.equal(torch.signbit(got[..., R:])[there], torch.signbit(tail)[there])
+        assert torch.equal(got[..., :R], ref[..., :R])
