@@ -199,9 +199,6 @@ __device__ __forceinline__ bool tree_find_of(const TreeParams& P, int x, TreeIte
       }
       it.h = z;
       it.part = part + (it.rb * P.H_kv + it.h) * it.cuts;
-      it.seen = it.ctx;
-      it.t0 = (int)((int64_t)it.tiles * it.cut / it.cuts);
-      it.t1 = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
       return true;
     }
     base += lane_of(at, 63);
@@ -256,7 +253,11 @@ __device__ __forceinline__ bool find_cut_unit(const TreeParams& P, int x, TreeIt
 template <int KT, int R, bool CHUNK>
 __device__ __forceinline__ bool find_item(const TreeParams& P, TreeItem& it) {
   if constexpr (!CHUNK) {
-    return tree_find<KT, R, true>(P, blockIdx.x, it);
+    if (!tree_find<KT, R, true>(P, blockIdx.x, it)) return false;
+    it.seen = it.ctx;
+    it.t0 = (int)((int64_t)it.tiles * it.cut / it.cuts);
+    it.t1 = (int)((int64_t)it.tiles * (it.cut + 1) / it.cuts);
+    return true;
   } else {
     const int i = blockIdx.x / P.H_kv;
     if (i >= P.plan[0]) return false;
@@ -1084,23 +1085,30 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
   // with neither).  The others work them out anew in each tile, from values that pass through a
   // register of unknown value.
   constexpr bool KEEP = NJ <= 2;
-  auto piece_of = [&](const char* base, bool is_v, int j) {
+  // Where a lane stages eight rows (2 waves, 128 channels), the next tiles are staged in front of a step and not among its
+  // score products, and V is not read ahead of them: what the staging needs lives across the products otherwise, and 30
+  // SGPRs spill, not 8 (16 requests of 12 nodes over 8192 rows: 119.9 us, and 124.2 among them).  With four rows a lane
+  // and fewer the order gains or is even: 16 requests of 64 nodes over 8192 rows 222 us, 235 with the staging in
+  // front; of 24 nodes with 64 channels 67 and 70.5.
+  constexpr bool AMONG = NJ <= 4;
+  auto piece = [&](bool is_v, int j) {
     const int k = my_key + j * L::STEP, slot = lane % L::SL;
-    return base + ((slot ^ (is_v ? tree_vswz<RB>(k) : tree_kswz<RB>(k))) << 4);
+    return (slot ^ (is_v ? tree_vswz<RB>(k) : tree_kswz<RB>(k))) << 4;
   };
   const char* kept[2][KEEP ? NJ : 1];
   if constexpr (KEEP) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      kept[0][j] = piece_of(kh, false, j);
-      kept[1][j] = piece_of(vh, true, j);
+      kept[0][j] = kh + piece(false, j);
+      kept[1][j] = vh + piece(true, j);
       asm volatile("" : "+v"(kept[0][j]), "+v"(kept[1][j]));
     }
   }
   auto issue = [&](const Tile& x, const char* base, char* st, bool is_v) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const char* from = (KEEP ? kept[is_v][j % (KEEP ? NJ : 1)] : piece_of(base, is_v, j)) + (int64_t)x.pl[j] * 16;
+      const int64_t at = (int64_t)x.pl[j] * 16;
+      const char* from = KEEP ? kept[is_v][j % (KEEP ? NJ : 1)] + at : base + at + piece(is_v, j);
       tree_dma(x.pl[j] == kNoRow ? reinterpret_cast<const char*>(tree_zeros) : from, st + (wave * NJ + j) * 1024);
     }
   };
@@ -1217,13 +1225,13 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
     char* const knxt = stage ? sK0 : sK1;  // K(t+1)
     char* const vcur = stage ? sV1 : sV0;  // V(t)
     char* const vnxt = stage ? sV0 : sV1;  // receives V(t+1)
-    if (!active) {
-      stage_next(kcur, vnxt);
-    } else {
+    if (!AMONG || !active) stage_next(kcur, vnxt);
+    if (active) {
       // Both blocks are issued in source order (a scheduling barrier after
       // each MFMA step): every MFMA's operand was read RING steps earlier, and
       // the VALU work is spread evenly between the MFMAs.  The next tiles are
-      // staged among them too (a prompt of 8192 rows: 565 us, and 578 with it in front).
+      // staged among them too (a prompt of 8192 rows: 565 us, and 578 with it in front),
+      // but for the widths that AMONG names.
       int kx = kx0, vx = vx0;
       if (!KEEP) asm volatile("" : "+v"(kx), "+v"(vx));
       uint4 kr[RING], vr[RING];
@@ -1236,8 +1244,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       for (int i = 0; i < NKS; ++i) {
         Sn[i & 1] = PMfma<DT>::run(kr[i % RING], qb[i >> 1], i < 2 ? pf32x16{} : Sn[i & 1]);
         if (i + RING < NKS) kr[i % RING] = kread(knxt, i + RING, kx);
-        else vr[i + RING - NKS] = vread(vcur, i + RING - NKS, vx);
-        if (i == NKS / 2) stage_next(kcur, vnxt);
+        else if (AMONG) vr[i + RING - NKS] = vread(vcur, i + RING - NKS, vx);
+        if (AMONG && i == NKS / 2) stage_next(kcur, vnxt);
 #pragma unroll
         for (int x = 0; x < EPM; x += 2) {
           const int w = (i * EPM + x) / 2, e = 2 * (w & 7);
@@ -1258,6 +1266,10 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 
       constexpr int MPM = 32 / NPV;  // score elements folded into the max per output MFMA
       float bm = -INFINITY;
+      if (!AMONG) {
+#pragma unroll
+        for (int i = 0; i < RING; ++i) vr[i] = vread(vcur, i, vx);
+      }
 #pragma unroll
       for (int i = 0; i < NPV; ++i) {
         const uint32_t* pb = pw + 4 * (i / DB);
