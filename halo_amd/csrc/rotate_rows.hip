@@ -87,8 +87,10 @@ __device__ __forceinline__ void weights8(const void* at, bool f32, int i, float*
 // reads and writes lie far apart.  Few heads are bound by the chain position ->
 // cosines -> store, which one head a group has shortest: 768 heads 5.0 us with one
 // and 6.3 with three, 12288 heads 6.2 and 6.8, 49152 heads 11.6 and 9.2.
+// PART: R < D, and channels behind R stay as they are (with c = 1 and s = 0 an infinity
+// among them would make a neighbour NaN); where all turn that test cost 2 us of 171.
 constexpr int64_t kRotFew = 16384;
-template <int DT, int D, int UB>
+template <int DT, int D, int UB, bool PART>
 __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P) {
   constexpr int G = D / 16;  // lanes of a head
   constexpr int ES = DT == HALO_F32 ? 4 : 2, PIECES = ES / 2;
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
   if (n >= P.N) return;
   const int part = unit - n * P.parts, lane = threadIdx.x & (G - 1);
   const int R = P.R, heads = P.H + 2 * P.H_kv;
-  const bool turns = 16 * lane < R, halves = turns && !P.interleaved;
+  const bool turns = !PART || 16 * lane < R, halves = turns && !P.interleaved;
   const int ca = halves ? 8 * lane : 16 * lane, cb = halves ? R / 2 + 8 * lane : 16 * lane + 8;
   u32x4 w[UB][2 * PIECES];
 #pragma unroll
@@ -163,8 +165,8 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] = a[i] * inv * wa[i], b[i] = b[i] * inv * wb[i];
     }
-    // Channels behind R stay as they are: with c = 1 and s = 0 an infinity among them would make a neighbour NaN.
-    if (turns && P.interleaved) {
+    if (PART && !turns) {
+    } else if (P.interleaved) {
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const float a0 = a[i], a1 = a[i + 1], b0 = b[i], b1 = b[i + 1];
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kRotThreads) rotate_rows_kernel(RotateParams P
         b[i] = b0 * c[4 + i / 2] - b1 * s[4 + i / 2];
         b[i + 1] = b1 * c[4 + i / 2] + b0 * s[4 + i / 2];
       }
-    } else if (turns) {
+    } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = a[i], y = b[i];
@@ -248,17 +250,23 @@ extern "C" int halo_rotate_rows(const halo_block_pool* pool, const void* q, int6
   const int per = kRotThreads / (pool->D / 16);
   const dim3 grid((unsigned)(((int64_t)p.parts * N + per - 1) / per)), block(kRotThreads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+#define HALO_ROTATE_PART(DTV, DV, UBV)                                                                                 \
+  do {                                                                                                                 \
+    if (R < DV) hipLaunchKernelGGL((rotate_rows_kernel<DTV, DV, UBV, true>), grid, block, 0, st, p);                   \
+    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, DV, UBV, false>), grid, block, 0, st, p);                         \
+  } while (0)
 #define HALO_ROTATE(DTV)                                                                                               \
   do {                                                                                                                 \
-    if (pool->D == 128 && ub == 3) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128, 3>), grid, block, 0, st, p);       \
-    else if (pool->D == 128) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 128, 1>), grid, block, 0, st, p);             \
-    else if (ub == 3) hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64, 3>), grid, block, 0, st, p);                     \
-    else hipLaunchKernelGGL((rotate_rows_kernel<DTV, 64, 1>), grid, block, 0, st, p);                                  \
+    if (pool->D == 128 && ub == 3) HALO_ROTATE_PART(DTV, 128, 3);                                                      \
+    else if (pool->D == 128) HALO_ROTATE_PART(DTV, 128, 1);                                                            \
+    else if (ub == 3) HALO_ROTATE_PART(DTV, 64, 3);                                                                    \
+    else HALO_ROTATE_PART(DTV, 64, 1);                                                                                 \
   } while (0)
   if (pool->dtype == HALO_F32) HALO_ROTATE(HALO_F32);
   else if (pool->dtype == HALO_BF16) HALO_ROTATE(HALO_BF16);
   else HALO_ROTATE(HALO_F16);
 #undef HALO_ROTATE
+#undef HALO_ROTATE_PART
   HALO_CHECK_HIP(hipGetLastError());
   return HALO_OK;
 }
