@@ -23,7 +23,7 @@ using at::Tensor;
 
 namespace {
 
-constexpr int kMaxNodes = 512, kMaxPath = 64;
+constexpr int kMaxNodes = 512, kMaxPath = 64, kPlanRequests = 4096;
 
 struct Entries {
   decltype(&halo_update_block_tables) update;
@@ -202,6 +202,8 @@ py::object attend(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, c
       !ints(cu, B + 1, d))
     return py::none();
   if (max_nodes > N) max_nodes = chunk ? N : max_nodes;  // no request has more rows than there are
+  // the plan of chunks holds kPlanRequests; rows of more are nodes of trees without masks
+  if (B > kPlanRequests && max_nodes <= kMaxNodes) chunk = false;
   const int64_t per = 16 / q.element_size();
   if (q.stride(2) != 1 || q.stride(0) % per || q.stride(1) % per || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16)
     return py::none();

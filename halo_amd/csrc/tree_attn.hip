@@ -1841,7 +1841,25 @@ size_t chunk_bytes(const ChunkShape& s, int D) {
 // requests: 48 rows each 46 and 48, 96 rows 85 and 77, 256 rows 129 and 116 (from
 // nothing 14 and 23, 27 and 25, 44 and 37).
 constexpr int kChunkTreeRows = 256;
+// In 16 bits the tree kernels too where no request has more than this many rows of
+// query heads: a unit of 256 would be half empty, and few of its workgroup's waves
+// have rows.  32/8 heads of 128, bf16, behind 0, 200 and 2000 rows, tree and chunk
+// kernels: 257 requests of 1 row 46 and 99, 71 and 138, 385 and 490 us; 512 of 8
+// rows 92 and 175, 157 and 262, 741 and 890; behind 0, 500 and 4000: 32 of 32 rows
+// (128 of heads) 12 and 27, 36 and 42, 128 and 127; 128 of 32 36 and 63, 106 and
+// 131, 413 and 458.  Above: 192 rows of heads 13.5 to 577 us where the others take
+// 23 to 569, 256 18 to 656 and 23 to 652, but 160 of 40/1 heads 355 and 282, 384 of
+// 8 requests behind 4000 122 and 97.  28/4 heads 11 and 27, 63 and 68 (112 rows of
+// heads), 8/8 31 and 52 (32), 64 channels 10 and 28, 59 and 84 (128).  From about
+// 3000 requests of a row and no context on the search for an item costs more (4000:
+// 1776 and 1215, behind 2000 rows 5639 and 6439).  fp32 has units of 32 rows in both,
+// and neither is ahead throughout: 64 of 16 rows from nothing 57 and 68, 1024 of 4
+// 530 and 379.
+constexpr int kChunkTreeHeadRows = 128;
 int tree_rows_of(int N, int max_rows) { return max_rows < N ? max_rows : N; }
+bool short_chunks(int dtype, int N, int rep, int max_rows) {
+  return dtype != HALO_F32 && (int64_t)tree_rows_of(N, max_rows) * rep <= kChunkTreeHeadRows;
+}
 
 }  // namespace
 
@@ -1849,6 +1867,10 @@ extern "C" size_t halo_chunk_workspace_size(int dtype, int B, int N, int H, int 
   if (N <= 0 || max_rows <= 0) return 0;
   if (N <= kChunkTreeRows) return halo_tree_workspace_size(dtype, B, H, H_kv, D, max_keys, tree_rows_of(N, max_rows));
   if (!tree_sizes_ok(B, H, H_kv, D, max_keys, 1)) return 0;
+  if (short_chunks(dtype, N, H / H_kv, max_rows)) {
+    const size_t need = halo_tree_workspace_size(dtype, B, H, H_kv, D, max_keys, tree_rows_of(N, max_rows));
+    return need < 16 ? 16 : need;
+  }
   return chunk_bytes(chunk_shape(dtype, B, N, H, H_kv, D), D);
 }
 
@@ -1873,10 +1895,14 @@ extern "C" int halo_chunk_attn(const halo_block_pool* pool, const void* q, int64
   // the units' number in 31 bits whatever cu_rows holds
   HALO_CHECK_ARG((s.units * p.H_kv + s.partials) < (1ll << 31) && s.units * B < (1ll << 31), "too many rows and heads");
   HALO_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace missing or not 16-byte aligned");
-  if (workspace_bytes < chunk_bytes(s, D)) {
+  if (workspace_bytes < halo_chunk_workspace_size(dtype, B, N, H, p.H_kv, D, (int64_t)W * pool->block_size, max_rows)) {
     set_error("workspace too small");
     return HALO_E_WORKSPACE;
   }
+  if (short_chunks(dtype, N, p.rep, max_rows))
+    return halo_tree_attn(pool, q, q_stride_n, q_stride_h, N, H, table, table_stride, B, W, lengths, cu_rows,
+                          tree_rows_of(N, max_rows), nullptr, 0, scale, out, out_stride_n, out_stride_h, out_dtype, lse,
+                          workspace, workspace_bytes, stream);
   const int NW = s.R / 32;
   p.part_o = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + s.partials * NW * 32 * (D / 4));

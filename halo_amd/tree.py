@@ -23,6 +23,8 @@ from . import _native as nat
 from . import block_pool as pool_calls
 from .block_pool import _DTYPES, MAX_NODES, check_ints, check_table, on_stream, overlap, pack_pool
 
+PLAN_REQUESTS = 4096  # requests that the plan of a call of chunks holds
+
 
 def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                    lengths: torch.Tensor, cu_nodes: torch.Tensor, *, max_nodes: int,
@@ -77,8 +79,8 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     (``append_rows``, ``rotate_rows``).  Requests may have any numbers of new
     rows, none and one among them; ``max_rows`` is the largest (further rows are
     left out).  The lengths are read on the device, so a captured call follows
-    them.  Calls of more than 256 rows in all have at most 4096 requests; N times
-    H / H_kv stays below 2^30."""
+    them.  Calls of more than 4096 requests have at most 512 rows each, or 256 in
+    all; N times H / H_kv stays below 2^30."""
     if pool_calls.calls is not None and stream is None and out_dtype is None:
         r = pool_calls.calls.chunk_attention(q, k_pool, v_pool, block_table, lengths, cu_rows, max_rows, scale, out, lse,
                                              return_lse)
@@ -87,9 +89,12 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     nat.lib()
     if max_rows < 1:
         raise AssertionError(f"max_rows must be at least 1, got {max_rows}")
-    # (no request has more rows than there are)
-    return _attend(q, k_pool, v_pool, block_table, lengths, cu_rows, "cu_rows", min(max_rows, max(q.shape[0], 1)) if q.dim() else 1,
-                   None, True, scale, out, out_dtype, lse, return_lse, stream)
+    if q.dim():  # no request has more rows than there are
+        max_rows = min(max_rows, max(q.shape[0], 1))
+    # the plan of chunks holds PLAN_REQUESTS; rows of more are nodes of trees without masks
+    chunk = lengths.numel() <= PLAN_REQUESTS or max_rows > MAX_NODES
+    return _attend(q, k_pool, v_pool, block_table, lengths, cu_rows, "cu_rows", max_rows, None, chunk, scale, out, out_dtype, lse,
+                   return_lse, stream)
 
 
 def _attend(q, k_pool, v_pool, block_table, lengths, cu, cu_name, max_nodes, mask, chunk, scale, out, out_dtype, lse,

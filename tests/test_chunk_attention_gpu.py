@@ -273,3 +273,41 @@ def test_huge_scores(dev):
         top = float(b.args["v_pool"].max()) * (1 + 2 * HALF[dtype]) * (1 + 8000 * U)
         assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
         assert float(out.min()) >= 0 and float(out.max()) <= top
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,Hk,most", [(8, 2, 32), (8, 2, 33), (8, 2, 1), (28, 4, 18), (28, 4, 19), (8, 8, 128), (8, 8, 130), (40, 1, 3),
+                                       (40, 1, 4)])
+def test_batches_of_short_chunks(dev, dtype, H, Hk, most):
+    """Around 128 rows of query heads a request, where 16-bit calls change kernels: also empty requests and single rows."""
+    B = 1 + 2000 // (8 * most) * 8
+    rows = [most if b % 3 == 0 else (b * 5) % (most + 1) for b in range(B)]
+    rows[0] += max(0, 257 - sum(rows))  # more than 256 in all
+    b = Batch(dev, lengths=[(b * 37) % 300 for b in range(B)], nodes=rows, H=H, Hk=Hk, dtype=dtype, seed=most)
+    got = b.run(max_rows=max(rows))
+    check(b, *got, b.exact())
+    again = b.run(max_rows=max(rows), stream=torch.cuda.current_stream())
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    if dtype != F32 and max(rows) * (H // Hk) <= 128:
+        want = tree_launch.Batch.run(b)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("most", [1, 3, 512])
+def test_more_requests_than_a_plan_holds(dev, dtype, most):
+    B = 4999
+    rows = [most if b in (7, 4500) else (b * 7) % (min(most, 3) + 1) for b in range(B)]
+    b = Batch(dev, lengths=[(b * 13) % 50 for b in range(B)], nodes=rows, H=4, Hk=2, dtype=dtype, seed=most)
+    got = b.run()
+    check(b, *got, b.exact())
+    again = b.run(stream=torch.cuda.current_stream())
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+def test_many_requests_of_many_rows_are_refused(dev):
+    b = Batch(dev, lengths=[1] * 4097, nodes=[513] + [0] * 4096, H=4, Hk=2, seed=1)
+    for kw in ({}, dict(stream=torch.cuda.current_stream())):
+        with pytest.raises(Exception, match="4096"):
+            b.run(**kw)
+    b.run(max_rows=512)
