@@ -246,6 +246,19 @@ def test_tree_layout_leaves_padding_and_further_nodes(dev):
     assert depth.tolist() == [0, 1, 2, 0, 1, 2, 3, 78, 78, 78]
 
 
+def test_tree_layout_of_any_cu_nodes(dev):
+    """Ranges whose difference does not fit 32 bits are empty, or cut at the nodes there are."""
+    import halo_amd
+    parents = _i32([-1, 0, 1, 0, 2, 9, 9], dev)
+    for cu, there in (([-7, 2 ** 30, -2 ** 31, 2 ** 31 - 1, 0], True), ([2 ** 31 - 1, -2 ** 31, 2 ** 30, -5, -1], True),
+                      ([7, 4, 3, 2, -2 ** 31], False)):
+        mask = torch.full((7, 1), 77, dtype=torch.int64, device=dev)
+        depth = torch.full((7,), 78, dtype=torch.int32, device=dev)
+        halo_amd.tree_layout(parents, _i32(cu, dev), max_nodes=5, mask=mask, depth=depth)
+        assert mask[:, 0].tolist() == ([1, 3, 7, 9, 23] if there else [77] * 5) + [77] * 2
+        assert depth.tolist() == ([0, 1, 2, 1, 3] if there else [78] * 5) + [78] * 2
+
+
 # ---------------------------------------------------------------- accepted paths
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

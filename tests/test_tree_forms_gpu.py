@@ -49,3 +49,31 @@ def test_a_request_alone_and_among_others(dev, dtype):
         exact = one.exact()
         check(one, *one.run(), exact)
         check(one, out, lse, exact, rows=slice(lo, hi))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("masks", [False, True])
+@pytest.mark.parametrize("nodes", [5, 20, 70])
+def test_cu_nodes_of_any_values(dev, dtype, masks, nodes):
+    """Requests have the rows from max(cu[b], 0) up to cu[b + 1], max_nodes at most, also where their difference does not fit
+    32 bits; other rows of out and lse, and what lies around them, stay as they are."""
+    import halo_amd
+    N, H, D = 3 * nodes, 8, 64
+    one = tree_launch.Batch(dev, lengths=[50], nodes=[nodes], H=H, Hk=2, D=D, bs=16, dtype=dtype, seed=nodes, masks=masks)
+    g = torch.Generator().manual_seed(nodes)
+    a = dict(one.args, block_table=one.args["block_table"].repeat(4, 1), lengths=one.args["lengths"].repeat(4),
+             q=torch.cat([one.args["q"], torch.randn(2 * nodes, H, D, generator=g).to(dtype).to(dev)]))
+    if masks:
+        a["mask"] = torch.cat([a["mask"], torch.zeros(2 * nodes, a["mask"].shape[1], dtype=torch.int64, device=dev)])
+    for cu, there in (([-7, 2 ** 30, -2 ** 31, 2 ** 31 - 1, 0], True), ([2 ** 31 - 1, -2 ** 31, 2 ** 30, -5, -1], True),
+                      ([-2 ** 31, 2 ** 31 - 1, -2 ** 31, -2 ** 31, -2 ** 31], True), ([N, 4, 3, 2, -2 ** 31], False)):
+        a["cu_nodes"] = torch.tensor(cu, dtype=torch.int32, device=dev)
+        held = torch.full((N + 20, H, D), 9.0, dtype=dtype, device=dev)
+        held_lse = torch.full((N + 20, H), 7.0, device=dev)
+        out, lse = held[10:N + 10], held_lse[10:N + 10]
+        halo_amd.tree_attention(**a, max_nodes=nodes, out=out, lse=lse, return_lse=True)
+        if there:
+            check(one, out[:nodes], lse[:nodes], one.exact())
+        rest = torch.ones(N + 20, dtype=torch.bool, device=dev)
+        rest[10:10 + nodes * there] = False
+        assert bool((held[rest] == 9).all()) and bool((held_lse[rest] == 7).all())
