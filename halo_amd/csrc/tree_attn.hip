@@ -1592,7 +1592,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(ChunkPlanParam
     const int c0 = cut + scan(cuts > 1, cut_all);
     const int lo = cuts > 0 ? max(P.cu[b], 0) : 0;
 #pragma unroll 1
-    for (int k = 0; k < cuts; ++k) {  // t < 2^25, k <= 32
+    for (int k = 0; k < cuts; ++k) {  // t < 2^26 (keys of 32 in fp32), k <= 32
       int4* it = C.items + (int64_t)(i0 + k) * kItemInts4;
       it[0] = make_int4(b, rb, k, cuts);
       it[1] = make_int4(t * k / cuts, t * (k + 1) / cuts, p0, lo);

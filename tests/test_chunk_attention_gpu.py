@@ -7,6 +7,8 @@ of |v|, d the largest scale * sum |q_d k_d|, T the attended rows:
   |lse - exact| <= (D + 6) u d + (T + 8) u + 4 u |lse|"""
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -311,3 +313,81 @@ def test_many_requests_of_many_rows_are_refused(dev):
         with pytest.raises(Exception, match="4096"):
             b.run(**kw)
     b.run(max_rows=512)
+
+
+def part_of(b, request, lo, n):
+    """Rows lo .. lo + n - 1 of q as those of one request, alone."""
+    c = copy.copy(b)
+    c.lengths, c.nodes = [b.lengths[request]], [n]
+    c.args = {**b.args, "q": b.args["q"][lo:lo + n], "block_table": b.args["block_table"][request:request + 1]}
+    return c
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_cu_rows_of_any_values_give_each_request_its_rows(dev, dtype):
+    """Request b has the rows from max(cu[b], 0) up to cu[b + 1], max_rows at most: rows of one request are the definition's,
+    rows of none, and what lies around out and lse, stay as they are."""
+    b = Batch(dev, lengths=[10, 20, 30, 40], nodes=[600, 5, 600, 5], dtype=dtype)
+    N, H, D = 1210, b.H, b.D
+    for cu in ([0, 1210, 0, 1210, 5000], [0, 600, 300, 1210, 1210], [-7, 2 ** 30, -2 ** 31, 2 ** 31 - 1, 0], [1210, 5, 4, 3, 2],
+               [0, 300, 301, 900, 2 ** 31 - 1], [-2 ** 31, 1, 1, 700, 1209]):
+        b.args["cu_nodes"].copy_(torch.tensor(cu))
+        for most in (600, 300):
+            held = torch.full((N + 20, H, D), 9.0, dtype=dtype, device=dev)
+            held_lse = torch.full((N + 20, H), 7.0, device=dev)
+            b.run(out=held[10:N + 10], lse=held_lse[10:N + 10], max_rows=most)
+            out, lse = held[10:N + 10], held_lse[10:N + 10]
+            owners = torch.zeros(N, dtype=torch.int64)
+            mine = []
+            for r in range(4):
+                lo = max(cu[r], 0)
+                n = max(min(min(max(cu[r + 1], 0), N) - lo, most), 0)
+                mine.append((lo, n))
+                owners[lo:lo + n] += 1
+            none = torch.cat([torch.ones(10, dtype=torch.bool), owners == 0, torch.ones(10, dtype=torch.bool)]).to(dev)
+            assert bool((held[none] == 9).all()) and bool((held_lse[none] == 7).all())
+            assert bool(torch.isfinite(held).all()) and not bool((lse[(owners > 0).to(dev)] == 7).all(1).any())
+            for r, (lo, n) in enumerate(mine):
+                alone = (owners[lo:lo + n] == 1).to(dev)
+                if n and bool(alone.any()):
+                    c = part_of(b, r, lo, n)
+                    check(c, out[lo:lo + n][alone], lse[lo:lo + n][alone], [x[alone] for x in c.exact()])
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_means_of_huge_scores(dev, dtype):
+    """As test_huge_scores, V in [1, 2]: out is no less than 1 and no more than 2 but for the weights' and out's roundings, and
+    lse is the float64 one within the bound above."""
+    b = Batch(dev, lengths=[700], nodes=[600], seed=3, dtype=dtype)
+    for t in (b.args["q"], b.args["k_pool"]):
+        t.mul_(2.0 ** 13).clamp_(-60000, 60000)
+    v = b.args["v_pool"]
+    v.copy_(1 + (v.abs() / v.abs().max()).clamp(max=1))
+    up = -8 if dtype == F16 else -3
+    out, lse = b.run(scale=2.0 ** up)
+    c = part_of(b, 0, 0, 600)
+    c.args["q"] = c.args["q"].float() * 2.0 ** up * 8  # the default scale is 1 / 8
+    _, z, _, dots = c.exact()
+    err = 2 * HALF[dtype] + 8000 * U
+    assert float(out.min()) >= 1 - err and float(out.max()) <= 2 * (1 + err)
+    assert bool(((lse.double() - z).abs() <= (64 + 6) * U * dots + (1300 + 8) * U + 4 * U * z.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_queries_of_any_strides(dev, dtype):
+    b = Batch(dev, lengths=[77, 0], nodes=[520, 9], dtype=dtype, seed=7)
+    want, q = b.run(), b.args["q"]
+    pad = torch.nn.functional.pad
+    for form in (q.transpose(0, 1).contiguous().transpose(0, 1), torch.cat([q, q], 2)[..., :64], pad(q, (1, 5))[..., 1:65],
+                 pad(q, (8, 8))[..., 8:72], q.repeat_interleave(2, 2)[..., ::2], q.repeat_interleave(2, 1)[:, ::2]):
+        assert torch.equal(form, q) and form.stride() != q.stride()
+        got = b.run(q=form)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_more_units_than_the_plan_keeps(dev):
+    """fp32 has units of 32 rows; from 8192 units on the plan works the first ones out anew."""
+    rows = [3000, 1, 2601, 0, 1000]
+    b = Batch(dev, lengths=[40, 500, 0, 9, 300], nodes=rows, H=40, Hk=1, D=64, dtype=F32, seed=11)
+    assert sum(-(-n * 40 // 32) for n in rows) > 8192
+    check(b, *b.run(), b.exact())
