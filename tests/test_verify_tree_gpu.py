@@ -316,3 +316,60 @@ def test_replayed_on_another_stream_and_side_by_side(dev):
     torch.cuda.synchronize()
     for c, r in zip(cases, got):
         c.check(r)
+
+
+@pytest.mark.parametrize("draft", ["none", "with", "without"])
+@pytest.mark.parametrize("V", [131073, 151936, 2 ** 20 + 77])
+def test_vocabularies_of_several_narrowing_rounds(dev, V, draft):
+    """More than 131072 tokens: the range that holds the last token is found in two rounds and more, each with the rejected
+    tokens left out."""
+    c = Case(dev, nodes=[5, 3], V=V, draft=draft, seed=V, spread=3.0)
+    c.check()
+    c.accept = 1 - c.accept * 2.0 ** -10  # most children are rejected
+    for u in (0.0, 0.25, 0.999, 1 - 2.0 ** -24):
+        c.sample.fill_(u)
+        c.check()
+    c.probs[:, :-40] = 0  # everything in the last range
+    for u in (0.0, 0.5, 1 - 2.0 ** -24):
+        c.sample.fill_(u)
+        c.check()
+
+
+@pytest.mark.parametrize("draft", ["none", "with", "without"])
+def test_a_vocabulary_near_the_largest(dev, draft):
+    c = Case(dev, nodes=[2], V=2 ** 24 - 5, draft=draft, dtype=torch.bfloat16, seed=1, fan=1)
+    for u in (0.0, 0.7, 1 - 2.0 ** -24):
+        c.sample.fill_(u)
+        c.check()
+    c.accept.fill_(1 - 2.0 ** -24)
+    c.probs[:, :2 ** 23] = 0
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_rejected_tokens_whose_marks_are_the_same(dev, dtype):
+    """Without draft probabilities rejected tokens are found by marks that tokens 131072 apart share."""
+    V, far = 3 * 131072 + 11, 131072
+    kids = [40, 40 + far, 41, 47 + 2 * far, 3 * far + 3, 9 + far, V - 1, 40, far - 1]
+    c = Case(dev, nodes=[1 + len(kids)] * 4, V=V, draft="none", dtype=dtype, seed=6)
+    c.probs[:] = 0
+    near = sorted({min(max(t + d, 0), V - 1) for t in kids for d in range(-9, 10)} | {t % far for t in kids} | {t % far + far for t in kids})
+    g = torch.Generator().manual_seed(7)
+    for b in range(4):
+        lo = c.cu[b]
+        c.probs[lo:lo + 10, near] = (torch.rand(10, len(near), generator=g) / len(near)).to(dtype)
+        c.parents[lo + 1:lo + 10], c.tokens[lo + 1:lo + 10] = [0] * 9, kids
+    c.accept.fill_(1 - 2.0 ** -24)
+    for u in (0.0, 0.1, 0.35, 0.6, 0.85, 1 - 2.0 ** -24):
+        c.sample = torch.tensor([u, u * 0.99, u * 0.9, u * 0.7])
+        assert c.check() == [1] * 4
+
+
+@pytest.mark.parametrize("draft", ["none", "with", "without"])
+@pytest.mark.parametrize("share", [0.25, 0.9, 1.5])
+def test_rows_that_do_not_sum_to_one(dev, draft, share):
+    """Z begins at 1 whatever p sums to; without draft probabilities it is 1 less the rejected tokens' p, not the sum of what
+    is left."""
+    c = Case(dev, nodes=[12, 30, 7, 25], V=90, fan=5, draft=draft, seed=12, noise=1.5)
+    c.probs *= share
+    c.check()
