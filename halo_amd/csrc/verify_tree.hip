@@ -14,9 +14,10 @@
 // max(a - b - c, 0) for b, c >= 0, so one number says what is left:
 //   R_j(v) = max(p(v) - S_j q(v), 0), 0 for rejected tokens,
 //   S_{j+1} = S_j + Z_j, or + Z_j / (1 - Q_j) without replacement,
-// and without draft probabilities R is p without the rejected tokens.  Where no
-// child is accepted the next token is the first v whose R(0) + .. + R(v)
-// exceeds u sum R.  Sums and products are in 64 bits: a sum of 100 000 terms in
+// and without draft probabilities R is p without the rejected tokens, and Z_j is
+// 1 less their p: no pass over the row, whose sum differs only by what the rounded
+// p lack of 1.  Where no child is accepted the next token is the first v whose
+// R(0) + .. + R(v) exceeds u sum R.  Sums and products are in 64 bits: a sum of 100 000 terms in
 // 32 would move the borders between tokens.
 //
 // The reference drafts no tokens; this is the library's own.

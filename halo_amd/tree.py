@@ -79,8 +79,8 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     (``append_rows``, ``rotate_rows``).  Requests may have any numbers of new
     rows, none and one among them; ``max_rows`` is the largest (further rows are
     left out).  The lengths are read on the device, so a captured call follows
-    them.  Calls of more than 4096 requests have at most 512 rows each, or 256 in
-    all; N times H / H_kv stays below 2^30."""
+    them.  Calls of more than 4096 requests have at most 512 rows each; N times
+    H / H_kv stays below 2^30."""
     if pool_calls.calls is not None and stream is None and out_dtype is None:
         r = pool_calls.calls.chunk_attention(q, k_pool, v_pool, block_table, lengths, cu_rows, max_rows, scale, out, lse,
                                              return_lse)

@@ -43,13 +43,16 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, cu_nodes: torch.Ten
     taken as chosen (the draft's likeliest tokens, say).
 
     From node 0 on, the children of the node reached are tried in the order of
-    their numbers.  With R what is left of the node's probabilities p, of sum Z, at
-    first p and 1, a child with token t drawn from q is accepted where
+    their numbers.  With R what is left of the node's probabilities p, at first p,
+    and Z = 1 at first, a child with token t drawn from q is accepted where
     ``accept * q[t] * Z < R[t]`` and the walk goes on from it; else R becomes
-    ``max(R - Z q, 0)``, without t, and Z its sum.  Where no child is accepted, or
-    the path has ``max_path`` (<= 64; default min(max_nodes, 64)) nodes, the next
-    token is the first one at which the running sum of R exceeds ``sample`` times
-    its whole (of p, should R be 0).
+    ``max(R - Z q, 0)``, without t, and Z its sum.  Without draft probabilities a
+    child is accepted where ``accept * Z < R[t]``; else t leaves R, and Z falls by
+    ``p[t]`` (1 less the rejected tokens' p, also where p does not sum to 1, as
+    rounded rows do not).  Where no child is accepted, or the path has ``max_path``
+    (<= 64; default min(max_nodes, 64)) nodes, the next token is the first one at
+    which the running sum of R exceeds ``sample`` times its whole (of p, should R
+    be 0).
 
     ``max_nodes`` (<= 512) is the largest tree, further nodes are left out; V <=
     2^24.  Tokens outside [0, V) are not accepted; NaN and negative probabilities
