@@ -1847,18 +1847,25 @@ constexpr int kChunkTreeRows = 256;
 // kernels: 257 requests of 1 row 46 and 99, 71 and 138, 385 and 490 us; 512 of 8
 // rows 92 and 175, 157 and 262, 741 and 890; behind 0, 500 and 4000: 32 of 32 rows
 // (128 of heads) 12 and 27, 36 and 42, 128 and 127; 128 of 32 36 and 63, 106 and
-// 131, 413 and 458.  Above: 192 rows of heads 13.5 to 577 us where the others take
-// 23 to 569, 256 18 to 656 and 23 to 652, but 160 of 40/1 heads 355 and 282, 384 of
-// 8 requests behind 4000 122 and 97.  28/4 heads 11 and 27, 63 and 68 (112 rows of
-// heads), 8/8 31 and 52 (32), 64 channels 10 and 28, 59 and 84 (128).  From about
-// 3000 requests of a row and no context on the search for an item costs more (4000:
-// 1776 and 1215, behind 2000 rows 5639 and 6439).  fp32 has units of 32 rows in both,
-// and neither is ahead throughout: 64 of 16 rows from nothing 57 and 68, 1024 of 4
-// 530 and 379.
+// 131, 413 and 458.  28/4 heads 11 and 27, 63 and 68 (112 rows of heads), 8/8 31 and
+// 52 (32), 64 channels 10 and 28, 59 and 84 (128).  From about 3000 requests of a row
+// and no context on the search for an item costs more (4000: 1776 and 1215, behind
+// 2000 rows 5639 and 6439).  fp32 has units of 32 rows in both, and neither is ahead
+// throughout: 64 of 16 rows from nothing 57 and 68, 1024 of 4 530 and 379.
 constexpr int kChunkTreeHeadRows = 128;
+// Up to one unit a request, where the call has no more than this many rows of query
+// heads: 8 requests of 48 rows (192 of heads) from nothing 13.5 and 22.7 us, behind
+// 4000 rows 63.7 and 63.2; 32 of 64 (256, 8192 in all) 25 and 33, 163 and 175; 64 of
+// 32 with 28/4 heads (14336 in all) 16 and 31, behind 2000 85 and 96.  More: 128 of
+// 64 (32768) 86 and 81, 656 and 652, 1024 of 4 with 40/1 heads (163840) behind 2000
+// 355 and 282.  More than a unit: 8 of 96 (384 of heads) 25.5 and 23.9, behind 4000
+// 122 and 97.
+constexpr int kChunkTreeUnit = 256, kChunkTreeAllRows = 16384;
 int tree_rows_of(int N, int max_rows) { return max_rows < N ? max_rows : N; }
 bool short_chunks(int dtype, int N, int rep, int max_rows) {
-  return dtype != HALO_F32 && (int64_t)tree_rows_of(N, max_rows) * rep <= kChunkTreeHeadRows;
+  const int64_t rows = (int64_t)tree_rows_of(N, max_rows) * rep;
+  return dtype != HALO_F32 &&
+         (rows <= kChunkTreeHeadRows || (rows <= kChunkTreeUnit && (int64_t)N * rep <= kChunkTreeAllRows));
 }
 
 }  // namespace

@@ -295,6 +295,20 @@ def test_batches_of_short_chunks(dev, dtype, H, Hk, most):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("H,Hk,B,most,trees", [(8, 2, 8, 48, True), (8, 2, 64, 64, True), (8, 2, 65, 64, False), (8, 2, 8, 65, False),
+                                               (28, 4, 9, 36, True), (28, 4, 70, 36, False), (8, 8, 3, 256, True)])
+def test_batches_of_up_to_a_unit(dev, dtype, H, Hk, B, most, trees):
+    """Around 256 rows of query heads a request, and 16384 in all."""
+    b = Batch(dev, lengths=[(k * 61) % 700 for k in range(B)], nodes=[most] * B, H=H, Hk=Hk, D=128, dtype=dtype, seed=B)
+    assert trees == (most * H // Hk <= 256 and B * most * H // Hk <= 16384)
+    got = b.run()
+    check(b, *got, b.exact())
+    if trees:
+        want = tree_launch.Batch.run(b)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("most", [1, 3, 512])
 def test_more_requests_than_a_plan_holds(dev, dtype, most):
