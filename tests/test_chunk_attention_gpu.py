@@ -405,3 +405,41 @@ def test_more_units_than_the_plan_keeps(dev):
     b = Batch(dev, lengths=[40, 500, 0, 9, 300], nodes=rows, H=40, Hk=1, D=64, dtype=F32, seed=11)
     assert sum(-(-n * 40 // 32) for n in rows) > 8192
     check(b, *b.run(), b.exact())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,most", [(60, 24), (4200, 3)])
+def test_short_chunks_padded_replayed_and_on_two_streams(dev, dtype, B, most):
+    """Batches that the tree kernels take: one graph for changing lengths and rows, padding rows left as they are, two calls at
+    once."""
+    lengths, rows = [(k * 31) % 90 for k in range(B)], [(k * 7) % (most + 1) for k in range(B)]
+    b = Batch(dev, lengths=lengths, nodes=rows, dtype=dtype, seed=B)
+    a, N = b.args, sum(rows)
+    pad = {**a, "q": torch.cat([a["q"], a["q"][:20]])}
+    b.args = pad
+    held = torch.full((N + 20, b.H, b.D), 9.0, dtype=dtype, device=dev)
+    held_lse = torch.full((N + 20, b.H), 7.0, device=dev)
+    b.run(max_rows=most)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run(max_rows=most, out=held, lse=held_lse)
+    for turn in range(3):
+        b.lengths = [(c + 13 * turn) % 90 for c in lengths]
+        b.nodes = rows[turn:] + rows[:turn]
+        a["lengths"].copy_(torch.tensor(b.lengths))
+        a["cu_nodes"].copy_(torch.tensor([0] + b.nodes).cumsum(0))
+        graph.replay()
+        eager = b.run(max_rows=most)
+        assert torch.equal(held[:N], eager[0][:N]) and torch.equal(held_lse[:N], eager[1][:N])
+        assert bool((held[N:] == 9).all()) and bool((held_lse[N:] == 7).all())
+        if turn != 1:
+            check(b, held[:N], held_lse[:N], b.exact())
+    other = Batch(dev, lengths=[9] * 40, nodes=[7] * 40, dtype=dtype, seed=1)
+    want = [b.run(max_rows=most), other.run()]
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [x.run(stream=t, max_rows=most if x is b else 7) for x, t in zip((b, other), s)]
+    torch.cuda.synchronize()
+    for g, w, n in zip(got, want, (N, 280)):
+        assert torch.equal(g[0][:n], w[0][:n]) and torch.equal(g[1][:n], w[1][:n])
